@@ -65,9 +65,28 @@ class GdrLayerIO(ctypes.Structure):
     ]
 
 
+class GdrLaParams(ctypes.Structure):
+    """``struct gdr_la_params`` of include/gdr.h."""
+
+    _fields_ = [(name, ctypes.c_int32) for name in (
+        "batch", "seq_len", "n_seqs", "heads_qk", "heads_v", "d_k", "d_v", "dtype", "algo",
+        "split_chunks")] + [("scale", ctypes.c_double)]
+
+
+class GdrQkNormRopeParams(ctypes.Structure):
+    """``struct gdr_qk_norm_rope_params`` of include/gdr.h."""
+
+    _fields_ = [(name, ctypes.c_int64) for name in (
+        "tokens", "q_token_stride", "q_head_stride", "k_token_stride", "k_head_stride")] + [
+        (name, ctypes.c_int32) for name in (
+            "heads_q", "heads_k", "head_dim", "rotary_dim", "table_rows", "interleaved",
+            "dtype")] + [("eps", ctypes.c_double)]
+
+
 _RULE_ARGS = [ctypes.POINTER(GdrParams), _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]
 _LAYER_ARGS = [ctypes.POINTER(GdrParams), _vp, _vp, _vp, _vp, _vp, ctypes.POINTER(GdrLayerIO),
                _vp, _vp, _vp, _vp, _vp]
+_LA_ARGS = [ctypes.POINTER(GdrLaParams), *[_vp] * 9]
 SIGNATURES = {
     "gdr_recurrent": (_i32, _RULE_ARGS),
     "gdr_chunked": (_i32, _RULE_ARGS),
@@ -90,6 +109,11 @@ SIGNATURES = {
                          _vp, _vp, _vp, _sz, _vp]),
     "gdr_mixed_noalloc": (_i32, [ctypes.POINTER(GdrParams), _vp, _vp, _vp, _vp, _vp, _vp, _vp,
                                  _i32, _vp, _vp, _vp]),
+    "gdr_la_recurrent": (_i32, _LA_ARGS),
+    "gdr_la_chunked": (_i32, _LA_ARGS),
+    "gdr_la_backward": (_i32, [ctypes.POINTER(GdrLaParams), *[_vp] * 13]),
+    "gdr_qk_norm_rope": (_i32, [ctypes.POINTER(GdrQkNormRopeParams), *[_vp] * 10]),
+    "gdr_qk_norm_rope_backward": (_i32, [ctypes.POINTER(GdrQkNormRopeParams), *[_vp] * 14]),
     "gdr_selftest_wait_timeout": (_i32, [ctypes.c_int64, _vp]),
     "gdr_release_scratch": (_i32, []),
     "gdr_device_error": (_i32, []),

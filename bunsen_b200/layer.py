@@ -6,7 +6,11 @@ libgdr's C ABI (include/gdr.h):
   with the layer's silu and its q / k / v channel split
   (``blocks/transformers/mixers/gated_delta_net.rs:396-420``);
 * ``gated_norm`` -- ``GatedNorm`` (``gated_delta_net.rs:439-440``) on its own;
-* ``state_reorder`` -- ``DeltaNetState::reorder`` (``state.rs:112-135``).
+* ``state_reorder`` -- ``DeltaNetState::reorder`` (``state.rs:112-135``);
+* ``qk_norm_rope`` and its gradient ``qk_norm_rope_backward`` -- the RMS norm of
+  every query and key head with the position rotation in the same pass, which
+  a mixer with norms on its heads (``LinearAttention``'s, or a softmax one) runs
+  on q and k before the rule.
 
 The gates and the gated norm run with the rule itself:
 ``GatedDeltaRule.chunked(..., gates=..., norm=...)``.
@@ -19,7 +23,7 @@ import ctypes
 import torch
 
 from . import _lib
-from .rule import _DTYPES, _ptr, _stream
+from .rule import _DTYPES, _ptr, _stream, on_device
 
 
 def causal_conv1d(x, weight, state=None, *, cu_seqlens=None, silu=False, splits=None,
@@ -103,3 +107,86 @@ def state_reorder(src, sources, out=None):
                                            rows, src.shape[0], row_bytes, _stream(src.device))
     _lib.check("gdr_state_reorder", status)
     return out
+
+
+def _rope_args(q, k, positions, cos, sin, q_weight, k_weight, eps, interleaved):
+    """The checks and the call's struct, the tensors it points at and the
+    leading shape of ``qk_norm_rope``."""
+    if q.dtype not in _DTYPES or k.dtype != q.dtype:
+        raise TypeError("q and k share one dtype, f32, bf16 or f16")
+    if q.dim() < 3 or k.dim() != q.dim() or k.shape[:-2] != q.shape[:-2] \
+            or k.shape[-1] != q.shape[-1]:
+        raise ValueError(f"q is [..., H_q, d] and k [..., H_k, d] with the same leading dims; got "
+                         f"{tuple(q.shape)} and {tuple(k.shape)}")
+    lead, d = q.shape[:-2], q.shape[-1]
+    if positions.shape != lead or positions.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"positions are int32 or int64 {tuple(lead)}, one for each token")
+    if cos.dim() != 2 or sin.shape != cos.shape or not 0 < 2 * cos.shape[1] <= d \
+            or cos.shape[0] == 0:
+        raise ValueError("cos and sin are [positions, rotary_dim / 2], rotary_dim at most d")
+    for w in (q_weight, k_weight):
+        if w is not None and tuple(w.shape) != (d,):
+            raise ValueError(f"the weights are [d] = ({d},)")
+    dev = q.device
+    if dev.type != "cuda":
+        raise RuntimeError("libgdr runs on CUDA tensors only")
+    for x in (k, positions, cos, sin, q_weight, k_weight):
+        if x is not None and x.device != dev:
+            raise ValueError(f"every tensor is on q's device {dev}; got one on {x.device}")
+    q, k = _token_rows(q), _token_rows(k)
+    if positions.dtype != torch.int32:  # far positions stay outside the tables
+        positions = positions.clamp(-1, 2**31 - 1).to(torch.int32)
+    positions = positions.contiguous()
+    cos, sin = cos.to(torch.float32).contiguous(), sin.to(torch.float32).contiguous()
+    q_weight, k_weight = (None if w is None else w.to(torch.float32).contiguous()
+                          for w in (q_weight, k_weight))
+    p = _lib.GdrQkNormRopeParams(
+        q.shape[0], q.stride(0), q.stride(1), k.stride(0), k.stride(1), q.shape[1], k.shape[1], d,
+        2 * cos.shape[1], cos.shape[0], int(interleaved), _DTYPES[q.dtype], float(eps))
+    return p, (q, k, positions, cos, sin, q_weight, k_weight), lead, dev
+
+
+def _token_rows(x):
+    """``[..., H, d]`` as ``[tokens, H, d]`` with contiguous features: a view
+    where the strides allow one (a part of a fused projection), else a copy."""
+    y = x if x.dim() == 3 else x.flatten(0, -3)
+    return y if y.stride(2) == 1 else y.contiguous()
+
+
+def qk_norm_rope(q, k, positions, cos, sin, q_weight=None, k_weight=None, eps=1e-6, *,
+                 interleaved=False):
+    """The RMS norm of every head vector of q ``[..., H_q, d]`` and k
+    ``[..., H_k, d]`` (weights ``[d]`` or None), then the rotation of its first
+    ``2 cos.shape[1]`` features by the angles of its token's position (cos and
+    sin f32 ``[positions, rotary_dim / 2]``, rows picked by ``positions``
+    ``[...]``): the pairs ``(i, i + rotary_dim / 2)``, or ``(2i, 2i + 1)`` when
+    ``interleaved``. One pass; q and k may be strided parts of one tensor.
+    Returns new contiguous ``(q, k)`` in q's dtype. A position outside the
+    tables leaves its rows unwritten; ``gdr_device_error`` reports it."""
+    p, x, lead, dev = _rope_args(q, k, positions, cos, sin, q_weight, k_weight, eps, interleaved)
+    q_out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    k_out = torch.empty(k.shape, dtype=k.dtype, device=dev)
+    on_device(dev, "gdr_qk_norm_rope", ctypes.byref(p), *(_ptr(t) for t in x), q_out.data_ptr(),
+              k_out.data_ptr())
+    return q_out, k_out
+
+
+def qk_norm_rope_backward(dq_out, dk_out, q, k, positions, cos, sin, q_weight=None, k_weight=None,
+                          eps=1e-6, *, interleaved=False):
+    """The gradients of ``qk_norm_rope`` from those of its outputs: ``(dq, dk,
+    dq_weight, dk_weight)``, dq and dk contiguous in q's dtype, the weights' in
+    f32 (None for a weight that is None), summed over all rows in a fixed order. A row
+    whose position is outside the tables is left unwritten and adds nothing."""
+    p, x, lead, dev = _rope_args(q, k, positions, cos, sin, q_weight, k_weight, eps, interleaved)
+    for g, y in ((dq_out, q), (dk_out, k)):
+        if g.shape != y.shape or g.dtype != y.dtype or g.device != dev:
+            raise ValueError("dq_out and dk_out are shaped, typed and placed like q and k")
+    dq_out, dk_out = dq_out.contiguous(), dk_out.contiguous()
+    dq = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    dk = torch.empty(k.shape, dtype=k.dtype, device=dev)
+    dw = [None if w is None else torch.empty(q.shape[-1], dtype=torch.float32, device=dev)
+          for w in (q_weight, k_weight)]
+    on_device(dev, "gdr_qk_norm_rope_backward", ctypes.byref(p), dq_out.data_ptr(),
+              dk_out.data_ptr(), *(_ptr(t) for t in x), dq.data_ptr(), dk.data_ptr(),
+              *(_ptr(w) for w in dw))
+    return dq, dk, dw[0], dw[1]

@@ -42,6 +42,17 @@ def _stream(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+def on_device(device: torch.device, fn: str, *args) -> None:
+    """Calls libgdr's ``fn`` with ``args`` and the current stream of ``device``,
+    with that device current (the library launches on the current one)."""
+    call = getattr(_lib.load(), fn)
+    if device.index == torch.cuda.current_device():
+        _lib.check(fn, call(*args, _stream(device)))
+    else:
+        with torch.cuda.device(device):
+            _lib.check(fn, call(*args, _stream(device)))
+
+
 def _layer_io(gates, norm, q, v, g, beta):
     """The ``gdr_layer_io`` of a call's ``gates=(a, b, a_log, dt_bias)`` and
     ``norm=(z, weight, eps)``, the tensors it points at (kept alive by the

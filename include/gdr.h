@@ -307,10 +307,102 @@ gdr_status gdr_mixed_noalloc(const gdr_params* params, const void* q, const void
                              const int32_t* state_slots, int32_t n_slots, void* out,
                              const int32_t* cu_seqlens, void* stream);
 
+/* ---- Linear attention with a decay for each head ---------------------------
+ * Beside the gated delta rule, for mixers whose state is decayed but not
+ * corrected: per (sequence, value head h), w = exp(log_decay[h]),
+ *   S_t = w S_{t-1} + k_t v_t^T        o_t = scale S_t^T q_t.
+ * Layouts, heads, dtypes, `state_in` / `state_out`, dense and packed batches
+ * are gdr_chunked's; log_decay is [H_v] f32 on the device, at most 0 (minus
+ * infinity: a position sees only itself), a constant without a gradient.
+ * dtypes f32, bf16 and f16; d_k and d_v up to 256 (else
+ * GDR_ERR_UNSUPPORTED). A sequence of length 0 passes its state through;
+ * positions behind the last sequence are neither read nor written. */
+typedef struct gdr_la_params {
+    int32_t batch;        /* B of a dense batch; ignored when cu_seqlens != NULL */
+    int32_t seq_len;      /* T of a dense batch, or T_total of a packed one      */
+    int32_t n_seqs;       /* sequences of a packed batch (cu_seqlens has +1)     */
+    int32_t heads_qk;     /* heads of q and k; divides heads_v                   */
+    int32_t heads_v;      /* heads of v and of the states                        */
+    int32_t d_k;
+    int32_t d_v;
+    int32_t dtype;        /* gdr_dtype of q, k, v, out and their gradients       */
+    int32_t algo;         /* gdr_algo, chunked and backward calls                */
+    int32_t split_chunks; /* segment length of a split call in chunks, 0: chosen */
+    double scale;         /* of the output; usually 1 / sqrt(d_k)                */
+} gdr_la_params;
+
+/* One position at a time: a decode step is a call with T = 1 (dense) or with
+ * every sequence of length 1 (packed). */
+gdr_status gdr_la_recurrent(const gdr_la_params* params, const void* q, const void* k,
+                            const void* v, const float* log_decay, const float* state_in,
+                            void* out, float* state_out, const int32_t* cu_seqlens, void* stream);
+
+/* A chunk at a time, for prompts. Agrees with gdr_la_recurrent up to rounding. */
+gdr_status gdr_la_chunked(const gdr_la_params* params, const void* q, const void* k, const void* v,
+                          const float* log_decay, const float* state_in, void* out,
+                          float* state_out, const int32_t* cu_seqlens, void* stream);
+
+/* The gradients of gdr_la_chunked (and of gdr_la_recurrent): from d_out
+ * (shaped and typed like out) and d_state_out (of the state after the last
+ * position; NULL: zeros), dq, dk, dv (shaped and typed like q, k, v) and
+ * d_state_in (f32; NULL: not wanted). state_in as in the forward call. The
+ * gradient of a key head is the sum over its value heads, in f32 and in a
+ * fixed order. Scratch (f32 [T, H_v, d_k] where key heads are shared) comes
+ * from the library's pool. No output may overlap an input. */
+gdr_status gdr_la_backward(const gdr_la_params* params, const void* q, const void* k,
+                           const void* v, const float* log_decay, const void* d_out,
+                           const float* state_in, const float* d_state_out, void* dq, void* dk,
+                           void* dv, float* d_state_in, const int32_t* cu_seqlens, void* stream);
+
+/* ---- Head norms with the position rotation ---------------------------------
+ * What a mixer runs on q and k before the rule: the RMS norm of every head
+ * vector (weight [d] f32, NULL: ones) and, in the same pass, the rotation of
+ * its first `rotary_dim` features by the angles of the token's position: with
+ * c, s = cos, sin[positions[token]], (y1, y2) = (n1 c - n2 s, n2 c + n1 s) over
+ * the pairs (i, i + rotary_dim / 2), or (2i, 2i + 1) when interleaved.
+ * q [tokens, heads_q, head_dim] and k [tokens, heads_k, head_dim] may be parts
+ * of a larger tensor: token and head strides are in elements, features are
+ * contiguous; outputs are contiguous and must not overlap inputs. cos and sin
+ * are f32 [table_rows, rotary_dim / 2]. A position outside the tables leaves
+ * its rows unwritten and is reported by gdr_device_error as GDR_ERR_INVALID.
+ * head_dim up to 256 (else GDR_ERR_UNSUPPORTED). */
+typedef struct gdr_qk_norm_rope_params {
+    int64_t tokens;
+    int64_t q_token_stride;
+    int64_t q_head_stride;
+    int64_t k_token_stride;
+    int64_t k_head_stride;
+    int32_t heads_q;
+    int32_t heads_k;
+    int32_t head_dim;
+    int32_t rotary_dim;  /* even, 2 to head_dim                                  */
+    int32_t table_rows;
+    int32_t interleaved;
+    int32_t dtype;       /* of q, k and their outputs: f32, bf16 or f16          */
+    double eps;
+} gdr_qk_norm_rope_params;
+
+gdr_status gdr_qk_norm_rope(const gdr_qk_norm_rope_params* params, const void* q, const void* k,
+                            const int32_t* positions, const float* cos, const float* sin,
+                            const float* q_weight, const float* k_weight, void* q_out,
+                            void* k_out, void* stream);
+
+/* Its gradients: dq, dk (contiguous) and the weights' gradients summed over
+ * all rows (f32 [head_dim]; NULL: not wanted; the sums' order is fixed) from
+ * dq_out, dk_out (contiguous). A row whose position is outside the tables adds
+ * nothing and leaves its gradient unwritten. Scratch for the sums comes from
+ * the library's pool. */
+gdr_status gdr_qk_norm_rope_backward(const gdr_qk_norm_rope_params* params, const void* dq_out,
+                                     const void* dk_out, const void* q, const void* k,
+                                     const int32_t* positions, const float* cos, const float* sin,
+                                     const float* q_weight, const float* k_weight, void* dq,
+                                     void* dk, float* dq_weight, float* dk_weight, void* stream);
+
 /* What the kernels of this library recorded on the device since the last
  * call (the record is then cleared): GDR_ERR_TIMEOUT if one gave up a bounded
  * wait, else GDR_ERR_INVALID if gdr_mixed met a state slot outside its pool,
- * else GDR_OK. Synchronous: waits for the device's outstanding work. */
+ * gdr_state_reorder a source row or gdr_qk_norm_rope a position outside its
+ * tables, else GDR_OK. Synchronous: waits for the device's outstanding work. */
 gdr_status gdr_device_error(void);
 
 /* A self-test of failure detection: launches one thread that waits, at most
