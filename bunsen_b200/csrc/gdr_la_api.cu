@@ -10,7 +10,10 @@ cudaError_t library_pool(cudaMemPool_t* pool, bool create);
 
 namespace {
 
-gdr_status la_status(cudaError_t e) { return e == cudaSuccess ? GDR_OK : GDR_ERR_CUDA; }
+gdr_status la_status(cudaError_t e) {
+    if (e == cudaErrorNotSupported) return GDR_ERR_UNSUPPORTED;  // run_core's: no such kernel
+    return e == cudaSuccess ? GDR_OK : GDR_ERR_CUDA;
+}
 
 // out[t, j, :] = the sum over a key head's `group` value heads of the f32
 // partials [T, heads, d], in head order, for the packed positions that belong
@@ -99,8 +102,10 @@ void operands(LaCore& p, const void* x, int hx, const void* y, int hy, const voi
 
 // The kernel that runs a core.
 cudaError_t run_core(const gdr_la_params& a, const LaCore& p, bool chunked, cudaStream_t s) {
-    (void)a;
-    (void)chunked;
+    if (!chunked || la_tokens(p) == 0) return launch_la_recurrent(p, s);
+    const bool tc = la_tc_supports(p);
+    if (!tc && a.algo >= GDR_ALGO_TENSOR) return cudaErrorNotSupported;
+    if (tc && a.algo != GDR_ALGO_CUDA_CORE) return launch_la_tc(p, s);
     return launch_la_recurrent(p, s);
 }
 

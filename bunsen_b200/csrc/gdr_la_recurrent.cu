@@ -41,7 +41,10 @@ la_recurrent(const LaCore p) {
     la_span(p, s, t0, t1);
     const int64_t hs = (static_cast<int64_t>(s) * p.heads + h) * p.d_b * p.d_c;
     const int64_t rs = p.state_t ? 1 : p.d_c, cs = p.state_t ? p.d_b : 1;  // state strides
-    const float w = expf(p.log_decay[h]);
+    // The decay in two parts: applied position after position, the rounding of
+    // one part would add up.
+    const double wd = exp(static_cast<double>(p.log_decay[h]));
+    const float w = static_cast<float>(wd), w_lo = static_cast<float>(wd - w);
 
     float st[kRows][kVec];
 #pragma unroll
@@ -94,10 +97,10 @@ la_recurrent(const LaCore p) {
             const float ar = ab[par][0][rg + kRG * r], br = ab[par][1][rg + kRG * r];
 #pragma unroll
             for (int v = 0; v < kVec; ++v) {
-                if (!p.reverse) st[r][v] *= w;
+                if (!p.reverse) st[r][v] = fmaf(st[r][v], w, st[r][v] * w_lo);
                 st[r][v] = fmaf(br, c[v], st[r][v]);
                 acc[v] = fmaf(ar, st[r][v], acc[v]);
-                if (p.reverse) st[r][v] *= w;
+                if (p.reverse) st[r][v] = fmaf(st[r][v], w, st[r][v] * w_lo);
             }
         }
 #pragma unroll
