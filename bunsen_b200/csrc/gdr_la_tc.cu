@@ -9,22 +9,28 @@
 // is 1 for any decay, minus infinity included.
 //
 // One CTA per SM, persistent over (sequence, head) items, warp-specialised, so
-// that the loads, the matrix products and the three conversions of
-// consecutive chunks run beside one another:
-//   warp 12      TMA loads of the a, b, c tiles, two stages of 96 KiB
-//   warp 13      issues every tcgen05.mma
+// that the loads, the matrix products and the conversions of consecutive
+// chunks run beside one another:
 //   warps 0-3    scores -> decayed bf16 P; the inter product's row scale; the
 //                output (converted, staged in the stage's a tile, TMA store)
-//   warps 4-7    the state: f32 in TMEM -> its bf16 copy in shared memory, and
-//                scaled by w^C in TMEM; initial and final states
-//   warps 8-11   the update's operand, c scaled by w^{C-1-j}
+//   warps 4-11   the state, f32 in registers (64 values a thread): adds a
+//                chunk's update, writes the bf16 copy; initial and final states
+//   warps 12-15  the update's operand, c scaled by w^{C-1-j}
+//   warp 16      TMA loads of the a, b, c tiles, two stages of 96 KiB
+//   warp 17      issues the products of the outputs
+//   warp 18      issues the products of the update
 // The products of a chunk, M = N = 128 each, f32 accumulators in TMEM:
 //   scores = A B^T              both from shared memory
 //   O      = A Sb               Sb the state's bf16 copy (K-major rows of c)
-//   S^T   += (w c)^T B          (w c)^T from TMEM, B read MN-major
 //   O     += P C                P from TMEM, C read MN-major
-// TMEM (512 columns): S^T 128, scores with P over them 128, O 128, (w c)^T two
+//   U^T    = (w c)^T B          (w c)^T from TMEM, B read MN-major
+// TMEM (512 columns): U^T 128, scores with P over them 128, O 128, (w c)^T two
 // buffers of 48 (32 positions in three parts).
+// Two issuing warps, because a wait and a commit cost their thread 100 to 200
+// cycles each beside products that keep shared memory busy, 17 of them a
+// chunk; the state in registers rather than scaled in TMEM, because there the
+// next update waited for the scaling (4.0 us a chunk with one issuer and the
+// state in TMEM, TIMEUS so).
 //
 // What is rounded: P and Sb to bf16 (2^-8 relative each, on disjoint parts of
 // an output, which is itself rounded to bf16: inputs are bf16, so another
@@ -54,18 +60,18 @@ namespace {
 using namespace sm100;
 
 constexpr int kC = 128, kD = 128;
-constexpr int kThreads = 448;
+constexpr int kThreads = 608;
 constexpr uint32_t kTile = 32768;         // 128 positions x 128 bf16, two 64-wide halves
 constexpr uint32_t kHalf = kTile / 2;
 constexpr uint32_t kStage = 3 * kTile;    // a, b, c
 constexpr uint32_t kOffSb = 2 * kStage, kOffMisc = kOffSb + kTile;
 constexpr uint32_t kSmemBytes = kOffMisc + 2048 + 1024;  // + alignment slack
-constexpr uint32_t kColS = 0, kColP = 128, kColO = 256, kColW = 384, kColWBuf = 48;
+constexpr uint32_t kColU = 0, kColP = 128, kColO = 256, kColW = 384, kColWBuf = 48;
 constexpr uint64_t kWaitLimitNs = 2000000000ull;
 
 struct Bars {
     uint64_t full[2], kv_free[2], q_free[2];
-    uint64_t sc_full, in_full, o_full, o_free, pa_ready, st_ready, st_full, fix, drain;
+    uint64_t sc_full, in_full, o_full, o_free, pa_ready, sb_ready, u_full, u_free, fix[2], drain[2];
     uint64_t wv_full[2], wv_free[2];
     uint32_t tmem;
 };
@@ -113,6 +119,29 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16
         : "memory");
 }
 
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, float (&v)[16]) {
+    uint32_t r[16];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32"
+        " {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+          "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]),
+          "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+// 16 lanes x 16 columns: thread t's register 2 i holds lane t / 4, column 4 i +
+// t % 4, and register 2 i + 1 the lane 8 below it.
+__device__ __forceinline__ void tmem_st_16x128(uint32_t taddr, const uint32_t (&v)[8]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.16x128b.x4.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(
+            taddr),
+        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+        : "memory");
+}
+
 // D[tmem] = A[tmem] B (+ D): A's rows are the lanes, K pairs its columns.
 __device__ __forceinline__ void umma_bf16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc,
                                              uint32_t idesc, uint32_t accumulate) {
@@ -133,35 +162,74 @@ __device__ __forceinline__ uint32_t pack_bf16(float x, float y) {
 __device__ __forceinline__ float low_f32(uint32_t p) { return __uint_as_float(p << 16); }
 __device__ __forceinline__ float high_f32(uint32_t p) { return __uint_as_float(p & 0xffff0000u); }
 
-// w^n to f32 accuracy (the exponent in f64), 1 for n = 0.
-__device__ __forceinline__ double power(double g, int n) { return n <= 0 ? 1.0 : exp(g * n); }
+// Pairs of f32 in one 64-bit register: one instruction for two products or sums.
+__device__ __forceinline__ uint64_t pair(float x, float y) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+    return r;
+}
+__device__ __forceinline__ void unpair(uint64_t p, float& x, float& y) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(p));
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint32_t pack_bf16(uint64_t p) {
+    float x, y;
+    unpair(p, x, y);
+    return pack_bf16(x, y);
+}
+__device__ __forceinline__ uint64_t widen(uint32_t p) { return pair(low_f32(p), high_f32(p)); }
 
-__device__ __forceinline__ Item item_of(const LaCore& p, int64_t id) {
+// w^n for 0 <= n <= 128, 1 for n = 0 (minus infinity included): the exponent's
+// rounding error goes in as a factor, e^(p + d) = e^p (1 + d).
+__device__ __forceinline__ float power(float g, int n) {
+    if (n <= 0) return 1.f;
+    const float p = g * n;
+    if (p < -104.f) return 0.f;  // below the smallest f32
+    const float e = expf(p);
+    return fmaf(e, fmaf(g, static_cast<float>(n), -p), e);
+}
+
+__device__ __forceinline__ Item item_of(const LaCore& p, int id) {
     Item it;
-    const int s = static_cast<int>(id / p.heads);
-    it.h = static_cast<int>(id - static_cast<int64_t>(s) * p.heads);
+    const int s = id / p.heads;
+    it.h = id - s * p.heads;
     int64_t end;
     la_span(p, s, it.start, end);
     it.len = static_cast<int>(end - it.start);
-    const int64_t at = id * p.d_b * p.d_c;
+    const int64_t at = static_cast<int64_t>(id) * p.d_b * p.d_c;
     it.in = p.state_in != nullptr ? p.state_in + at : nullptr;
     it.out = p.state_out != nullptr ? p.state_out + at : nullptr;
     it.in_t = it.out_t = p.state_t != 0;
     return it;
 }
 
-// Chunk c of an item, in the order they run.
-__device__ __forceinline__ void chunk_of(const LaCore& p, const Item& it, int nch, int c,
+// Chunk c of an item, in the order they run: its length, and its first row.
+template <bool kRev>
+__device__ __forceinline__ int chunk_len(const Item& it, int nch, int c) {
+    return min(kC, it.len - (kRev ? nch - 1 - c : c) * kC);
+}
+template <bool kRev>
+__device__ __forceinline__ void chunk_of(const Item& it, int nch, int c,
                                          int64_t& row, int& len) {
-    const int x = p.reverse ? nch - 1 - c : c;
+    const int x = kRev ? nch - 1 - c : c;
     row = it.start + static_cast<int64_t>(x) * kC;
     len = min(kC, it.len - x * kC);
 }
 
+template <bool kRev>
 __global__ void __launch_bounds__(kThreads, 1)
 la_tc(const LaCore p, const __grid_constant__ CUtensorMap ma,
       const __grid_constant__ CUtensorMap mb, const __grid_constant__ CUtensorMap mc,
-      const __grid_constant__ CUtensorMap mo, int64_t items) {
+      const __grid_constant__ CUtensorMap mo, int items) {
     extern __shared__ uint8_t raw[];
     uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
@@ -171,7 +239,9 @@ la_tc(const LaCore p, const __grid_constant__ CUtensorMap ma,
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) {
             mbar_init(&B.full[i], 1);
-            mbar_init(&B.kv_free[i], 1);
+            mbar_init(&B.kv_free[i], 2);
+            mbar_init(&B.drain[i], 1);
+            mbar_init(&B.fix[i], 4);
             mbar_init(&B.q_free[i], 4);
             mbar_init(&B.wv_full[i], 4);
             mbar_init(&B.wv_free[i], 1);
@@ -181,13 +251,12 @@ la_tc(const LaCore p, const __grid_constant__ CUtensorMap ma,
         mbar_init(&B.o_full, 1);
         mbar_init(&B.o_free, 4);
         mbar_init(&B.pa_ready, 4);
-        mbar_init(&B.st_ready, 4);
-        mbar_init(&B.st_full, 1);
-        mbar_init(&B.fix, 4);
-        mbar_init(&B.drain, 1);
+        mbar_init(&B.sb_ready, 8);
+        mbar_init(&B.u_full, 1);
+        mbar_init(&B.u_free, 8);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 13) {
+    if (warp == 18) {
         tmem_alloc(&B.tmem, 512);
         tmem_relinquish();
     }
@@ -197,12 +266,12 @@ la_tc(const LaCore p, const __grid_constant__ CUtensorMap ma,
     const uint32_t tm = B.tmem;
     const uint32_t quad = tm + (static_cast<uint32_t>(warp & 3) << 21);  // this warp's lanes
 
-    if (warp == 12) {
+    if (warp == 16) {
         // ---- loads -------------------------------------------------------------
         if (lane == 0) {
             uint32_t n = 0;
             bool ok = true;
-            for (int64_t id = blockIdx.x; ok && id < items; id += gridDim.x) {
+            for (int id = blockIdx.x; ok && id < items; id += gridDim.x) {
                 const Item it = item_of(p, id);
                 const int nch = (it.len + kC - 1) / kC;
                 const int ha = it.h / (p.heads / p.heads_a), hb = it.h / (p.heads / p.heads_b),
@@ -212,7 +281,7 @@ la_tc(const LaCore p, const __grid_constant__ CUtensorMap ma,
                     const uint32_t ph = ((n >> 1) & 1) ^ 1;
                     int64_t row;
                     int len;
-                    chunk_of(p, it, nch, c, row, len);
+                    chunk_of<kRev>(it, nch, c, row, len);
                     uint8_t* base = sm + st * kStage;
                     if (n >= 2 && !(ok = lane_wait(&B.kv_free[st], ph))) break;
                     mbar_expect_tx(&B.full[st], kStage);
@@ -231,109 +300,147 @@ la_tc(const LaCore p, const __grid_constant__ CUtensorMap ma,
                 lane_wait(&B.full[i & 1], (i >> 1) & 1);
         }
         __syncwarp();
-    } else if (warp == 13) {
-        // ---- products ------------------------------------------------------------
+    } else if (warp == 17) {
+        // ---- the outputs' products -------------------------------------------------
         if (lane == 0) {
             constexpr uint32_t kKK = idesc_bf16(128, 128, 0, 0, 0);
             constexpr uint32_t kKMn = idesc_bf16(128, 128, 0, 1, 0);
-            const uint32_t sb = smem_u32(sm + kOffSb);
-            uint32_t n = 0, w = 0, tails = 0;
+            const uint64_t tile0 = sdesc_sw128(smem_u32(sm), 16, 1024);
+            const uint64_t sb = sdesc_sw128(smem_u32(sm + kOffSb), 16, 1024);
+            const uint64_t mn0 = sdesc_sw128(smem_u32(sm), kHalf, 1024);
+            uint32_t n = 0, tails = 0;
             bool ok = true;
-            for (int64_t id = blockIdx.x; ok && id < items; id += gridDim.x) {
+            for (int id = blockIdx.x; ok && id < items; id += gridDim.x) {
                 const Item it = item_of(p, id);
                 const int nch = (it.len + kC - 1) / kC;
                 for (int c = 0; c < nch; ++c, ++n) {
-                    const int st = n & 1;
-                    const uint32_t ph = n & 1;
-                    int64_t row;
-                    int len;
-                    chunk_of(p, it, nch, c, row, len);
-                    const uint32_t a = smem_u32(sm + st * kStage), b = a + kTile, v = b + kTile;
+                    const uint32_t st = n & 1, ph = n & 1;
+                    const uint64_t a = tile0 + st * (kStage >> 4), bt = a + (kTile >> 4);
                     if (!(ok = lane_wait(&B.full[st], (n >> 1) & 1))) break;
-                    if (len < kC && !(ok = lane_wait(&B.fix, tails++ & 1))) break;
+                    if (chunk_len<kRev>(it, nch, c) < kC) {  // (by stage: bits of `tails`)
+                        if (!(ok = lane_wait(&B.fix[st], (tails >> st) & 1))) break;
+                        tails ^= 1u << st;
+                    }
                     tc_fence_after();
-#pragma unroll
-                    for (int k = 0; k < 8; ++k) {
-                        const uint32_t off = (k >> 2) * kHalf + (k & 3) * 32;
-                        umma_bf16(tm + kColP, sdesc_sw128(a + off, 16, 1024),
-                                  sdesc_sw128(b + off, 16, 1024), kKK, k > 0);
+#pragma unroll 1
+                    for (uint32_t k = 0; k < 8; ++k) {
+                        const uint32_t off = ((k >> 2) * kHalf + (k & 3) * 32) >> 4;
+                        umma_bf16(tm + kColP, a + off, bt + off, kKK, k);
                     }
                     umma_commit(&B.sc_full);
-                    if (!(ok = lane_wait(&B.st_ready, ph))) break;
+                    if (!(ok = lane_wait(&B.sb_ready, ph))) break;
                     if (n > 0 && !(ok = lane_wait(&B.o_free, ph ^ 1))) break;
                     tc_fence_after();
-#pragma unroll
-                    for (int k = 0; k < 8; ++k) {
-                        const uint32_t off = (k >> 2) * kHalf + (k & 3) * 32;
-                        umma_bf16(tm + kColO, sdesc_sw128(a + off, 16, 1024),
-                                  sdesc_sw128(sb + off, 16, 1024), kKK, k > 0);
+#pragma unroll 1
+                    for (uint32_t k = 0; k < 8; ++k) {
+                        const uint32_t off = ((k >> 2) * kHalf + (k & 3) * 32) >> 4;
+                        umma_bf16(tm + kColO, a + off, sb + off, kKK, k);
                     }
                     umma_commit(&B.in_full);
-                    for (int q = 0; ok && q < 4; ++q, ++w) {
-                        const int buf = w & 1;
-                        if (!(ok = lane_wait(&B.wv_full[buf], (w >> 1) & 1))) break;
-                        tc_fence_after();
-#pragma unroll
-                        for (int k = 0; k < 2; ++k) {
-                            const uint64_t d = sdesc_sw128(b + (32 * q + 16 * k) * 128, kHalf, 1024);
-#pragma unroll
-                            for (int t = 0; t < 3; ++t)
-                                umma_bf16_ts(tm + kColS, tm + kColW + buf * kColWBuf + 16 * t + 8 * k,
-                                             d, kKMn, 1);
-                        }
-                        umma_commit(&B.wv_free[buf]);
-                    }
-                    if (!ok) break;
-                    umma_commit(&B.st_full);
                     if (!(ok = lane_wait(&B.pa_ready, ph))) break;
                     tc_fence_after();
-#pragma unroll
-                    for (int k = 0; k < 8; ++k)
-                        umma_bf16_ts(tm + kColO, tm + kColP + 8 * k,
-                                     sdesc_sw128(v + 16 * k * 128, kHalf, 1024), kKMn, 1);
+                    const uint64_t v = mn0 + ((st * kStage + 2 * kTile) >> 4);
+#pragma unroll 1
+                    for (uint32_t k = 0; k < 8; ++k)
+                        umma_bf16_ts(tm + kColO, tm + kColP + 8 * k, v + k * (2048 >> 4), kKMn, 1);
                     umma_commit(&B.o_full);
                     umma_commit(&B.kv_free[st]);
                 }
             }
-            umma_commit(&B.drain);
-            lane_wait(&B.drain, 0);
+            umma_commit(&B.drain[0]);
+            lane_wait(&B.drain[0], 0);
+        }
+        __syncwarp();
+    } else if (warp == 18) {
+        // ---- the update's products -------------------------------------------------
+        if (lane == 0) {
+            constexpr uint32_t kKMn = idesc_bf16(128, 128, 0, 1, 0);
+            const uint64_t mn0 = sdesc_sw128(smem_u32(sm) + kTile, kHalf, 1024);
+            uint32_t n = 0, w = 0, tails = 0;
+            bool ok = true;
+            for (int id = blockIdx.x; ok && id < items; id += gridDim.x) {
+                const Item it = item_of(p, id);
+                const int nch = (it.len + kC - 1) / kC;
+                for (int c = 0; c < nch; ++c, ++n) {
+                    const uint32_t st = n & 1;
+                    const uint64_t bt = mn0 + st * (kStage >> 4);
+                    if (!(ok = lane_wait(&B.full[st], (n >> 1) & 1))) break;
+                    if (chunk_len<kRev>(it, nch, c) < kC) {  // (by stage: bits of `tails`)
+                        if (!(ok = lane_wait(&B.fix[st], (tails >> st) & 1))) break;
+                        tails ^= 1u << st;
+                    }
+                    if (n > 0 && !(ok = lane_wait(&B.u_free, (n & 1) ^ 1))) break;
+                    for (uint32_t q = 0; q < 4; ++q, ++w) {
+                        const uint32_t buf = w & 1;
+                        if (!(ok = lane_wait(&B.wv_full[buf], (w >> 1) & 1))) break;
+                        tc_fence_after();
+                        const uint32_t op = tm + kColW + buf * kColWBuf;
+#pragma unroll 1
+                        for (uint32_t k = 0; k < 2; ++k) {
+                            const uint64_t d = bt + (2 * q + k) * (2048 >> 4);
+#pragma unroll
+                            for (uint32_t t = 0; t < 3; ++t)
+                                umma_bf16_ts(tm + kColU, op + 16 * t + 8 * k, d, kKMn, q | k | t);
+                        }
+                        umma_commit(&B.wv_free[buf]);
+                    }
+                    if (!ok) break;
+                    umma_commit(&B.u_full);
+                    umma_commit(&B.kv_free[st]);
+                }
+            }
+            umma_commit(&B.drain[1]);
+            lane_wait(&B.drain[1], 0);
         }
         __syncwarp();
     } else if (warp < 4) {
         // ---- scores, outputs -------------------------------------------------------
-        float* tab = tables + 32 * warp;  // w^n, n < 32
-        const int i = 32 * warp + lane;   // this thread's row of the chunk
+        // Where w^-128 is far from overflow, the powers come out of the sums:
+        //   out_i = tau w^{i+1} [ a_i . S + sum_{j<=i} sigma w^{-(j+1)} (a_i.b_j) c_j ]
+        // (backward w^{len-1-i} and w^{-(len-1-j)}): one column factor on the
+        // scores, one row factor on the output, the inter product untouched. Each row's
+        // terms keep their ratios, so no bits are lost. Steeper heads scale scores by
+        // w^{i-j} and the inter product by rows, a pass over O more.
+        float* tab = tables + 32 * warp;
+        const int i = 32 * warp + lane;  // this thread's row of the chunk
+        const float both = p.sigma * p.tau;
         uint32_t n = 0;
         bool ok = true, pending = false;
         int pending_st = 0;
-        for (int64_t id = blockIdx.x; ok && id < items; id += gridDim.x) {
+        for (int id = blockIdx.x; ok && id < items; id += gridDim.x) {
             const Item it = item_of(p, id);
             const int nch = (it.len + kC - 1) / kC;
-            const double g = p.log_decay[it.h];
+            const float g = p.log_decay[it.h];
+            const bool gentle = g >= -0.4f && g <= 0.4f;
             __syncwarp();
-            tab[lane] = static_cast<float>(power(g, lane));
+            tab[lane] = gentle ? power(-g, kRev ? 31 - lane : lane + 1) : power(g, lane);
             __syncwarp();
-            // Off the diagonal block the exponent splits in two that are not
-            // negative: (row part, 32 m) and the column's, from the table.
-            const float edge = static_cast<float>(power(g, p.reverse ? 32 - lane : lane + 1));
-            const float w32 = static_cast<float>(power(g, 32)), w64 = static_cast<float>(power(g, 64));
-            float ahead = 0.f;  // the inter product's row scale
-            int known = 0;      // the chunk length it is for
+            // Steep heads, off the diagonal block: the exponent splits in two
+            // that are not negative, (row part, 32 m) and the column's, from the table.
+            const float edge = power(g, kRev ? 32 - lane : lane + 1) * both;
+            const float w32 = power(g, 32), w64 = power(g, 64);
+            float ahead = 0.f, fb[4];  // row factor; gentle heads' column factor by block
+            int known = 0;             // the chunk length they are for
             for (int c = 0; c < nch; ++c, ++n) {
                 const uint32_t ph = n & 1;
                 const int st = n & 1;
                 int64_t row;
                 int len;
-                chunk_of(p, it, nch, c, row, len);
+                chunk_of<kRev>(it, nch, c, row, len);
                 if (len != known) {
-                    ahead = static_cast<float>(power(g, p.reverse ? max(len - 1 - i, 0) : i + 1));
+                    ahead = power(g, kRev ? max(len - 1 - i, 0) : i + 1) * p.tau;
+#pragma unroll
+                    for (int cb = 0; cb < 4; ++cb) {
+                        const int e = kRev ? len - 32 - 32 * cb : 32 * cb;
+                        fb[cb] = p.sigma * (e < 0 ? power(g, -e) : power(-g, e));
+                    }
                     known = len;
                 }
                 if (!(ok = warp_wait(&B.sc_full, ph))) break;
                 tc_fence_after();
 #pragma unroll 1
                 for (int cb = 0; cb < 4; ++cb) {
-                    const int apart = p.reverse ? cb - warp : warp - cb;  // blocks apart
+                    const int apart = kRev ? cb - warp : warp - cb;  // blocks apart
                     uint32_t packed[16];
                     if (apart < 0) {
 #pragma unroll
@@ -341,28 +448,45 @@ la_tc(const LaCore p, const __grid_constant__ CUtensorMap ma,
                     } else {
                         float s[32];
                         tmem_ld32(quad + kColP + 32 * cb, s);
+                        float f = cb < 2 ? (cb == 0 ? fb[0] : fb[1]) : (cb == 2 ? fb[2] : fb[3]);
+                        if (!gentle) f = edge * (apart <= 1 ? 1.f : apart == 2 ? w32 : w64);
+                        const uint64_t f2 = pair(f, f);
                         tmem_wait_ld();
-                        if (apart > 0) {
-                            const float f = p.sigma * edge *
-                                            (apart == 1 ? 1.f : apart == 2 ? w32 : w64);
+                        if (gentle || apart > 0) {
 #pragma unroll
                             for (int j4 = 0; j4 < 8; ++j4) {
-                                const float4 x = reinterpret_cast<const float4*>(
-                                    tab)[p.reverse ? j4 : 7 - j4];
-                                const float y[4] = {p.reverse ? x.x : x.w, p.reverse ? x.y : x.z,
-                                                    p.reverse ? x.z : x.y, p.reverse ? x.w : x.x};
-#pragma unroll
-                                for (int j = 0; j < 4; ++j) s[4 * j4 + j] *= f * y[j];
+                                // Steep heads take the table backwards when forward in time.
+                                float4 x;
+                                if (kRev || gentle) {
+                                    x = reinterpret_cast<const float4*>(tab)[j4];
+                                } else {
+                                    const float4 y = reinterpret_cast<const float4*>(tab)[7 - j4];
+                                    x = make_float4(y.w, y.z, y.y, y.x);
+                                }
+                                packed[2 * j4] =
+                                    pack_bf16(mul2(pair(s[4 * j4], s[4 * j4 + 1]),
+                                                   mul2(f2, pair(x.x, x.y))));
+                                packed[2 * j4 + 1] =
+                                    pack_bf16(mul2(pair(s[4 * j4 + 2], s[4 * j4 + 3]),
+                                                   mul2(f2, pair(x.z, x.w))));
                             }
                         } else {
 #pragma unroll
-                            for (int j = 0; j < 32; ++j) {
-                                const int e = p.reverse ? j - lane : lane - j;
-                                s[j] = e >= 0 ? s[j] * (p.sigma * tab[e & 31]) : 0.f;
+                            for (int j = 0; j < 16; ++j) {
+                                const int e = kRev ? 2 * j - lane : lane - 2 * j;
+                                packed[j] = pack_bf16(
+                                    s[2 * j] * (both * tab[e & 31]),
+                                    s[2 * j + 1] * (both * tab[(kRev ? e + 1 : e - 1) & 31]));
                             }
                         }
+                        if (apart == 0) {  // the diagonal block: j <= i, or j >= i
 #pragma unroll
-                        for (int j = 0; j < 16; ++j) packed[j] = pack_bf16(s[2 * j], s[2 * j + 1]);
+                            for (int j = 0; j < 16; ++j) {
+                                const bool k0 = kRev ? 2 * j >= lane : 2 * j <= lane;
+                                const bool k1 = kRev ? 2 * j + 1 >= lane : 2 * j + 1 <= lane;
+                                packed[j] &= (k0 ? 0xffffu : 0u) | (k1 ? 0xffff0000u : 0u);
+                            }
+                        }
                     }
                     tmem_st16(quad + kColP + 16 * cb, packed);
                 }
@@ -373,16 +497,18 @@ la_tc(const LaCore p, const __grid_constant__ CUtensorMap ma,
                     }
                     pending = false;
                 }
-                if (!(ok = warp_wait(&B.in_full, ph))) break;
-                tc_fence_after();
+                if (!gentle) {
+                    if (!(ok = warp_wait(&B.in_full, ph))) break;
+                    tc_fence_after();
 #pragma unroll 1
-                for (int cb = 0; cb < 4; ++cb) {
-                    float s[32];
-                    tmem_ld32(quad + kColO + 32 * cb, s);
-                    tmem_wait_ld();
+                    for (int cb = 0; cb < 4; ++cb) {
+                        float s[32];
+                        tmem_ld32(quad + kColO + 32 * cb, s);
+                        tmem_wait_ld();
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) s[j] *= ahead;
-                    tmem_st32(quad + kColO + 32 * cb, s);
+                        for (int j = 0; j < 32; ++j) s[j] *= ahead;
+                        tmem_st32(quad + kColO + 32 * cb, s);
+                    }
                 }
                 tmem_wait_st();
                 tc_fence_before();
@@ -392,21 +518,23 @@ la_tc(const LaCore p, const __grid_constant__ CUtensorMap ma,
                 tc_fence_after();
                 uint8_t* tile = sm + st * kStage;  // a's, read by now
                 const int live = min(max(len - 32 * warp, 0), 32);
-                const int64_t orow = (row + i) * p.heads + it.h;
+                const float scale = gentle ? ahead : 1.f;
+                const uint64_t scale2 = pair(scale, scale);
+                float* out32 = static_cast<float*>(p.out) + ((row + i) * p.heads + it.h) * p.d_c;
 #pragma unroll 1
                 for (int cb = 0; cb < 4; ++cb) {
                     float s[32];
                     tmem_ld32(quad + kColO + 32 * cb, s);
                     tmem_wait_ld();
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) s[j] *= p.tau;
+                    for (int j = 0; j < 32; j += 2)
+                        unpair(mul2(pair(s[j], s[j + 1]), scale2), s[j], s[j + 1]);
                     if (p.out_f32) {
-                        float* o = static_cast<float*>(p.out) + orow * p.d_c + 32 * cb;
                         if (lane < live)
 #pragma unroll
                             for (int j = 0; j < 8; ++j)
                                 if (32 * cb + 4 * j < p.d_c)
-                                    reinterpret_cast<float4*>(o)[j] = make_float4(
+                                    reinterpret_cast<float4*>(out32 + 32 * cb)[j] = make_float4(
                                         s[4 * j], s[4 * j + 1], s[4 * j + 2], s[4 * j + 3]);
                     } else {
                         uint8_t* dst = tile + (cb >> 1) * kHalf + i * 128;
@@ -458,174 +586,178 @@ la_tc(const LaCore p, const __grid_constant__ CUtensorMap ma,
         }
         if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
         if (pending && lane == 0) mbar_arrive(&B.q_free[pending_st]);
-    } else if (warp < 8) {
+    } else if (warp < 12) {
         // ---- the state -----------------------------------------------------------
-        const int col = 32 * (warp - 4) + lane;  // this thread's column of S (row of S^T)
-        uint8_t* sb = sm + kOffSb + col * 128;
-        uint32_t n = 0;
+        const int col = 32 * (warp & 3) + lane;  // this thread's column of S (row of U^T),
+        const int half = (warp - 4) >> 2, b0 = 64 * half;  // and its rows b0 .. b0 + 63
+        uint8_t* sb = sm + kOffSb + half * kHalf + col * 128;
+        uint32_t n = 0;  // chunks begun
         bool ok = true;
-        for (int64_t id = blockIdx.x; ok && id < items; id += gridDim.x) {
+        float s[64];
+        for (int id = blockIdx.x; ok && id < items; id += gridDim.x) {
             const Item it = item_of(p, id);
             const int nch = (it.len + kC - 1) / kC;
-            const double g = p.log_decay[it.h];
-            const int rs_in = it.in_t ? 1 : p.d_c, rs_out = it.out_t ? 1 : p.d_c;
-            const float* src = it.in ? it.in + (it.in_t ? col * p.d_b : col) : nullptr;
-            float* dst = it.out ? it.out + (it.out_t ? col * p.d_b : col) : nullptr;
-            float hi = 1.f, lo = 0.f;  // w^len, in two parts: it is applied every chunk
-            int known = 0;             // the chunk length they are for
-            for (int c = 0; c <= nch; ++c) {
-                if (c < nch) {
-                    int64_t row;
-                    int len;
-                    chunk_of(p, it, nch, c, row, len);
-                    if (len != known) {
-                        const double f = power(g, len);
-                        hi = static_cast<float>(f);
-                        lo = static_cast<float>(f - hi);
-                        known = len;
-                    }
-                }
-                if (c > 0) {
-                    if (!(ok = warp_wait(&B.st_full, (n - 1) & 1))) break;
-                    tc_fence_after();
-                }
-                const bool last = c == nch;
-#pragma unroll 1
-                for (int blk = 0; blk < 4; ++blk) {
-                    float s[32];
-                    if (c > 0) {
-                        tmem_ld32(quad + kColS + 32 * blk, s);
-                        tmem_wait_ld();
-                    } else {
+            const float g = p.log_decay[it.h];
+            const int64_t rs_in = it.in_t ? 1 : p.d_c, rs_out = it.out_t ? 1 : p.d_c;
+            const bool mine = col < p.d_c;
+            if (it.in != nullptr && mine) {
+                const float* src = it.in + (it.in_t ? col * p.d_b : col) + b0 * rs_in;
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) {
-                            const int b = 32 * blk + j;
-                            s[j] = src != nullptr && col < p.d_c && b < p.d_b
-                                       ? src[static_cast<int64_t>(b) * rs_in]
-                                       : 0.f;
-                        }
-                    }
-                    if (last) {
-                        if (dst != nullptr && col < p.d_c)
+                for (int j = 0; j < 64; ++j, src += rs_in) s[j] = b0 + j < p.d_b ? *src : 0.f;
+            } else {
 #pragma unroll
-                            for (int j = 0; j < 32; ++j) {
-                                const int b = 32 * blk + j;
-                                if (b < p.d_b) dst[static_cast<int64_t>(b) * rs_out] = s[j];
-                            }
-                        continue;
-                    }
+                for (int j = 0; j < 64; ++j) s[j] = 0.f;
+            }
+            // w^len in two parts: it is applied chunk after chunk.
+            uint64_t hi2 = 0, lo2 = 0;
+            int known = 0;
+            for (int c = 0; c < nch; ++c, ++n) {
+                // Sb, once the last chunk's product has read its own.
+                if (n > 0 && !(ok = warp_wait(&B.in_full, (n - 1) & 1))) break;
 #pragma unroll
-                    for (int m = 0; m < 4; ++m)
-                        *reinterpret_cast<uint4*>(sb + (blk >> 1) * kHalf +
-                                                  ((((blk & 1) * 4 + m) ^ (col & 7)) << 4)) =
-                            make_uint4(pack_bf16(s[8 * m], s[8 * m + 1]),
-                                       pack_bf16(s[8 * m + 2], s[8 * m + 3]),
-                                       pack_bf16(s[8 * m + 4], s[8 * m + 5]),
-                                       pack_bf16(s[8 * m + 6], s[8 * m + 7]));
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) s[j] = fmaf(s[j], hi, s[j] * lo);
-                    tmem_st32(quad + kColS + 32 * blk, s);
-                }
-                if (last) {
-                    tc_fence_before();
-                    break;
-                }
-                tmem_wait_st();
+                for (int m = 0; m < 8; ++m)
+                    *reinterpret_cast<uint4*>(sb + ((m ^ (col & 7)) << 4)) =
+                        make_uint4(pack_bf16(s[8 * m], s[8 * m + 1]),
+                                   pack_bf16(s[8 * m + 2], s[8 * m + 3]),
+                                   pack_bf16(s[8 * m + 4], s[8 * m + 5]),
+                                   pack_bf16(s[8 * m + 6], s[8 * m + 7]));
                 fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&B.sb_ready);
+                const int len = chunk_len<kRev>(it, nch, c);
+                if (len != known) {
+                    const double f = exp(static_cast<double>(g) * len);
+                    const float hi = static_cast<float>(f), lo = static_cast<float>(f - hi);
+                    hi2 = pair(hi, hi);
+                    lo2 = pair(lo, lo);
+                    known = len;
+                }
+                if (!(ok = warp_wait(&B.u_full, n & 1))) break;
+                tc_fence_after();
+#pragma unroll
+                for (int blk = 0; blk < 4; ++blk) {
+                    float u[16];
+                    tmem_ld16(quad + kColU + b0 + 16 * blk, u);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int j = 0; j < 16; j += 2) {
+                        const uint64_t x = pair(s[16 * blk + j], s[16 * blk + j + 1]);
+                        unpair(fma2(x, hi2, fma2(x, lo2, pair(u[j], u[j + 1]))), s[16 * blk + j],
+                               s[16 * blk + j + 1]);
+                    }
+                }
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&B.st_ready);
-                ++n;
+                if (lane == 0) mbar_arrive(&B.u_free);
+            }
+            if (ok && it.out != nullptr && mine) {
+                float* dst = it.out + (it.out_t ? col * p.d_b : col) + b0 * rs_out;
+#pragma unroll
+                for (int j = 0; j < 64; ++j, dst += rs_out)
+                    if (b0 + j < p.d_b) *dst = s[j];
             }
         }
     } else {
         // ---- the update's operand ----------------------------------------------------
-        float* tab = tables + 32 * (warp - 4);
-        const int col = 32 * (warp - 8) + lane;  // this thread's feature of c
-        const int cx = ((col & 63) >> 3) << 4, cy = (col >> 6) * kHalf + (col & 7) * 2;
+        // (w c)^T, features on the TMEM lanes: 8 x 8 blocks of the c tile come
+        // transposed from ldmatrix, thread t holding feature t / 4 (and + 8)
+        // at positions 2 (t % 4), + 1 of each 8, which is where tcgen05.st's
+        // 16x128b shape puts them. (One 16-bit load a position and feature
+        // took 2.2 times the shared-memory cycles, beside products that need
+        // nearly all of them: 4.4 us a chunk against TIMEUS.)
+        float* tab = tables + 32 * (warp - 8);
+        const int wc = warp - 12;
+        const int row = ((lane >> 4) << 3) + (lane & 7);  // ldmatrix row of this lane
+        const uint32_t src0 = smem_u32(sm) + 2 * kTile + (wc >> 1) * kHalf + row * 128;
+        const int chunk0 = 4 * (wc & 1) + ((lane >> 3) & 1);
+        const uint64_t minus = pair(-1.f, -1.f);
         uint32_t n = 0, w = 0;
         bool ok = true;
-        for (int64_t id = blockIdx.x; ok && id < items; id += gridDim.x) {
+        for (int id = blockIdx.x; ok && id < items; id += gridDim.x) {
             const Item it = item_of(p, id);
             const int nch = (it.len + kC - 1) / kC;
-            const double g = p.log_decay[it.h];
+            const float g = p.log_decay[it.h];
             __syncwarp();  // every lane has read the last item's table
-            tab[lane] = static_cast<float>(power(g, p.reverse ? lane + 1 : 31 - lane));
+            tab[lane] = power(g, kRev ? lane + 1 : 31 - lane);
             __syncwarp();
-            const float w32 = static_cast<float>(power(g, 32)), w64 = static_cast<float>(power(g, 64)),
-                        w96 = static_cast<float>(power(g, 96));
+            const float w32 = power(g, 32), w64 = power(g, 64), w96 = power(g, 96);
             for (int c = 0; c < nch; ++c, ++n) {
                 const int st = n & 1;
-                int64_t row;
+                int64_t first;
                 int len;
-                chunk_of(p, it, nch, c, row, len);
-                uint8_t* bt = sm + st * kStage + kTile;
-                uint8_t* ct = bt + kTile;
+                chunk_of<kRev>(it, nch, c, first, len);
                 if (!(ok = warp_wait(&B.full[st], (n >> 1) & 1))) break;
                 if (len < kC) {
                     // The rows past the sequence hold another's (or anything):
                     // zeros, so that no product of theirs is NaN.
-                    for (int r = len + (warp - 8); r < kC; r += 4) {
-                        uint8_t* tile = lane < 16 ? bt : ct;
+                    uint8_t* bt = sm + st * kStage + kTile;
+                    uint8_t* tile = lane < 16 ? bt : bt + kTile;
+                    for (int r = len + wc; r < kC; r += 4)
                         *reinterpret_cast<uint4*>(tile + ((lane & 15) >> 3) * kHalf + r * 128 +
                                                   (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
-                    }
                     fence_proxy_async();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(&B.fix);
+                    if (lane == 0) mbar_arrive(&B.fix[st]);
                 }
-                for (int q = 0; ok && q < 4; ++q, ++w) {
+                const int whole = len >> 5;  // quarters without a short one
+                for (int q = 0; q < 4; ++q, ++w) {
                     const int buf = w & 1;
                     if (w >= 2 && !(ok = warp_wait(&B.wv_free[buf], ((w >> 1) & 1) ^ 1))) break;
                     tc_fence_after();
-                    const uint8_t* src = ct + 32 * q * 128 + cy;
-                    uint32_t hi[16], mid[16], lo[16];
-                    auto split = [&](int j2, float x0, float x1) {
-                        hi[j2] = pack_bf16(x0, x1);
-                        x0 -= low_f32(hi[j2]);
-                        x1 -= high_f32(hi[j2]);
-                        mid[j2] = pack_bf16(x0, x1);
-                        lo[j2] = pack_bf16(x0 - low_f32(mid[j2]), x1 - high_f32(mid[j2]));
-                    };
-                    auto value = [&](int j) {
-                        return __uint_as_float(
-                            static_cast<uint32_t>(*reinterpret_cast<const unsigned short*>(
-                                src + j * 128 + (cx ^ ((j & 7) << 4))))
-                            << 16);
-                    };
-                    if (len == kC) {
-                        // w^(127 - j) = w^(96 - 32 q) w^(31 - jj), and
-                        // w^(j + 1) = w^(32 q) w^(jj + 1).
-                        const int e = p.reverse ? q : 3 - q;
-                        const float base =
-                            p.sigma * (e == 0 ? 1.f : e == 1 ? w32 : e == 2 ? w64 : w96);
+                    // Weights of this thread's positions j = 32 q + jj, jj = 8 k +
+                    // 2 (t % 4) + e: w^(j + 1) = w^(32 q) w^(jj + 1) backward;
+                    // forward, with len = 32 whole + r, w^(len - 1 - j) =
+                    // w^(32 (whole - q - 1)) w^r w^(31 - jj), and in the short
+                    // quarter w^(r - 1 - jj): the table shifted.
+                    const int r = len & 31, live = len - 32 * q;
+                    const int m = kRev ? q : whole - q - 1;
+                    const int shift = !kRev && q == whole ? 32 - r : 0;
+                    float base = p.sigma * (m <= 0 ? 1.f : m == 1 ? w32 : m == 2 ? w64 : w96);
+                    if (!kRev && q < whole) base *= tab[31 - r];
+                    uint64_t wt[4];
 #pragma unroll
-                        for (int j4 = 0; j4 < 8; ++j4) {
-                            const float4 t = reinterpret_cast<const float4*>(tab)[j4];
-                            split(2 * j4, value(4 * j4) * (base * t.x),
-                                  value(4 * j4 + 1) * (base * t.y));
-                            split(2 * j4 + 1, value(4 * j4 + 2) * (base * t.z),
-                                  value(4 * j4 + 3) * (base * t.w));
-                        }
-                    } else {
-                        // A short chunk: w^(len - 1 - j), the table shifted in
-                        // its last quarter; zeros past it.
-                        const int live = len - 32 * q;
-                        const float base = p.sigma * static_cast<float>(power(
-                                                         g, p.reverse ? 32 * q : max(live - 32, 0)));
-                        const int shift = p.reverse || live >= 32 ? 0 : 32 - live;
-#pragma unroll
-                        for (int j2 = 0; j2 < 16; ++j2) {
-                            const int j = 2 * j2;
-                            split(j2, j < live ? value(j) * (base * tab[(j + shift) & 31]) : 0.f,
-                                  j + 1 < live ? value(j + 1) * (base * tab[(j + 1 + shift) & 31])
-                                               : 0.f);
-                        }
+                    for (int k = 0; k < 4; ++k) {
+                        const int jj = 8 * k + 2 * (lane & 3) + shift;
+                        wt[k] = pair(base * tab[jj & 31], base * tab[(jj + 1) & 31]);
                     }
-                    const uint32_t at = quad + kColW + buf * kColWBuf;
-                    tmem_st16(at, hi);
-                    tmem_st16(at + 16, mid);
-                    tmem_st16(at + 32, lo);
+#pragma unroll 1
+                    for (int half = 0; half < 2; ++half) {
+                        uint32_t x[8];
+#pragma unroll
+                        for (int g2 = 0; g2 < 2; ++g2)
+                            asm volatile(
+                                "ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16"
+                                " {%0, %1, %2, %3}, [%4];"
+                                : "=r"(x[4 * g2]), "=r"(x[4 * g2 + 1]), "=r"(x[4 * g2 + 2]),
+                                  "=r"(x[4 * g2 + 3])
+                                : "r"(src0 + st * kStage + (32 * q + 16 * g2) * 128 +
+                                      (((chunk0 + 2 * half) ^ (lane & 7)) << 4))
+                                : "memory");
+                        if (live < 32) {  // what another sequence left there
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) {
+                                const int jj = 8 * k + 2 * (lane & 3);
+                                const uint32_t keep = (jj < live ? 0xffffu : 0u) |
+                                                      (jj + 1 < live ? 0xffff0000u : 0u);
+                                x[2 * k] &= keep;
+                                x[2 * k + 1] &= keep;
+                            }
+                        }
+                        uint32_t mid[8], lo[8];
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) {
+                            uint64_t v = mul2(widen(x[k]), wt[k >> 1]);
+                            x[k] = pack_bf16(v);
+                            v = fma2(widen(x[k]), minus, v);
+                            mid[k] = pack_bf16(v);
+                            lo[k] = pack_bf16(fma2(widen(mid[k]), minus, v));
+                        }
+                        const uint32_t at =
+                            quad + (static_cast<uint32_t>(half) << 20) + kColW + buf * kColWBuf;
+                        tmem_st_16x128(at, x);
+                        tmem_st_16x128(at + 16, mid);
+                        tmem_st_16x128(at + 32, lo);
+                    }
                     tmem_wait_st();
                     tc_fence_before();
                     __syncwarp();
@@ -638,7 +770,7 @@ la_tc(const LaCore p, const __grid_constant__ CUtensorMap ma,
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    if (warp == 13) tmem_dealloc(tm, 512);
+    if (warp == 18) tmem_dealloc(tm, 512);
 }
 
 PFN_cuTensorMapEncodeTiled_v12000 encoder() {
@@ -685,7 +817,8 @@ bool la_tc_supports(const LaCore& p) {
                             reinterpret_cast<uintptr_t>(p.c) | reinterpret_cast<uintptr_t>(p.out);
     return p.dtype == GDR_DTYPE_BF16 && p.d_b <= kD && p.d_c <= kD && p.d_b % 8 == 0 &&
            p.d_c % 8 == 0 && (align & 15) == 0 && la_tokens(p) > 0 &&
-           la_tokens(p) < (int64_t{1} << 31) - 2 * kC;
+           la_tokens(p) < (int64_t{1} << 31) - 2 * kC &&
+           static_cast<int64_t>(p.n_seqs) * p.heads < (int64_t{1} << 30);
 }
 
 cudaError_t launch_la_tc(const LaCore& p, cudaStream_t stream) {
@@ -699,12 +832,13 @@ cudaError_t launch_la_tc(const LaCore& p, cudaStream_t stream) {
         mo = mc;  // not used
     else if (!tile_map(&mo, p.out, tokens, p.heads, p.d_c, 32))
         return cudaErrorInvalidValue;
-    cudaError_t e = cudaFuncSetAttribute(la_tc, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         static_cast<int>(kSmemBytes));
+    auto* kernel = p.reverse ? la_tc<true> : la_tc<false>;
+    const cudaError_t e = cudaFuncSetAttribute(
+        kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmemBytes));
     if (e != cudaSuccess) return e;
     const int64_t items = static_cast<int64_t>(p.n_seqs) * p.heads;
     const int grid = static_cast<int>(std::min<int64_t>(items, sm_count()));
-    la_tc<<<grid, kThreads, kSmemBytes, stream>>>(p, ma, mb, mc, mo, items);
+    kernel<<<grid, kThreads, kSmemBytes, stream>>>(p, ma, mb, mc, mo, static_cast<int>(items));
     return cudaGetLastError();
 }
 
