@@ -11,14 +11,16 @@
 // One CTA per SM, persistent over (sequence, head) items, warp-specialised, so
 // that the loads, the matrix products and the conversions of consecutive
 // chunks run beside one another:
-//   warps 0-3    scores -> decayed bf16 P
-//   warps 4-11   the state, f32 in registers (64 values a thread): adds a
-//                chunk's update, writes the bf16 copy; initial and final states;
-//                the output (scaled, converted, stored)
-//   warps 12-15  the update's operand, c scaled by w^{C-1-j}
-//   warp 16      TMA loads of the a, b, c tiles, two stages of 96 KiB
-//   warp 17      issues the products of the outputs
-//   warp 18      issues the products of the update
+//   warps 0-7    scores -> decayed bf16 P; outputs (scaled, converted, staged)
+//   warps 8-15   the state, f32 in registers (64 values a thread): adds a
+//                chunk's update, writes the bf16 copy; initial and final states
+//   warps 16-23  the update's operand, c scaled by w^{C-1-j}
+//   warp 24      TMA loads of the a, b, c tiles, two stages of 96 KiB
+//   warp 25      issues the products of the outputs
+//   warp 26      issues the products of the update
+//   warp 27      TMA stores of the outputs (stored from registers, 32 bytes of 32
+//                rows at a time, they kept the load-store unit busy for 2000
+//                cycles a chunk)
 // The products of a chunk, M = N = 128 each, f32 accumulators in TMEM:
 //   scores = A B^T              both from shared memory
 //   O      = A Sb               Sb the state's bf16 copy (K-major rows of c)
@@ -60,18 +62,19 @@ namespace {
 using namespace sm100;
 
 constexpr int kC = 128, kD = 128;
-constexpr int kThreads = 640;
+constexpr int kThreads = 896;
 constexpr uint32_t kTile = 32768;         // 128 positions x 128 bf16, two 64-wide halves
 constexpr uint32_t kHalf = kTile / 2;
 constexpr uint32_t kStage = 3 * kTile;    // a, b, c
 constexpr uint32_t kOffSb = 2 * kStage, kOffMisc = kOffSb + kTile;
-constexpr uint32_t kSmemBytes = kOffMisc + 512 + 1024;  // + alignment slack
+constexpr uint32_t kSmemBytes = kOffMisc + 512;
 constexpr uint32_t kColU = 0, kColP = 128, kColO = 256, kColW = 384, kColWBuf = 48;
-constexpr int kWaitTries = 1 << 20;  // seconds
+constexpr int kWaitRounds = 1 << 24;  // of two tries: seconds
 
 struct Bars {
-    uint64_t a_full[2], b_full[2], c_full[2], a_free[2], b_free[2], c_free[2];
-    uint64_t sc_full, in_full, o_full, o_free, pa_ready, sb_ready, u_full, u_free, fix[2], drain[2];
+    uint64_t a_full[2], b_full[2], c_full[2], a_free[2], c_read[2], o_staged[2];
+    uint64_t in_full[2], o_full[2], u_full[2];
+    uint64_t sc_full, pa_ready, sb_ready, o_free, u_free, fix[2], drain[2];
     uint64_t wv_full[2], wv_free[2];
     uint32_t tmem;
 };
@@ -85,24 +88,69 @@ struct Item {
     bool in_t, out_t;  // stored [d_c, d_b]
 };
 
-// Waits for a phase; false once the tries ran out, which is recorded. The
-// hardware suspends a try for some microseconds, without issuing anything (a
-// try with a time of its own became a loop of sleeps: a third of all
-// instructions). Tries are counted rather than timed to keep the code small: six
-// roles' loops share one instruction cache.
+// Waits for a phase; false once the tries ran out. A try suspends the warp for
+// some 90 cycles (one with a time of its own becomes a loop of sleeps).
 __device__ __forceinline__ bool lane_wait(uint64_t* bar, uint32_t parity) {
-#pragma unroll 1
-    for (int i = 0; i < kWaitTries; ++i)
-        if (mbar_try_wait(bar, parity)) return true;
-    atomicOr(&g_la_error, 1);
-    return false;
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t.reg .b32 i;\n\t"
+        "mov.b32 i, %3;\n\t"
+        "LA_TRY:\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t@p bra LA_DONE;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t@p bra LA_DONE;\n\t"
+        "sub.s32 i, i, 1;\n\tsetp.ne.s32 q, i, 0;\n\t@q bra LA_TRY;\n\t"
+        "LA_DONE:\n\tselp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity), "n"(kWaitRounds)
+        : "memory");
+    return ok != 0;
 }
-// The same for a whole warp together: false for every lane.
+// The same for a whole warp.
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) {
     return __all_sync(0xffffffffu, lane_wait(bar, parity));
 }
+// One lane of a converged warp. (The compiler knows it: behind `lane == 0` it
+// wraps every product, commit and copy in an election of its own, 15
+// instructions each.)
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(p));
+    return p != 0;
+}
+// The same for the eight warps of a role together, in step: one of them waits for
+// the phase, the others at a hardware barrier, which costs them no issue
+// slots (24 warps trying took more than half of all instructions). The
+// barrier carries the outcome, so that all of them go on or none.
+__device__ __forceinline__ bool group_wait(uint64_t* bar, uint32_t parity, uint32_t id, bool waits) {
+    uint32_t failed = 0;
+    if (waits) failed = !lane_wait(bar, parity);
+    uint32_t any;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\t"
+        "barrier.cta.red.or.pred q, %2, 256, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+        : "=r"(any)
+        : "r"(failed), "r"(id)
+        : "memory");
+    return any == 0;
+}
 __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+
+// Where the x-th 128 bytes of the features of a stage's outputs are staged: the
+// a tile's halves, f32 outputs in the c tile's too.
+__device__ __forceinline__ uint8_t* staged(uint8_t* stage, int x) {
+    return stage + (x >> 1) * 2 * kTile + (x & 1) * kHalf;
+}
+
+__device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, const void* src, int c0,
+                                             int c1, int c2) {
+    asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];"
+                 ::"l"(reinterpret_cast<uint64_t>(map)),
+                 "r"(smem_u32(src)), "r"(c0), "r"(c1), "r"(c2)
+                 : "memory");
 }
 
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16]) {
@@ -120,6 +168,15 @@ __device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&v)[8])
         "tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr),
         "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
         : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint64_t (&v)[8]) {
+    uint32_t r[16];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        r[2 * i] = static_cast<uint32_t>(v[i]);
+        r[2 * i + 1] = static_cast<uint32_t>(v[i] >> 32);
+    }
+    tmem_st16(taddr, r);
 }
 
 // 32 lanes x 16 columns, as pairs of columns, arrived. (The loads take some 30
@@ -150,15 +207,87 @@ __device__ __forceinline__ void tmem_st_16x128(uint32_t taddr, const uint32_t (&
         : "memory");
 }
 
-// D[tmem] = A[tmem] B (+ D): A's rows are the lanes, K pairs its columns.
-__device__ __forceinline__ void umma_bf16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc,
-                                             uint32_t idesc, uint32_t accumulate) {
+// The products of a chunk, 128 x 128 each, issued by one elected thread. The
+// operands' addresses step inside the assembly, which takes four instructions a
+// product; stepped outside, or in a branch on the stage, two to four times that.
+
+// D = A B over 128 of K: both K-major in shared memory (two 64-wide halves).
+__device__ __forceinline__ void product_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
-        "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        "{\n\t.reg .pred p, t;\n\t.reg .b64 a, b;\n\t"
+        "setp.ne.b32 p, 0, 0;\n\tsetp.eq.b32 t, 0, 0;\n\t"
+        "mov.b64 a, %1;\n\tmov.b64 b, %2;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t"
+        "add.s64 a, a, 2;\n\tadd.s64 b, b, 2;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, t;\n\t"
+        "add.s64 a, a, 2;\n\tadd.s64 b, b, 2;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, t;\n\t"
+        "add.s64 a, a, 2;\n\tadd.s64 b, b, 2;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, t;\n\t"
+        "add.s64 a, a, 1018;\n\tadd.s64 b, b, 1018;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, t;\n\t"
+        "add.s64 a, a, 2;\n\tadd.s64 b, b, 2;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, t;\n\t"
+        "add.s64 a, a, 2;\n\tadd.s64 b, b, 2;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, t;\n\t"
+        "add.s64 a, a, 2;\n\tadd.s64 b, b, 2;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, t;\n\t"
+        "}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc)
         : "memory");
+}
+// D += A B over 128 of K: A in TMEM (its rows the lanes; the second half 64
+// columns from the first), B MN-major.
+__device__ __forceinline__ void product_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc) {
+    asm volatile(
+        "{\n\t.reg .pred t;\n\t.reg .b32 a;\n\t.reg .b64 b;\n\t"
+        "setp.eq.b32 t, 0, 0;\n\tmov.b32 a, %1;\n\tmov.b64 b, %2;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [a], b, %3, t;\n\t"
+        "add.u32 a, a, 8;\n\tadd.s64 b, b, 128;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [a], b, %3, t;\n\t"
+        "add.u32 a, a, 8;\n\tadd.s64 b, b, 128;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [a], b, %3, t;\n\t"
+        "add.u32 a, a, 8;\n\tadd.s64 b, b, 128;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [a], b, %3, t;\n\t"
+        "add.u32 a, a, 40;\n\tadd.s64 b, b, 128;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [a], b, %3, t;\n\t"
+        "add.u32 a, a, 8;\n\tadd.s64 b, b, 128;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [a], b, %3, t;\n\t"
+        "add.u32 a, a, 8;\n\tadd.s64 b, b, 128;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [a], b, %3, t;\n\t"
+        "add.u32 a, a, 8;\n\tadd.s64 b, b, 128;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [a], b, %3, t;\n\t"
+        "}" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc)
+        : "memory");
+}
+// D = (or +=) (A1 + A2 + A3) B over 32 of K: the parts 16 columns apart in TMEM.
+__device__ __forceinline__ void product_ts3(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc,
+                                            uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, t;\n\t.reg .b32 a;\n\t.reg .b64 b;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\tsetp.eq.b32 t, 0, 0;\n\tmov.b32 a, %1;\n\tmov.b64 b, %2;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [a], b, %3, p;\n\t"
+        "add.u32 a, a, 16;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [a], b, %3, t;\n\t"
+        "add.u32 a, a, 16;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [a], b, %3, t;\n\t"
+        "sub.u32 a, a, 24;\n\tadd.s64 b, b, 128;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [a], b, %3, t;\n\t"
+        "add.u32 a, a, 16;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [a], b, %3, t;\n\t"
+        "add.u32 a, a, 16;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [a], b, %3, t;\n\t"
+        "}" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+// The n lowest bits (all 32 from n = 32 on).
+__device__ __forceinline__ uint32_t low_bits(uint32_t n) {
+    uint32_t r;
+    asm("bmsk.clamp.b32 %0, 0, %1;" : "=r"(r) : "r"(n));
+    return r;
 }
 
 // Two f32 as bf16, x in the low half.
@@ -170,8 +299,8 @@ __device__ __forceinline__ uint32_t pack_bf16(float x, float y) {
 __device__ __forceinline__ float low_f32(uint32_t p) { return __uint_as_float(p << 16); }
 __device__ __forceinline__ float high_f32(uint32_t p) { return __uint_as_float(p & 0xffff0000u); }
 
-// Moves registers between the roles: the launch gives each thread 96, 480 for
-// the five warpgroups' lanes together; 40 + 80 + 2 x 128 + 96 = 472 of them.
+// Moves registers between the roles: the launch gives each thread 72, 504 for
+// the seven warpgroups' lanes together: 2 x 72 + 2 x 96 + 2 x 64 + 40.
 template <int kRegs>
 __device__ __forceinline__ void give_registers() {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegs));
@@ -227,12 +356,6 @@ __device__ __forceinline__ float2 power2(float g, int n) {
 // Heads whose decay's powers to w^-128 are far from overflow (e^51).
 __device__ __forceinline__ bool is_gentle(float g) { return g >= -0.4f && g <= 0.4f; }
 
-// tau times the decay of the state before the chunk at its row i.
-template <bool kRev>
-__device__ __forceinline__ float row_factor(const LaCore& p, float g, int len, int i) {
-    return p.tau * power(g, kRev ? max(len - 1 - i, 0) : i + 1);
-}
-
 __device__ __forceinline__ Item item_of(const LaCore& p, int id) {
     Item it;
     const int s = id / p.heads;
@@ -263,52 +386,55 @@ __device__ __forceinline__ void chunk_of(const Item& it, int nch, int c,
 template <bool kRev>
 __global__ void __launch_bounds__(kThreads, 1)
 la_tc(const LaCore p, const __grid_constant__ CUtensorMap ma,
-      const __grid_constant__ CUtensorMap mb, const __grid_constant__ CUtensorMap mc, int items) {
-    extern __shared__ uint8_t raw[];
-    uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) &
-                                             ~static_cast<uintptr_t>(1023));
+      const __grid_constant__ CUtensorMap mb, const __grid_constant__ CUtensorMap mc,
+      const __grid_constant__ CUtensorMap mo, int items) {
+    extern __shared__ __align__(1024) uint8_t sm[];  // (checked below: swizzled tiles need it)
     Bars& B = *reinterpret_cast<Bars*>(sm + kOffMisc);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) {
             mbar_init(&B.a_full[i], 1);
             mbar_init(&B.b_full[i], 1);
-            mbar_init(&B.c_full[i], 1);
             mbar_init(&B.a_free[i], 1);
-            mbar_init(&B.b_free[i], 1);
-            mbar_init(&B.c_free[i], 5);  // its product's end, and the operand's warps
-            mbar_init(&B.drain[i], 1);
-            mbar_init(&B.fix[i], 4);
-            mbar_init(&B.wv_full[i], 4);
+            mbar_init(&B.o_staged[i], 8);
+            mbar_init(&B.c_full[i], 1);
+            mbar_init(&B.c_read[i], 8);
+            mbar_init(&B.in_full[i], 1);
+            mbar_init(&B.o_full[i], 1);
+            mbar_init(&B.u_full[i], 1);
+            mbar_init(&B.fix[i], 8);
+            mbar_init(&B.wv_full[i], 8);
             mbar_init(&B.wv_free[i], 1);
+            mbar_init(&B.drain[i], 1);
         }
         mbar_init(&B.sc_full, 1);
-        mbar_init(&B.in_full, 1);
-        mbar_init(&B.o_full, 1);
+        mbar_init(&B.pa_ready, 8);
         mbar_init(&B.o_free, 8);
-        mbar_init(&B.pa_ready, 4);
         mbar_init(&B.sb_ready, 8);
-        mbar_init(&B.u_full, 1);
         mbar_init(&B.u_free, 8);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 18) {
+    if (warp == 26) {
         tmem_alloc(&B.tmem, 512);
         tmem_relinquish();
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tm = B.tmem;
+    bool ok = true;  // false: a wait ran out, and its role with it
+    // All 512 columns are this CTA's, so they begin at 0: a constant, as the
+    // tiles' addresses are, keeps the products' operands in uniform registers.
+    constexpr uint32_t tm = 0;
+    if (B.tmem != 0 || (smem_u32(sm) & 1023) != 0) items = 0;  // never: nothing would be right
+    if (items == 0) ok = false;
     const uint32_t quad = tm + (static_cast<uint32_t>(warp & 3) << 21);  // this warp's lanes
 
-    if (warp >= 16) {
+    if (warp >= 24) {
         give_registers<40>();
-    if (warp == 16) {
+    if (warp == 24) {
         // ---- loads -------------------------------------------------------------
-        if (lane == 0) {
+        {
             uint32_t n = 0;
-            bool ok = true;
 #pragma unroll 1
             for (int id = blockIdx.x; ok && id < items; id += gridDim.x) {
                 const Item it = item_of(p, id);
@@ -323,39 +449,49 @@ la_tc(const LaCore p, const __grid_constant__ CUtensorMap ma,
                     int len;
                     chunk_of<kRev>(it, nch, c, row, len);
                     const int r = static_cast<int>(row);
-                    auto load = [&](uint64_t* full, uint64_t* free, uint8_t* dst,
-                                    const CUtensorMap* map, int head) {
-                        if (n >= 2 && !(ok = lane_wait(free, ph))) return;
-                        mbar_expect_tx(full, kTile);
-                        tma_load_3d(dst, map, full, 0, head, r);
-                        tma_load_3d(dst + kHalf, map, full, 64, head, r);
-                    };
-                    // a is free after the scores' and the inter product, b then after
-                    // the update's, c after P C and the operand's warps.
                     uint8_t* base = sm + st * kStage;
-                    load(&B.a_full[st], &B.a_free[st], base, &ma, ha);
-                    if (ok) load(&B.b_full[st], &B.b_free[st], base + kTile, &mb, hb);
-                    if (ok) load(&B.c_full[st], &B.c_free[st], base + 2 * kTile, &mc, hc);
-                    if (!ok) break;
+                    auto load = [&](uint64_t* full, uint8_t* dst, const CUtensorMap* map, int head) {
+                        if (elect_one()) {
+                            mbar_expect_tx(full, kTile);
+                            tma_load_3d(dst, map, full, 0, head, r);
+                            tma_load_3d(dst + kHalf, map, full, 64, head, r);
+                        }
+                    };
+                    // Chunk n - 2: its products with b and with c are done, its operand's
+                    // warps have read c, and its output has left the tiles.
+                    if (n >= 2 && !(ok = warp_wait(&B.in_full[st], ph))) break;
+                    if (n >= 2 && !(ok = warp_wait(&B.u_full[st], ph))) break;
+                    load(&B.b_full[st], base + kTile, &mb, hb);
+                    if (n >= 2 && p.out_f32 && !(ok = warp_wait(&B.a_free[st], ph))) break;
+                    if (n >= 2 && !(ok = warp_wait(&B.o_full[st], ph))) break;
+                    if (n >= 2 && !(ok = warp_wait(&B.c_read[st], ph))) break;
+                    load(&B.c_full[st], base + 2 * kTile, &mc, hc);
+                    if (n >= 2 && !(ok = warp_wait(&B.a_free[st], ph))) break;
+                    load(&B.a_full[st], base, &ma, ha);
                 }
             }
             // Nothing of this CTA's may be in flight when it ends.
 #pragma unroll 1
             for (uint32_t i = n >= 2 ? n - 2 : 0; i < n + (ok ? 0 : 1); ++i)
                 for (uint64_t* full : {B.a_full, B.b_full, B.c_full})
-                    lane_wait(&full[i & 1], (i >> 1) & 1);
+                    warp_wait(&full[i & 1], (i >> 1) & 1);
         }
         __syncwarp();
-    } else if (warp == 17) {
+    } else if (warp == 25) {
         // ---- the outputs' products -------------------------------------------------
-        if (lane == 0) {
+        {
             constexpr uint32_t kKK = idesc_bf16(128, 128, 0, 0, 0);
             constexpr uint32_t kKMn = idesc_bf16(128, 128, 0, 1, 0);
-            const uint64_t tile0 = sdesc_sw128(smem_u32(sm), 16, 1024);
-            const uint64_t sb = sdesc_sw128(smem_u32(sm + kOffSb), 16, 1024);
-            const uint64_t mn0 = sdesc_sw128(smem_u32(sm), kHalf, 1024);
+            const uint32_t base = smem_u32(sm);
+            auto from_a = [&](uint32_t st, uint32_t d, uint32_t b_tile) {
+                product_ss(tm + d, sdesc_sw128(base + st * kStage, 16, 1024),
+                           sdesc_sw128(b_tile, 16, 1024), kKK);
+            };
+            auto from_p = [&](uint32_t st) {
+                product_ts(tm + kColO, tm + kColP,
+                           sdesc_sw128(base + st * kStage + 2 * kTile, kHalf, 1024), kKMn);
+            };
             uint32_t n = 0, tails = 0;
-            bool ok = true;
 #pragma unroll 1
             for (int id = blockIdx.x; ok && id < items; id += gridDim.x) {
                 const Item it = item_of(p, id);
@@ -363,52 +499,48 @@ la_tc(const LaCore p, const __grid_constant__ CUtensorMap ma,
 #pragma unroll 1
                 for (int c = 0; c < nch; ++c, ++n) {
                     const uint32_t st = n & 1, ph = n & 1;
-                    const uint64_t a = tile0 + st * (kStage >> 4), bt = a + (kTile >> 4);
-                    if (!(ok = lane_wait(&B.a_full[st], (n >> 1) & 1))) break;
-                    if (!(ok = lane_wait(&B.b_full[st], (n >> 1) & 1))) break;
+                    if (!(ok = warp_wait(&B.b_full[st], (n >> 1) & 1))) break;
+                    if (!(ok = warp_wait(&B.a_full[st], (n >> 1) & 1))) break;
                     if (chunk_len<kRev>(it, nch, c) < kC) {  // (by stage: bits of `tails`)
-                        if (!(ok = lane_wait(&B.fix[st], (tails >> st) & 1))) break;
+                        if (!(ok = warp_wait(&B.fix[st], (tails >> st) & 1))) break;
                         tails ^= 1u << st;
                     }
                     tc_fence_after();
-#pragma unroll 1
-                    for (uint32_t k = 0; k < 8; ++k) {
-                        const uint32_t off = ((k >> 2) * kHalf + (k & 3) * 32) >> 4;
-                        umma_bf16(tm + kColP, a + off, bt + off, kKK, k);
+                    if (elect_one()) {
+                        from_a(st, kColP, base + st * kStage + kTile);
+                        umma_commit(&B.sc_full);
                     }
-                    umma_commit(&B.sc_full);
-                    if (!(ok = lane_wait(&B.sb_ready, ph))) break;
-                    if (n > 0 && !(ok = lane_wait(&B.o_free, ph ^ 1))) break;
+                    if (!(ok = warp_wait(&B.sb_ready, ph))) break;
+                    if (n > 0 && !(ok = warp_wait(&B.o_free, ph ^ 1))) break;
                     tc_fence_after();
-#pragma unroll 1
-                    for (uint32_t k = 0; k < 8; ++k) {
-                        const uint32_t off = ((k >> 2) * kHalf + (k & 3) * 32) >> 4;
-                        umma_bf16(tm + kColO, a + off, sb + off, kKK, k);
+                    if (elect_one()) {
+                        from_a(st, kColO, base + kOffSb);
+                        umma_commit(&B.in_full[st]);
                     }
-                    umma_commit(&B.in_full);
-                    umma_commit(&B.a_free[st]);
-                    if (!(ok = lane_wait(&B.c_full[st], (n >> 1) & 1))) break;
-                    if (!(ok = lane_wait(&B.pa_ready, ph))) break;
+                    // (P is written, and the c tile is there: its warps waited for it.)
+                    if (!(ok = warp_wait(&B.pa_ready, ph))) break;
                     tc_fence_after();
-                    const uint64_t v = mn0 + ((st * kStage + 2 * kTile) >> 4);
-#pragma unroll 1
-                    for (uint32_t k = 0; k < 8; ++k)
-                        umma_bf16_ts(tm + kColO, tm + kColP + 8 * k, v + k * (2048 >> 4), kKMn, 1);
-                    umma_commit(&B.o_full);
-                    umma_commit(&B.c_free[st]);
+                    if (elect_one()) {
+                        from_p(st);
+                        umma_commit(&B.o_full[st]);
+                    }
                 }
             }
-            umma_commit(&B.drain[0]);
-            lane_wait(&B.drain[0], 0);
+            if (elect_one()) umma_commit(&B.drain[0]);
+            warp_wait(&B.drain[0], 0);
         }
         __syncwarp();
-    } else if (warp == 18) {
+    } else if (warp == 26) {
         // ---- the update's products -------------------------------------------------
-        if (lane == 0) {
+        {
             constexpr uint32_t kKMn = idesc_bf16(128, 128, 0, 1, 0);
-            const uint64_t mn0 = sdesc_sw128(smem_u32(sm) + kTile, kHalf, 1024);
-            uint32_t n = 0, w = 0, tails = 0;
-            bool ok = true;
+            const uint32_t base = smem_u32(sm);
+            auto update = [&](uint32_t st, uint32_t q) {  // 32 positions, in buffer q % 2
+                product_ts3(tm + kColU, tm + kColW + (q & 1) * kColWBuf,
+                            sdesc_sw128(base + st * kStage + kTile + q * 4096, kHalf, 1024), kKMn,
+                            q);
+            };
+            uint32_t n = 0, tails = 0;
 #pragma unroll 1
             for (int id = blockIdx.x; ok && id < items; id += gridDim.x) {
                 const Item it = item_of(p, id);
@@ -416,41 +548,80 @@ la_tc(const LaCore p, const __grid_constant__ CUtensorMap ma,
 #pragma unroll 1
                 for (int c = 0; c < nch; ++c, ++n) {
                     const uint32_t st = n & 1;
-                    const uint64_t bt = mn0 + st * (kStage >> 4);
-                    if (!(ok = lane_wait(&B.b_full[st], (n >> 1) & 1))) break;
+                    if (!(ok = warp_wait(&B.b_full[st], (n >> 1) & 1))) break;
                     if (chunk_len<kRev>(it, nch, c) < kC) {  // (by stage: bits of `tails`)
-                        if (!(ok = lane_wait(&B.fix[st], (tails >> st) & 1))) break;
+                        if (!(ok = warp_wait(&B.fix[st], (tails >> st) & 1))) break;
                         tails ^= 1u << st;
                     }
-                    if (n > 0 && !(ok = lane_wait(&B.u_free, (n & 1) ^ 1))) break;
+                    if (n > 0 && !(ok = warp_wait(&B.u_free, (n & 1) ^ 1))) break;
 #pragma unroll 1
-                    for (uint32_t q = 0; q < 4; ++q, ++w) {
-                        const uint32_t buf = w & 1;
-                        if (!(ok = lane_wait(&B.wv_full[buf], (w >> 1) & 1))) break;
+                    for (uint32_t q = 0; q < 4; ++q) {
+                        // (Buffer q % 2 for the (2 n + q / 2)th time.)
+                        if (!ok || !(ok = warp_wait(&B.wv_full[q & 1], (q >> 1) & 1))) break;
                         tc_fence_after();
-                        const uint32_t op = tm + kColW + buf * kColWBuf;
-#pragma unroll 1
-                        for (uint32_t k = 0; k < 2; ++k) {
-                            const uint64_t d = bt + (2 * q + k) * (2048 >> 4);
-#pragma unroll
-                            for (uint32_t t = 0; t < 3; ++t)
-                                umma_bf16_ts(tm + kColU, op + 16 * t + 8 * k, d, kKMn, q | k | t);
+                        if (elect_one()) {
+                            update(st, q);
+                            umma_commit(&B.wv_free[q & 1]);
+                            if (q == 3) umma_commit(&B.u_full[st]);
                         }
-                        umma_commit(&B.wv_free[buf]);
                     }
                     if (!ok) break;
-                    umma_commit(&B.u_full);
-                    umma_commit(&B.b_free[st]);
                 }
             }
-            umma_commit(&B.drain[1]);
-            lane_wait(&B.drain[1], 0);
+            if (elect_one()) umma_commit(&B.drain[1]);
+            warp_wait(&B.drain[1], 0);
         }
         __syncwarp();
+    } else if (warp == 27) {
+        // ---- the outputs' stores -----------------------------------------------------
+        uint32_t n = 0;
+#pragma unroll 1
+        for (int id = blockIdx.x; ok && id < items; id += gridDim.x) {
+            const Item it = item_of(p, id);
+            const int nch = (it.len + kC - 1) / kC;
+#pragma unroll 1
+            for (int c = 0; c < nch; ++c, ++n) {
+                const uint32_t st = n & 1;
+                int64_t row;
+                int len;
+                chunk_of<kRev>(it, nch, c, row, len);
+                if (!(ok = lane_wait(&B.o_staged[st], (n >> 1) & 1))) break;
+                uint8_t* tile = sm + st * kStage;
+                // Boxes of 32 positions, 128 bytes of features each; the last rows one
+                // by one: behind them another sequence's stay as they are.
+                const int whole = len & ~31, boxes = p.out_f32 ? 4 : 2, width = p.out_f32 ? 32 : 64;
+                if (lane == 0) {
+#pragma unroll 1
+                    for (int x = 0; x < boxes && x * width < p.d_c; ++x)
+#pragma unroll 1
+                        for (int r = 0; r < whole; r += 32)
+                            tma_store_3d(&mo, staged(tile, x) + r * 128, x * width, it.h,
+                                         static_cast<int>(row) + r);
+                    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                }
+                const int piece = p.out_f32 ? 4 : 8;  // features in 16 bytes
+                uint8_t* out = static_cast<uint8_t*>(p.out);
+#pragma unroll 1
+                for (int r = whole; r < len; ++r) {
+                    const int64_t at = ((row + r) * p.heads + it.h) * p.d_c + lane * piece;
+                    if (lane * piece < p.d_c)
+                        *reinterpret_cast<uint4*>(out + at * (16 / piece)) =
+                            *reinterpret_cast<const uint4*>(staged(tile, lane >> 3) + r * 128 +
+                                                            (((lane & 7) ^ (r & 7)) << 4));
+                }
+                fence_proxy_async();  // the tile's next writer is the async proxy
+                __syncwarp();
+                if (lane == 0) {
+                    asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+                    mbar_arrive(&B.a_free[st]);
+                }
+            }
+        }
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+        __syncwarp();
     }
-    } else if (warp < 4) {
-        give_registers<80>();
-        // ---- scores -----------------------------------------------------------------
+    } else if (warp < 8) {
+        // ---- scores and outputs -------------------------------------------------------
         // Where w^-128 is far from overflow, the powers come out of the sums:
         //   out_i = tau w^{i+1} [ a_i . S + sum_{j<=i} sigma w^{-(j+1)} (a_i.b_j) c_j ]
         // (backward w^{len-1-i} and w^{-(len-1-j)}): one column factor on the
@@ -460,10 +631,14 @@ la_tc(const LaCore p, const __grid_constant__ CUtensorMap ma,
         // A block's 32 column factors run from the largest exponent down by
         // products with w^2 in registers: a table in shared memory waits there
         // behind the tensor cores' operands.
-        const int i = 32 * warp + lane;  // this thread's row of the chunk
-        const int blocks = kRev ? 4 - warp : warp + 1, cb0 = kRev ? warp : 0;  // not masked
+        // Two warps share 32 rows: of the scores blocks 0, 1 and 2, 3 (P goes over the
+        // first scores of either pair), of the outputs 64 features each.
+        const int quarter = warp & 3, half = warp >> 2, i = 32 * quarter + lane;
+        // This warp's blocks that the mask leaves: [first, last).
+        const int first = kRev ? max(2 * half, quarter) : 2 * half;
+        const int last = kRev ? 2 * half + 2 : min(2 * half + 2, quarter + 1);
+        const uint32_t pcol = quad + kColP + 64 * half;  // P's and the scores' columns
         uint32_t n = 0;
-        bool ok = true;
 #pragma unroll 1
         for (int id = blockIdx.x; ok && id < items; id += gridDim.x) {
             const Item it = item_of(p, id);
@@ -471,38 +646,48 @@ la_tc(const LaCore p, const __grid_constant__ CUtensorMap ma,
             const float g = p.log_decay[it.h], w = power(g, 1);
             const bool gentle = is_gentle(g);
             const uint64_t step = pair(w * w, w * w);
-            const float w16 = power(g, 16), steep = power(g, kRev ? max(16 - lane, 0)
-                                                                  : max(lane - 15, 0));
-            float ahead = 0.f, fb[4];  // steep: O's row factor; each block's first column factor
+            const float w16 = power(g, 16);
+            // Steep, the diagonal block's second half.
+            const float steep = p.sigma * p.tau * power(g, kRev ? max(16 - lane, 0)
+                                                                : max(lane - 15, 0));
+            float ahead = 0.f, fb[2];  // O's row factor; the blocks' first column factors
             int known = 0;             // the chunk length they are for
 #pragma unroll 1
             for (int c = 0; c < nch; ++c, ++n) {
-                const uint32_t ph = n & 1;
+                const uint32_t st = n & 1, ph = n & 1, ph2 = (n >> 1) & 1;
                 const int len = chunk_len<kRev>(it, nch, c);
                 if (len != known) {
-                    ahead = row_factor<kRev>(p, g, len, i);
+                    ahead = p.tau * power(g, kRev ? max(len - 1 - i, 0) : i + 1);
                     // Steep, off the diagonal block: w^{i-j} splits in two
                     // exponents that are not negative, rows' and columns'.
                     const float edge = p.sigma * p.tau * power(g, kRev ? 32 - lane : lane + 1);
 #pragma unroll
-                    for (int cb = 0; cb < 4; ++cb) {
+                    for (int x = 0; x < 2; ++x) {
+                        const int cb = 2 * half + x;
                         const int e = kRev ? len - 1 - 32 * cb : 32 * cb + 32;
-                        const int apart = kRev ? cb - warp : warp - cb;
-                        fb[cb] = (gentle ? p.sigma : edge) *
-                                 power(gentle && e >= 0 ? -g : g,
-                                       gentle ? abs(e) : 32 * (apart - 1));
+                        const int apart = kRev ? cb - quarter : quarter - cb;
+                        fb[x] = (gentle ? p.sigma : edge) *
+                                power(gentle && e >= 0 ? -g : g,
+                                      gentle ? abs(e) : 32 * (apart - 1));
                     }
                     known = len;
                 }
-                // Half block y = 2 x + (upper half), 16 scores a thread. The powers run
-                // from the larger exponents' side ...
-                auto decay = [&](int y, uint64_t (&s)[8]) {
-                    const int x = y >> 1, hb = y & 1, cb = cb0 + x;
-                    const bool diag = kRev ? x == 0 : x == blocks - 1;
-                    const bool far = kRev ? hb == 1 : hb == 0;
+                if (!(ok = group_wait(&B.sc_full, ph, 1, warp == 0))) break;
+                tc_fence_after();
+#pragma unroll 1
+                for (int cb = first; cb < last; ++cb) {
+#pragma unroll
+                for (int hb = 0; hb < 2; ++hb) {  // half blocks: 16 scores a thread
+                    const int x = cb & 1;
+                    const bool diag = cb == quarter;
+                    uint64_t s[8];
+                    tmem_ld16(pcol + 32 * x + 16 * hb, s);
                     uint32_t packed[8];
+                    // The powers run from the larger exponents' side of either half.
+                    const bool far = kRev ? hb == 1 : hb == 0;
+                    const int me = lane - 16 * hb;  // this row's column in the half, if diag
                     if (gentle || !diag) {
-                        float f = cb < 2 ? (cb == 0 ? fb[0] : fb[1]) : (cb == 2 ? fb[2] : fb[3]);
+                        float f = x == 0 ? fb[0] : fb[1];
                         if (far) f *= w16;
                         uint64_t f2 = kRev ? pair(f, f * w) : pair(f * w, f);
 #pragma unroll
@@ -512,84 +697,107 @@ la_tc(const LaCore p, const __grid_constant__ CUtensorMap ma,
                             f2 = mul2(f2, step);
                         }
                     } else {
-                        const int me = lane - 16 * hb;  // this row's column in the half
-                        float f = p.sigma * p.tau * (far ? steep : 1.f);
+                        float f = far ? steep : p.sigma * p.tau;
 #pragma unroll
                         for (int t = 0; t < 8; ++t) {
                             const int j = kRev ? t : 7 - t;
-                            float x, y2;
-                            unpair(s[j], x, y2);
-                            (kRev ? x : y2) *= f;
+                            float u, v;
+                            unpair(s[j], u, v);
+                            (kRev ? u : v) *= f;
                             if (kRev ? 2 * j >= me : 2 * j + 1 <= me) f *= w;
-                            (kRev ? y2 : x) *= f;
+                            (kRev ? v : u) *= f;
                             if (kRev ? 2 * j + 1 >= me : 2 * j <= me) f *= w;
-                            packed[j] = pack_bf16(x, y2);
+                            packed[j] = pack_bf16(u, v);
                         }
                     }
                     if (diag) {  // j <= i, or j >= i
-                        const int me = lane - 16 * hb;
+                        const int edge16 = 16 * (kRev ? me : me + 1);  // bits of the pairs kept, or not
 #pragma unroll
                         for (int j = 0; j < 8; ++j) {
-                            const bool k0 = kRev ? 2 * j >= me : 2 * j <= me;
-                            const bool k1 = kRev ? 2 * j + 1 >= me : 2 * j + 1 <= me;
-                            packed[j] &= (k0 ? 0xffffu : 0u) | (k1 ? 0xffff0000u : 0u);
+                            const uint32_t low = low_bits(max(edge16 - 32 * j, 0));
+                            packed[j] &= kRev ? ~low : low;
                         }
                     }
-                    tmem_st8(quad + kColP + 16 * cb + 8 * hb, packed);
-                };
-                if (!(ok = warp_wait(&B.sc_full, ph))) break;
-                tc_fence_after();
-                // ... and P goes over the scores in their order, over blocks that are
-                // read by then.
-                const uint32_t scores = quad + kColP + 32 * cb0;
-#pragma unroll 1
-                for (int y = 0; y < 2 * blocks; ++y) {
-                    uint64_t s[8];
-                    tmem_ld16(scores + 16 * y, s);
-                    decay(y, s);
+                    tmem_st8(pcol + 16 * x + 8 * hb, packed);
+                }
                 }
                 uint32_t zero[16];
 #pragma unroll
                 for (int j = 0; j < 16; ++j) zero[j] = 0;
 #pragma unroll 1
-                for (int cb = kRev ? 0 : blocks; cb < (kRev ? cb0 : 4); ++cb)
-                    tmem_st16(quad + kColP + 16 * cb, zero);
+                for (int cb = 2 * half; cb < 2 * half + 2; ++cb)
+                    if (cb < first || cb >= last) tmem_st16(pcol + 16 * (cb & 1), zero);
                 if (!gentle) {
-                    if (!(ok = warp_wait(&B.in_full, ph))) break;
+                    if (!(ok = group_wait(&B.in_full[st], ph2, 1, warp == 0))) break;
                     tc_fence_after();
 #pragma unroll 1
-                    for (int cb = 0; cb < 4; ++cb) {
-                        float o[32];
-                        tmem_ld32(quad + kColO + 32 * cb, o);
-                        tmem_wait_ld();
+                    for (int blk = 0; blk < 4; ++blk) {
+                        const uint32_t at = quad + kColO + 64 * half + 16 * blk;
+                        uint64_t o[8];
+                        tmem_ld16(at, o);
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) o[j] *= ahead;
-                        tmem_st32(quad + kColO + 32 * cb, o);
+                        for (int j = 0; j < 8; ++j) o[j] = mul2(o[j], pair(ahead, ahead));
+                        tmem_st16(at, o);
                     }
                 }
+                if (!(ok = group_wait(&B.c_full[st], ph2, 1, warp == 0))) break;
                 tmem_wait_st();
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&B.pa_ready);
+
+                // The output: scaled, converted, staged where a was (f32: and c).
+                if (!(ok = group_wait(&B.o_full[st], ph2, 1, warp == 0))) break;
+                if (p.out_f32 && !(ok = group_wait(&B.c_read[st], ph2, 1, warp == 0))) break;
+                tc_fence_after();
+                const float last_factor = gentle ? ahead : 1.f;
+                const uint64_t scale = pair(last_factor, last_factor);
+                uint8_t* tile = sm + st * kStage;
+#pragma unroll 1
+                for (int blk = 0; blk < 4; ++blk) {
+                    uint64_t u[8];
+                    tmem_ld16(quad + kColO + 64 * half + 16 * blk, u);
+                    if (blk == 3) {
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&B.o_free);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) u[j] = mul2(u[j], scale);
+                    if (p.out_f32) {
+                        uint8_t* dst = staged(tile, 2 * half + (blk >> 1)) + i * 128;
+#pragma unroll
+                        for (int m = 0; m < 4; ++m)
+                            *reinterpret_cast<ulonglong2*>(
+                                dst + ((((blk & 1) * 4 + m) ^ (i & 7)) << 4)) =
+                                make_ulonglong2(u[2 * m], u[2 * m + 1]);
+                    } else {
+                        uint8_t* dst = staged(tile, half) + i * 128;
+#pragma unroll
+                        for (int m = 0; m < 2; ++m)
+                            *reinterpret_cast<uint4*>(dst + (((blk * 2 + m) ^ (i & 7)) << 4)) =
+                                make_uint4(pack_bf16(u[4 * m]), pack_bf16(u[4 * m + 1]),
+                                           pack_bf16(u[4 * m + 2]), pack_bf16(u[4 * m + 3]));
+                    }
+                }
+                fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&B.o_staged[st]);
             }
         }
-    } else if (warp < 12) {
-        take_registers<128>();
-        // ---- the state and the outputs ----------------------------------------------
+    } else if (warp < 16) {
+        take_registers<96>();
+        // ---- the state -----------------------------------------------------------
         const int col = 32 * (warp & 3) + lane;  // this thread's column of S (row of U^T),
-        const int half = (warp - 4) >> 2, b0 = 64 * half;  // and its rows b0 .. b0 + 63; of the
-        uint8_t* sb = sm + kOffSb + half * kHalf + col * 128;  // output, row col of the chunk
-        uint32_t n = 0;  // chunks begun                       // and those features
-        bool ok = true;
-        // 32-byte stores where every row piece is so aligned.
-        const bool wide = p.d_c % 16 == 0 && (reinterpret_cast<uintptr_t>(p.out) & 31) == 0;
+        const int half = (warp - 8) >> 2, b0 = 64 * half;  // and its rows b0 .. b0 + 63
+        uint8_t* sb = sm + kOffSb + half * kHalf + col * 128;
+        uint32_t n = 0;  // chunks begun
         uint64_t s[32];  // pairs of its rows
 #pragma unroll 1
         for (int id = blockIdx.x; ok && id < items; id += gridDim.x) {
             const Item it = item_of(p, id);
             const int nch = (it.len + kC - 1) / kC;
             const float g = p.log_decay[it.h];
-            const bool gentle = is_gentle(g);
             const int64_t rs_in = it.in_t ? 1 : p.d_c, rs_out = it.out_t ? 1 : p.d_c;
             const bool mine = col < p.d_c;
             if (it.in != nullptr && mine) {
@@ -602,126 +810,67 @@ la_tc(const LaCore p, const __grid_constant__ CUtensorMap ma,
 #pragma unroll
                 for (int j = 0; j < 32; ++j) s[j] = 0;
             }
-            // w^len in two parts (it is applied chunk after chunk); the output's
-            // row factor.
-            uint64_t hi2 = 0, lo2 = 0;
-            float ahead = 1.f;
+            uint64_t hi2 = 0, lo2 = 0;  // w^len in two parts: it is applied chunk after chunk
             int known = 0;
 #pragma unroll 1
-            for (int c = -1; c < nch; ++c) {
-                // The state's bf16 copy for chunk c + 1, once chunk c's product has read its own.
-                if (c >= 0) {
-                    const int len = chunk_len<kRev>(it, nch, c);
-                    if (len != known) {
-                        const float2 f = power2(g, len);
-                        hi2 = pair(f.x, f.x);
-                        lo2 = pair(f.y, f.y);
-                        ahead = gentle ? row_factor<kRev>(p, g, len, col) : 1.f;
-                        known = len;
-                    }
-                    if (!(ok = warp_wait(&B.u_full, n & 1))) break;
-                    tc_fence_after();
+            for (int c = 0; c < nch; ++c, ++n) {
+                // The bf16 copy, once the last chunk's product has read its own.
+                if (n > 0 && !(ok = group_wait(&B.in_full[(n - 1) & 1], ((n - 1) >> 1) & 1, 2, warp == 9))) break;
 #pragma unroll
-                    for (int blk = 0; blk < 4; ++blk) {
-                        uint64_t u[8];
-                        tmem_ld16(quad + kColU + b0 + 16 * blk, u);
-#pragma unroll
-                        for (int j = 0; j < 8; ++j)
-                            s[8 * blk + j] =
-                                fma2(s[8 * blk + j], hi2, fma2(s[8 * blk + j], lo2, u[j]));
-                    }
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&B.u_free);
+                for (int m = 0; m < 8; ++m)
+                    *reinterpret_cast<uint4*>(sb + ((m ^ (col & 7)) << 4)) =
+                        make_uint4(pack_bf16(s[4 * m]), pack_bf16(s[4 * m + 1]),
+                                   pack_bf16(s[4 * m + 2]), pack_bf16(s[4 * m + 3]));
+                fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&B.sb_ready);
+                const int len = chunk_len<kRev>(it, nch, c);
+                if (len != known) {
+                    const float2 f = power2(g, len);
+                    hi2 = pair(f.x, f.x);
+                    lo2 = pair(f.y, f.y);
+                    known = len;
                 }
-                if (c + 1 < nch) {
-                    const uint32_t before = c >= 0 ? n : n - 1;  // the last chunk begun
-                    if (n > 0 || c >= 0)
-                        if (!(ok = warp_wait(&B.in_full, before & 1))) break;
-#pragma unroll
-                    for (int m = 0; m < 8; ++m)
-                        *reinterpret_cast<uint4*>(sb + ((m ^ (col & 7)) << 4)) =
-                            make_uint4(pack_bf16(s[4 * m]), pack_bf16(s[4 * m + 1]),
-                                       pack_bf16(s[4 * m + 2]), pack_bf16(s[4 * m + 3]));
-                    fence_proxy_async();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&B.sb_ready);
-                }
-                if (c < 0) continue;
-                // The output: scaled, converted, stored from registers, 16 features
-                // of a row (one 32-byte sector) at a time; only rows of the sequence.
-                int64_t row;
-                int len;
-                chunk_of<kRev>(it, nch, c, row, len);
-                if (!(ok = warp_wait(&B.o_full, n & 1))) break;
+                if (!(ok = group_wait(&B.u_full[n & 1], (n >> 1) & 1, 2, warp == 9))) break;
                 tc_fence_after();
-                const bool live = col < len;
-                const uint64_t scale = pair(ahead, ahead);
-                const int64_t at = ((row + col) * p.heads + it.h) * p.d_c + b0;
-#pragma unroll 1
+#pragma unroll
                 for (int blk = 0; blk < 4; ++blk) {
                     uint64_t u[8];
-                    tmem_ld16(quad + kColO + b0 + 16 * blk, u);
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) u[j] = mul2(u[j], scale);
-                    const int left = p.d_c - b0 - 16 * blk;  // features of the row from here
-                    if (!live || left <= 0) continue;
-                    if (p.out_f32) {
-                        float* o = static_cast<float*>(p.out) + at + 16 * blk;
-#pragma unroll
-                        for (int j = 0; j < 4; ++j)
-                            if (4 * j < left) {
-                                float4 x;
-                                unpair(u[2 * j], x.x, x.y);
-                                unpair(u[2 * j + 1], x.z, x.w);
-                                reinterpret_cast<float4*>(o)[j] = x;
-                            }
-                    } else {
-                        uint32_t x[8];
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) x[j] = pack_bf16(u[j]);
-                        __nv_bfloat16* o = static_cast<__nv_bfloat16*>(p.out) + at + 16 * blk;
-                        if (wide) {
-                            asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
-                                         ::"l"(o), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]),
-                                         "r"(x[4]), "r"(x[5]), "r"(x[6]), "r"(x[7])
-                                         : "memory");
-                        } else {
-                            reinterpret_cast<uint4*>(o)[0] = make_uint4(x[0], x[1], x[2], x[3]);
-                            if (left > 8)
-                                reinterpret_cast<uint4*>(o)[1] = make_uint4(x[4], x[5], x[6], x[7]);
-                        }
+                    tmem_ld16(quad + kColU + b0 + 16 * blk, u);
+                    if (blk == 3) {
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&B.u_free);
                     }
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        s[8 * blk + j] = fma2(s[8 * blk + j], hi2, fma2(s[8 * blk + j], lo2, u[j]));
                 }
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&B.o_free);
-                ++n;
             }
             if (ok && it.out != nullptr && mine) {
                 float* dst = it.out + (it.out_t ? col * p.d_b : col) + b0 * rs_out;
 #pragma unroll
-                for (int j = 0; j < 32; ++j, dst += 2 * rs_out) {
-                    float x, y;
-                    unpair(s[j], x, y);
-                    if (b0 + 2 * j < p.d_b) dst[0] = x;
-                    if (b0 + 2 * j + 1 < p.d_b) dst[rs_out] = y;
+                for (int m = 0; m < 8; ++m) {  // (d_b is a multiple of 8)
+                    if (b0 + 8 * m >= p.d_b) break;
+#pragma unroll
+                    for (int j = 4 * m; j < 4 * m + 4; ++j, dst += 2 * rs_out)
+                        unpair(s[j], dst[0], dst[rs_out]);
                 }
             }
         }
     } else {
+        give_registers<64>();
         // ---- the update's operand ----------------------------------------------------
         // (w c)^T, features on the TMEM lanes: 8 x 8 blocks of the c tile come
         // transposed from ldmatrix, thread t holding feature t / 4 (and + 8)
         // at positions 2 (t % 4), + 1 of each 8, which is where tcgen05.st's
         // 16x128b shape puts them; a thread's weights stay in registers.
-        const int wc = warp - 12;
+        const int wc = warp & 3, half = (warp - 16) >> 2;  // 32 features, 16 of them
         const int row = ((lane >> 4) << 3) + (lane & 7);  // ldmatrix row of this lane
         const uint32_t src0 = smem_u32(sm) + 2 * kTile + (wc >> 1) * kHalf + row * 128;
-        const int chunk0 = 4 * (wc & 1) + ((lane >> 3) & 1);
+        const int chunk0 = 4 * (wc & 1) + 2 * half + ((lane >> 3) & 1);
         const uint64_t minus = pair(-1.f, -1.f);
         uint32_t n = 0, w = 0;
-        bool ok = true;
 #pragma unroll 1
         for (int id = blockIdx.x; ok && id < items; id += gridDim.x) {
             const Item it = item_of(p, id);
@@ -744,15 +893,15 @@ la_tc(const LaCore p, const __grid_constant__ CUtensorMap ma,
             for (int c = 0; c < nch; ++c, ++n) {
                 const int st = n & 1;
                 const int len = chunk_len<kRev>(it, nch, c);
-                if (!(ok = warp_wait(&B.c_full[st], (n >> 1) & 1))) break;
+                if (!(ok = group_wait(&B.c_full[st], (n >> 1) & 1, 3, warp == 18))) break;
                 if (len < kC) {
-                    if (!(ok = warp_wait(&B.b_full[st], (n >> 1) & 1))) break;
+                    if (!(ok = group_wait(&B.b_full[st], (n >> 1) & 1, 3, warp == 18))) break;
                     // The rows past the sequence hold another's (or anything):
                     // zeros, so that no product of theirs is NaN.
                     uint8_t* bt = sm + st * kStage + kTile;
                     uint8_t* tile = lane < 16 ? bt : bt + kTile;
 #pragma unroll 1
-                    for (int r = len + wc; r < kC; r += 4)
+                    for (int r = len + warp - 16; r < kC; r += 8)
                         *reinterpret_cast<uint4*>(tile + ((lane & 15) >> 3) * kHalf + r * 128 +
                                                   (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
                     fence_proxy_async();
@@ -762,22 +911,20 @@ la_tc(const LaCore p, const __grid_constant__ CUtensorMap ma,
 #pragma unroll 1
                 for (int q = 0; q < 4; ++q, ++w) {
                     const int buf = w & 1;
-                    uint32_t x[2][8];
+                    uint32_t x[8];
 #pragma unroll
-                    for (int half = 0; half < 2; ++half)
-#pragma unroll
-                        for (int g2 = 0; g2 < 2; ++g2)
-                            asm volatile(
-                                "ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16"
-                                " {%0, %1, %2, %3}, [%4];"
-                                : "=r"(x[half][4 * g2]), "=r"(x[half][4 * g2 + 1]),
-                                  "=r"(x[half][4 * g2 + 2]), "=r"(x[half][4 * g2 + 3])
-                                : "r"(src0 + st * kStage + (32 * q + 16 * g2) * 128 +
-                                      (((chunk0 + 2 * half) ^ (lane & 7)) << 4))
-                                : "memory");
+                    for (int g2 = 0; g2 < 2; ++g2)
+                        asm volatile(
+                            "ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16"
+                            " {%0, %1, %2, %3}, [%4];"
+                            : "=r"(x[4 * g2]), "=r"(x[4 * g2 + 1]), "=r"(x[4 * g2 + 2]),
+                              "=r"(x[4 * g2 + 3])
+                            : "r"(src0 + st * kStage + (32 * q + 16 * g2) * 128 +
+                                  ((chunk0 ^ (lane & 7)) << 4))
+                            : "memory");
                     if (q == 3) {
                         __syncwarp();
-                        if (lane == 0) mbar_arrive(&B.c_free[st]);
+                        if (lane == 0) mbar_arrive(&B.c_read[st]);
                     }
                     uint64_t f[4];
                     if (len == kC) {
@@ -805,32 +952,26 @@ la_tc(const LaCore p, const __grid_constant__ CUtensorMap ma,
                             f[k] = pair(v[0], v[1]);
                             const uint32_t keep =
                                 (j < live ? 0xffffu : 0u) | (j + 1 < live ? 0xffff0000u : 0u);
-#pragma unroll
-                            for (int half = 0; half < 2; ++half) {
-                                x[half][2 * k] &= keep;
-                                x[half][2 * k + 1] &= keep;
-                            }
+                            x[2 * k] &= keep;
+                            x[2 * k + 1] &= keep;
                         }
                     }
-                    if (w >= 2 && !(ok = warp_wait(&B.wv_free[buf], ((w >> 1) & 1) ^ 1))) break;
+                    if (w >= 2 && !(ok = group_wait(&B.wv_free[buf], ((w >> 1) & 1) ^ 1, 3, warp == 18))) break;
                     tc_fence_after();
+                    uint32_t mid[8], lo[8];
 #pragma unroll
-                    for (int half = 0; half < 2; ++half) {
-                        uint32_t mid[8], lo[8];
-#pragma unroll
-                        for (int k = 0; k < 8; ++k) {
-                            uint64_t v = mul2(widen(x[half][k]), f[k >> 1]);
-                            x[half][k] = pack_bf16(v);
-                            v = fma2(widen(x[half][k]), minus, v);
-                            mid[k] = pack_bf16(v);
-                            lo[k] = pack_bf16(fma2(widen(mid[k]), minus, v));
-                        }
-                        const uint32_t at =
-                            quad + (static_cast<uint32_t>(half) << 20) + kColW + buf * kColWBuf;
-                        tmem_st_16x128(at, x[half]);
-                        tmem_st_16x128(at + 16, mid);
-                        tmem_st_16x128(at + 32, lo);
+                    for (int k = 0; k < 8; ++k) {
+                        uint64_t v = mul2(widen(x[k]), f[k >> 1]);
+                        x[k] = pack_bf16(v);
+                        v = fma2(widen(x[k]), minus, v);
+                        mid[k] = pack_bf16(v);
+                        lo[k] = pack_bf16(fma2(widen(mid[k]), minus, v));
                     }
+                    const uint32_t at =
+                        quad + (static_cast<uint32_t>(half) << 20) + kColW + buf * kColWBuf;
+                    tmem_st_16x128(at, x);
+                    tmem_st_16x128(at + 16, mid);
+                    tmem_st_16x128(at + 32, lo);
                     tmem_wait_st();
                     tc_fence_before();
                     __syncwarp();
@@ -840,10 +981,11 @@ la_tc(const LaCore p, const __grid_constant__ CUtensorMap ma,
             }
         }
     }
+    if (!ok && lane == 0) atomicOr(&g_la_error, 1);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    if (warp == 18) tmem_dealloc(tm, 512);
+    if (warp == 26) tmem_dealloc(B.tmem, 512);
 }
 
 PFN_cuTensorMapEncodeTiled_v12000 encoder() {
@@ -859,19 +1001,23 @@ PFN_cuTensorMapEncodeTiled_v12000 encoder() {
     return fn;
 }
 
-// [tokens, heads, d] bf16 in boxes of 64 features x 1 head x 128 positions;
-// features past d read as zeros.
-bool tile_map(CUtensorMap* map, const void* base, int64_t tokens, int heads, int d) {
+// [tokens, heads, d] bf16 or f32 in boxes of 128 bytes of features x 1 head x
+// `rows` positions; features past d read as zeros and are not written.
+bool tile_map(CUtensorMap* map, const void* base, int64_t tokens, int heads, int d, int rows,
+              bool f32 = false) {
     auto encode = encoder();
     if (encode == nullptr) return false;
+    const cuuint64_t es = f32 ? 4 : 2;
     const cuuint64_t dims[3] = {static_cast<cuuint64_t>(d), static_cast<cuuint64_t>(heads),
                                 static_cast<cuuint64_t>(tokens)};
-    const cuuint64_t strides[2] = {static_cast<cuuint64_t>(d) * 2,
-                                   static_cast<cuuint64_t>(heads) * d * 2};
-    const cuuint32_t box[3] = {64, 1, static_cast<cuuint32_t>(kC)};
+    const cuuint64_t strides[2] = {d * es, static_cast<cuuint64_t>(heads) * d * es};
+    const cuuint32_t box[3] = {static_cast<cuuint32_t>(128 / es), 1,
+                               static_cast<cuuint32_t>(rows)};
     const cuuint32_t estride[3] = {1, 1, 1};
-    return encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides,
-                  box, estride, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+    return encode(map,
+                  f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
+                  const_cast<void*>(base), dims, strides, box, estride,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
@@ -895,11 +1041,12 @@ bool la_tc_supports(const LaCore& p) {
 }
 
 cudaError_t launch_la_tc(const LaCore& p, cudaStream_t stream) {
-    CUtensorMap ma, mb, mc;
+    CUtensorMap ma, mb, mc, mo;
     const int64_t tokens = la_tokens(p);
-    if (!tile_map(&ma, p.a, tokens, p.heads_a, p.d_b) ||
-        !tile_map(&mb, p.b, tokens, p.heads_b, p.d_b) ||
-        !tile_map(&mc, p.c, tokens, p.heads_c, p.d_c))
+    if (!tile_map(&ma, p.a, tokens, p.heads_a, p.d_b, kC) ||
+        !tile_map(&mb, p.b, tokens, p.heads_b, p.d_b, kC) ||
+        !tile_map(&mc, p.c, tokens, p.heads_c, p.d_c, kC) ||
+        !tile_map(&mo, p.out, tokens, p.heads, p.d_c, 32, p.out_f32 != 0))
         return cudaErrorInvalidValue;
     auto* kernel = p.reverse ? la_tc<true> : la_tc<false>;
     const cudaError_t e = cudaFuncSetAttribute(
@@ -907,7 +1054,7 @@ cudaError_t launch_la_tc(const LaCore& p, cudaStream_t stream) {
     if (e != cudaSuccess) return e;
     const int64_t items = static_cast<int64_t>(p.n_seqs) * p.heads;
     const int grid = static_cast<int>(std::min<int64_t>(items, sm_count()));
-    kernel<<<grid, kThreads, kSmemBytes, stream>>>(p, ma, mb, mc, static_cast<int>(items));
+    kernel<<<grid, kThreads, kSmemBytes, stream>>>(p, ma, mb, mc, mo, static_cast<int>(items));
     return cudaGetLastError();
 }
 
