@@ -58,7 +58,9 @@ __device__ __forceinline__ void la_span(const LaCore& p, int s, int64_t& start, 
 // Kernels of the core (each its own file) and what they take.
 cudaError_t launch_la_recurrent(const LaCore& p, cudaStream_t stream);
 bool la_tc_supports(const LaCore& p);
-cudaError_t launch_la_tc(const LaCore& p, cudaStream_t stream);
+// split: long sequences may go in segments (scratch from the library's pool);
+// must: they do even where it looks slower; forced: segment length in chunks, or 0.
+cudaError_t launch_la_tc(const LaCore& p, bool split, bool must, int forced, cudaStream_t stream);
 cudaError_t take_la_error(int* flag);
 constexpr int kLaMaxD = 256;  // d_k, d_v of any kernel here
 

@@ -105,7 +105,9 @@ cudaError_t run_core(const gdr_la_params& a, const LaCore& p, bool chunked, cuda
     if (!chunked || la_tokens(p) == 0) return launch_la_recurrent(p, s);
     const bool tc = la_tc_supports(p);
     if (!tc && a.algo >= GDR_ALGO_TENSOR) return cudaErrorNotSupported;
-    if (tc && a.algo != GDR_ALGO_CUDA_CORE) return launch_la_tc(p, s);
+    if (tc && a.algo != GDR_ALGO_CUDA_CORE)
+        return launch_la_tc(p, a.algo != GDR_ALGO_TENSOR, a.algo == GDR_ALGO_TENSOR_SPLIT,
+                            a.split_chunks, s);
     return launch_la_recurrent(p, s);
 }
 

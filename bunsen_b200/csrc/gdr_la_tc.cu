@@ -47,11 +47,14 @@
 #include <cudaTypedefs.h>
 
 #include <algorithm>
+#include <cmath>
 
 #include "gdr_la.cuh"
 #include "gdr_sm100.cuh"
 
 namespace gdr {
+
+cudaError_t library_pool(cudaMemPool_t* pool, bool create);
 
 // Device-side failures since the last gdr_device_error: bit 0, a bounded wait
 // ran out.
@@ -69,23 +72,24 @@ constexpr uint32_t kStage = 3 * kTile;    // a, b, c
 constexpr uint32_t kOffSb = 2 * kStage, kOffMisc = kOffSb + kTile;
 constexpr uint32_t kSmemBytes = kOffMisc + 512;
 constexpr uint32_t kColU = 0, kColP = 128, kColO = 256, kColW = 384, kColWBuf = 48;
+constexpr int64_t kStateBudget = int64_t{2} << 30;  // scratch states of a split call, bytes
 constexpr int kWaitRounds = 1 << 24;  // of two tries: seconds
+
+// What a CTA works on next: the positions [start, start + len) of a sequence with
+// head h, from state `in` to state `out` (see state_at); len < 0: nothing more.
+struct Job {
+    int start, len, h, in, out;
+};
+constexpr int kJobs = 4;  // in flight between the loading warp and the other roles
 
 struct Bars {
     uint64_t a_full[2], b_full[2], c_full[2], a_free[2], c_read[2], o_staged[2];
     uint64_t in_full[2], o_full[2], u_full[2];
     uint64_t sc_full, pa_ready, sb_ready, o_free, u_free, fix[2], drain[2];
     uint64_t wv_full[2], wv_free[2];
+    uint64_t job_full[kJobs], job_free[kJobs];
     uint32_t tmem;
-};
-
-// One (sequence or segment, head) of a pass.
-struct Item {
-    int64_t start;
-    int len, h;
-    const float* in;  // state before it (null: zeros)
-    float* out;       // state after it (null: not wanted)
-    bool in_t, out_t;  // stored [d_c, d_b]
+    Job jobs[kJobs];
 };
 
 // Waits for a phase; false once the tries ran out. A try suspends the warp for
@@ -356,38 +360,53 @@ __device__ __forceinline__ float2 power2(float g, int n) {
 // Heads whose decay's powers to w^-128 are far from overflow (e^51).
 __device__ __forceinline__ bool is_gentle(float g) { return g >= -0.4f && g <= 0.4f; }
 
-__device__ __forceinline__ Item item_of(const LaCore& p, int id) {
-    Item it;
-    const int s = id / p.heads;
-    it.h = id - s * p.heads;
-    int64_t end;
-    la_span(p, s, it.start, end);
-    it.len = static_cast<int>(end - it.start);
-    const int64_t at = static_cast<int64_t>(id) * p.d_b * p.d_c;
-    it.in = p.state_in != nullptr ? p.state_in + at : nullptr;
-    it.out = p.state_out != nullptr ? p.state_out + at : nullptr;
-    it.in_t = it.out_t = p.state_t != 0;
-    return it;
+// A list of work in device memory, made by la_plan: entries of positions and states,
+// each for every head, the longest first. null: one job a CTA, its sequence and
+// head by its index.
+struct Work {
+    int32_t count;    // entries
+    int32_t next;     // the next job not handed out (entry x heads + head)
+};
+struct Entry {
+    int32_t start, len, in, out;
+};
+
+// States by index: the call's own of sequence x >= 0, none (-1: zeros, or not
+// wanted), or segment -2 - x's in the scratch. Null, or row `r` columns `c` apart.
+struct StateAt {
+    const float* ptr;
+    int64_t row, col;
+};
+__device__ __forceinline__ StateAt state_at(const LaCore& p, int x, int h, const float* own,
+                                            const float* scratch) {
+    const int64_t size = static_cast<int64_t>(p.d_b) * p.d_c;
+    const float* base = x >= 0 ? own : x == -1 ? nullptr : scratch;
+    const bool turned = x >= 0 && p.state_t;
+    return {base != nullptr
+                ? base + (static_cast<int64_t>(x >= 0 ? x : -2 - x) * p.heads + h) * size
+                : nullptr,
+            turned ? 1 : p.d_c, turned ? p.d_b : 1};
 }
 
 // Chunk c of an item, in the order they run: its length, and its first row.
 template <bool kRev>
-__device__ __forceinline__ int chunk_len(const Item& it, int nch, int c) {
+__device__ __forceinline__ int chunk_len(const Job& it, int nch, int c) {
     return min(kC, it.len - (kRev ? nch - 1 - c : c) * kC);
 }
 template <bool kRev>
-__device__ __forceinline__ void chunk_of(const Item& it, int nch, int c,
+__device__ __forceinline__ void chunk_of(const Job& it, int nch, int c,
                                          int64_t& row, int& len) {
     const int x = kRev ? nch - 1 - c : c;
-    row = it.start + static_cast<int64_t>(x) * kC;
+    row = static_cast<int64_t>(it.start) + x * kC;
     len = min(kC, it.len - x * kC);
 }
 
-template <bool kRev>
+// kStateOnly: only the state after the positions is wanted (no a, no output).
+template <bool kRev, bool kStateOnly>
 __global__ void __launch_bounds__(kThreads, 1)
 la_tc(const LaCore p, const __grid_constant__ CUtensorMap ma,
       const __grid_constant__ CUtensorMap mb, const __grid_constant__ CUtensorMap mc,
-      const __grid_constant__ CUtensorMap mo, int items) {
+      const __grid_constant__ CUtensorMap mo, Work* work, const Entry* entries, float* scratch) {
     extern __shared__ __align__(1024) uint8_t sm[];  // (checked below: swizzled tiles need it)
     Bars& B = *reinterpret_cast<Bars*>(sm + kOffMisc);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -407,6 +426,10 @@ la_tc(const LaCore p, const __grid_constant__ CUtensorMap ma,
             mbar_init(&B.wv_free[i], 1);
             mbar_init(&B.drain[i], 1);
         }
+        for (int i = 0; i < kJobs; ++i) {
+            mbar_init(&B.job_full[i], 1);
+            mbar_init(&B.job_free[i], kStateOnly ? 17 : 27);  // every warp that reads it
+        }
         mbar_init(&B.sc_full, 1);
         mbar_init(&B.pa_ready, 8);
         mbar_init(&B.o_free, 8);
@@ -425,8 +448,14 @@ la_tc(const LaCore p, const __grid_constant__ CUtensorMap ma,
     // All 512 columns are this CTA's, so they begin at 0: a constant, as the
     // tiles' addresses are, keeps the products' operands in uniform registers.
     constexpr uint32_t tm = 0;
-    if (B.tmem != 0 || (smem_u32(sm) & 1023) != 0) items = 0;  // never: nothing would be right
-    if (items == 0) ok = false;
+    if (B.tmem != 0 || (smem_u32(sm) & 1023) != 0) ok = false;  // never: nothing would be right
+    // The job of a slot that is full, and the slot given back (its warp converged).
+    auto take = [&](uint32_t slot) {
+        const Job j = B.jobs[slot];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&B.job_free[slot]);
+        return j;
+    };
     const uint32_t quad = tm + (static_cast<uint32_t>(warp & 3) << 21);  // this warp's lanes
 
     if (warp >= 24) {
@@ -435,9 +464,38 @@ la_tc(const LaCore p, const __grid_constant__ CUtensorMap ma,
         // ---- loads -------------------------------------------------------------
         {
             uint32_t n = 0;
+            const int heads = p.heads;
+            const int jobs = work != nullptr ? work->count * heads : p.n_seqs * heads;
 #pragma unroll 1
-            for (int id = blockIdx.x; ok && id < items; id += gridDim.x) {
-                const Item it = item_of(p, id);
+            for (uint32_t k = 0; ok; ++k) {
+                const uint32_t slot = k % kJobs;
+                if (k >= kJobs && !(ok = warp_wait(&B.job_free[slot], (k / kJobs & 1) ^ 1))) break;
+                int id = k == 0 ? static_cast<int>(blockIdx.x) : jobs;
+                if (work != nullptr && k > 0) {
+                    if (lane == 0) id = atomicAdd(&work->next, 1);
+                    id = __shfl_sync(0xffffffffu, id, 0);
+                }
+                Job it{0, -1, 0, -1, -1};
+                if (id < jobs) {
+                    const int e = id / heads;
+                    it.h = id - e * heads;
+                    if (work != nullptr) {
+                        const Entry x = entries[e];
+                        it.start = x.start, it.len = x.len, it.in = x.in, it.out = x.out;
+                    } else {
+                        int64_t start, end;
+                        la_span(p, e, start, end);
+                        it.start = static_cast<int>(start);
+                        it.len = static_cast<int>(end - start);
+                        it.in = it.out = e;
+                    }
+                }
+                if (lane == 0) {
+                    B.jobs[slot] = it;
+                    mbar_arrive(&B.job_full[slot]);
+                }
+                __syncwarp();
+                if (it.len < 0) break;
                 const int nch = (it.len + kC - 1) / kC;
                 const int ha = it.h / (p.heads / p.heads_a), hb = it.h / (p.heads / p.heads_b),
                           hc = it.h / (p.heads / p.heads_c);
@@ -459,13 +517,16 @@ la_tc(const LaCore p, const __grid_constant__ CUtensorMap ma,
                     };
                     // Chunk n - 2: its products with b and with c are done, its operand's
                     // warps have read c, and its output has left the tiles.
-                    if (n >= 2 && !(ok = warp_wait(&B.in_full[st], ph))) break;
+                    if (!kStateOnly && n >= 2 && !(ok = warp_wait(&B.in_full[st], ph))) break;
                     if (n >= 2 && !(ok = warp_wait(&B.u_full[st], ph))) break;
                     load(&B.b_full[st], base + kTile, &mb, hb);
-                    if (n >= 2 && p.out_f32 && !(ok = warp_wait(&B.a_free[st], ph))) break;
-                    if (n >= 2 && !(ok = warp_wait(&B.o_full[st], ph))) break;
+                    if (!kStateOnly && n >= 2) {
+                        if (p.out_f32 && !(ok = warp_wait(&B.a_free[st], ph))) break;
+                        if (!(ok = warp_wait(&B.o_full[st], ph))) break;
+                    }
                     if (n >= 2 && !(ok = warp_wait(&B.c_read[st], ph))) break;
                     load(&B.c_full[st], base + 2 * kTile, &mc, hc);
+                    if (kStateOnly) continue;
                     if (n >= 2 && !(ok = warp_wait(&B.a_free[st], ph))) break;
                     load(&B.a_full[st], base, &ma, ha);
                 }
@@ -473,11 +534,11 @@ la_tc(const LaCore p, const __grid_constant__ CUtensorMap ma,
             // Nothing of this CTA's may be in flight when it ends.
 #pragma unroll 1
             for (uint32_t i = n >= 2 ? n - 2 : 0; i < n + (ok ? 0 : 1); ++i)
-                for (uint64_t* full : {B.a_full, B.b_full, B.c_full})
+                for (uint64_t* full : {B.b_full, B.c_full, kStateOnly ? B.b_full : B.a_full})
                     warp_wait(&full[i & 1], (i >> 1) & 1);
         }
         __syncwarp();
-    } else if (warp == 25) {
+    } else if (!kStateOnly && warp == 25) {
         // ---- the outputs' products -------------------------------------------------
         {
             constexpr uint32_t kKK = idesc_bf16(128, 128, 0, 0, 0);
@@ -493,8 +554,10 @@ la_tc(const LaCore p, const __grid_constant__ CUtensorMap ma,
             };
             uint32_t n = 0, tails = 0;
 #pragma unroll 1
-            for (int id = blockIdx.x; ok && id < items; id += gridDim.x) {
-                const Item it = item_of(p, id);
+            for (uint32_t k = 0; ok; ++k) {
+                if (!(ok = warp_wait(&B.job_full[k % kJobs], k / kJobs & 1))) break;
+                const Job it = take(k % kJobs);
+                if (it.len < 0) break;
                 const int nch = (it.len + kC - 1) / kC;
 #pragma unroll 1
                 for (int c = 0; c < nch; ++c, ++n) {
@@ -542,8 +605,10 @@ la_tc(const LaCore p, const __grid_constant__ CUtensorMap ma,
             };
             uint32_t n = 0, tails = 0;
 #pragma unroll 1
-            for (int id = blockIdx.x; ok && id < items; id += gridDim.x) {
-                const Item it = item_of(p, id);
+            for (uint32_t k = 0; ok; ++k) {
+                if (!(ok = warp_wait(&B.job_full[k % kJobs], k / kJobs & 1))) break;
+                const Job it = take(k % kJobs);
+                if (it.len < 0) break;
                 const int nch = (it.len + kC - 1) / kC;
 #pragma unroll 1
                 for (int c = 0; c < nch; ++c, ++n) {
@@ -572,12 +637,14 @@ la_tc(const LaCore p, const __grid_constant__ CUtensorMap ma,
             warp_wait(&B.drain[1], 0);
         }
         __syncwarp();
-    } else if (warp == 27) {
+    } else if (!kStateOnly && warp == 27) {
         // ---- the outputs' stores -----------------------------------------------------
         uint32_t n = 0;
 #pragma unroll 1
-        for (int id = blockIdx.x; ok && id < items; id += gridDim.x) {
-            const Item it = item_of(p, id);
+        for (uint32_t k = 0; ok; ++k) {
+            if (!(ok = warp_wait(&B.job_full[k % kJobs], k / kJobs & 1))) break;
+            const Job it = take(k % kJobs);
+            if (it.len < 0) break;
             const int nch = (it.len + kC - 1) / kC;
 #pragma unroll 1
             for (int c = 0; c < nch; ++c, ++n) {
@@ -640,8 +707,10 @@ la_tc(const LaCore p, const __grid_constant__ CUtensorMap ma,
         const uint32_t pcol = quad + kColP + 64 * half;  // P's and the scores' columns
         uint32_t n = 0;
 #pragma unroll 1
-        for (int id = blockIdx.x; ok && id < items; id += gridDim.x) {
-            const Item it = item_of(p, id);
+        for (uint32_t k = 0; !kStateOnly && ok; ++k) {
+            if (!(ok = group_wait(&B.job_full[k % kJobs], k / kJobs & 1, 1, warp == 0))) break;
+            const Job it = take(k % kJobs);
+            if (it.len < 0) break;
             const int nch = (it.len + kC - 1) / kC;
             const float g = p.log_decay[it.h], w = power(g, 1);
             const bool gentle = is_gentle(g);
@@ -794,36 +863,42 @@ la_tc(const LaCore p, const __grid_constant__ CUtensorMap ma,
         uint32_t n = 0;  // chunks begun
         uint64_t s[32];  // pairs of its rows
 #pragma unroll 1
-        for (int id = blockIdx.x; ok && id < items; id += gridDim.x) {
-            const Item it = item_of(p, id);
+        for (uint32_t k = 0; ok; ++k) {
+            if (!(ok = group_wait(&B.job_full[k % kJobs], k / kJobs & 1, 2, warp == 9))) break;
+            const Job it = take(k % kJobs);
+            if (it.len < 0) break;
             const int nch = (it.len + kC - 1) / kC;
             const float g = p.log_decay[it.h];
-            const int64_t rs_in = it.in_t ? 1 : p.d_c, rs_out = it.out_t ? 1 : p.d_c;
             const bool mine = col < p.d_c;
-            if (it.in != nullptr && mine) {
-                const float* src = it.in + (it.in_t ? col * p.d_b : col) + b0 * rs_in;
+            {
+                const StateAt in = state_at(p, it.in, it.h, p.state_in, scratch);
+                if (in.ptr != nullptr && mine) {
+                    const float* src = in.ptr + col * in.col + b0 * in.row;
 #pragma unroll
-                for (int j = 0; j < 32; ++j, src += 2 * rs_in)
-                    s[j] = pair(b0 + 2 * j < p.d_b ? src[0] : 0.f,
-                                b0 + 2 * j + 1 < p.d_b ? src[rs_in] : 0.f);
-            } else {
+                    for (int j = 0; j < 32; ++j, src += 2 * in.row)
+                        s[j] = pair(b0 + 2 * j < p.d_b ? src[0] : 0.f,
+                                    b0 + 2 * j + 1 < p.d_b ? src[in.row] : 0.f);
+                } else {
 #pragma unroll
-                for (int j = 0; j < 32; ++j) s[j] = 0;
+                    for (int j = 0; j < 32; ++j) s[j] = 0;
+                }
             }
             uint64_t hi2 = 0, lo2 = 0;  // w^len in two parts: it is applied chunk after chunk
             int known = 0;
 #pragma unroll 1
             for (int c = 0; c < nch; ++c, ++n) {
-                // The bf16 copy, once the last chunk's product has read its own.
-                if (n > 0 && !(ok = group_wait(&B.in_full[(n - 1) & 1], ((n - 1) >> 1) & 1, 2, warp == 9))) break;
+                if constexpr (!kStateOnly) {
+                    // The bf16 copy, once the last chunk's product has read its own.
+                    if (n > 0 && !(ok = group_wait(&B.in_full[(n - 1) & 1], ((n - 1) >> 1) & 1, 2, warp == 9))) break;
 #pragma unroll
-                for (int m = 0; m < 8; ++m)
-                    *reinterpret_cast<uint4*>(sb + ((m ^ (col & 7)) << 4)) =
-                        make_uint4(pack_bf16(s[4 * m]), pack_bf16(s[4 * m + 1]),
-                                   pack_bf16(s[4 * m + 2]), pack_bf16(s[4 * m + 3]));
-                fence_proxy_async();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&B.sb_ready);
+                    for (int m = 0; m < 8; ++m)
+                        *reinterpret_cast<uint4*>(sb + ((m ^ (col & 7)) << 4)) =
+                            make_uint4(pack_bf16(s[4 * m]), pack_bf16(s[4 * m + 1]),
+                                       pack_bf16(s[4 * m + 2]), pack_bf16(s[4 * m + 3]));
+                    fence_proxy_async();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&B.sb_ready);
+                }
                 const int len = chunk_len<kRev>(it, nch, c);
                 if (len != known) {
                     const float2 f = power2(g, len);
@@ -847,14 +922,15 @@ la_tc(const LaCore p, const __grid_constant__ CUtensorMap ma,
                         s[8 * blk + j] = fma2(s[8 * blk + j], hi2, fma2(s[8 * blk + j], lo2, u[j]));
                 }
             }
-            if (ok && it.out != nullptr && mine) {
-                float* dst = it.out + (it.out_t ? col * p.d_b : col) + b0 * rs_out;
+            const StateAt out = state_at(p, it.out, it.h, p.state_out, scratch);
+            if (ok && out.ptr != nullptr && mine) {
+                float* dst = const_cast<float*>(out.ptr) + col * out.col + b0 * out.row;
 #pragma unroll
                 for (int m = 0; m < 8; ++m) {  // (d_b is a multiple of 8)
                     if (b0 + 8 * m >= p.d_b) break;
 #pragma unroll
-                    for (int j = 4 * m; j < 4 * m + 4; ++j, dst += 2 * rs_out)
-                        unpair(s[j], dst[0], dst[rs_out]);
+                    for (int j = 4 * m; j < 4 * m + 4; ++j, dst += 2 * out.row)
+                        unpair(s[j], dst[0], dst[out.row]);
                 }
             }
         }
@@ -872,8 +948,10 @@ la_tc(const LaCore p, const __grid_constant__ CUtensorMap ma,
         const uint64_t minus = pair(-1.f, -1.f);
         uint32_t n = 0, w = 0;
 #pragma unroll 1
-        for (int id = blockIdx.x; ok && id < items; id += gridDim.x) {
-            const Item it = item_of(p, id);
+        for (uint32_t k = 0; ok; ++k) {
+            if (!(ok = group_wait(&B.job_full[k % kJobs], k / kJobs & 1, 3, warp == 18))) break;
+            const Job it = take(k % kJobs);
+            if (it.len < 0) break;
             const int nch = (it.len + kC - 1) / kC;
             const float g = p.log_decay[it.h];
             // Of position j = 32 q + jj, jj = 8 k + 2 (t % 4) + e, in a whole chunk:
@@ -988,6 +1066,211 @@ la_tc(const LaCore p, const __grid_constant__ CUtensorMap ma,
     if (warp == 26) tmem_dealloc(B.tmem, 512);
 }
 
+// ---- sequences in segments ------------------------------------------------------
+// A state passes through positions as S -> w^n S + B, B what they reach from zero.
+// So a long sequence, which one CTA would walk alone, goes in segments of L chunks:
+// one pass finds the B of every segment but the last (in the order of time), a
+// scan the states before the segments, and the main pass runs all segments at once.
+// The first pass reads b and c again: it is worth it where the longest
+// sequences would bound the call. la_plan decides from the lengths, which only
+// the device has.
+struct Split {
+    int32_t base, parts, seq, unused;  // segment r's state: slot base + r, r >= 1
+};
+struct Plan {
+    Work main, states;
+    int32_t splits, seg_tokens;
+    int32_t pad[2];
+};
+
+constexpr int kPlanThreads = 1024, kBuckets = 1024;
+// Costs in chunks of the main pass (3.8 us a chunk at one CTA an SM): a chunk of the
+// first pass, and what two more passes and a scan cost at all.
+constexpr float kStateCost = 0.55f, kSplitCost = 3.f, kLinkCost = 0.05f;
+
+// The block's sum (op 0) or maximum (op 1) of x.
+__device__ int block_reduce(int x, bool maximum, int* ws) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    for (int o = 16; o > 0; o >>= 1) {
+        const int y = __shfl_xor_sync(0xffffffffu, x, o);
+        x = maximum ? max(x, y) : x + y;
+    }
+    __syncthreads();
+    if (lane == 0) ws[warp] = x;
+    __syncthreads();
+    x = ws[lane];
+    for (int o = 16; o > 0; o >>= 1) {
+        const int y = __shfl_xor_sync(0xffffffffu, x, o);
+        x = maximum ? max(x, y) : x + y;
+    }
+    return x;
+}
+
+// The work lists: every sequence, or its segments, the longest first (by buckets of
+// chunk counts), and the first pass's segments. seg_cap: state slots; 0: no
+// splitting. forced: a given segment length.
+__global__ void __launch_bounds__(kPlanThreads)
+la_plan(const LaCore p, Plan* plan, Entry* main, Entry* states, Split* splits, int32_t* base,
+        int grid, int l_min, int seg_cap, int forced, bool must) {
+    __shared__ int ws[32], hist[kBuckets], slots, n_splits, n_states;
+    __shared__ float cost[32];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    auto chunks = [&](int s, int64_t& start, int64_t& len) {
+        int64_t end;
+        la_span(p, s, start, end);
+        len = end - start;
+        return static_cast<int>((len + kC - 1) / kC);
+    };
+    int64_t start, len;
+    int sum = 0, most = 0;
+    for (int s = tid; s < p.n_seqs; s += kPlanThreads) {
+        const int c = chunks(s, start, len);
+        sum += c;
+        most = max(most, c);
+    }
+    sum = block_reduce(sum, false, ws);
+    most = block_reduce(most, true, ws);
+    // Candidate lengths from l_min to the longest sequence, one a warp.
+    const float each = static_cast<float>(p.heads) / grid;
+    auto candidate = [&](int i) {
+        return forced > 0 ? forced
+                          : max(l_min, static_cast<int>(l_min * powf(fmaxf(1.f, static_cast<float>(most) / l_min),
+                                                                     i / 31.f)));
+    };
+    {
+        const int L = candidate(warp);
+        int again = 0, parts_most = 0, segs = 0;
+        for (int s = lane; s < p.n_seqs; s += 32) {
+            const int c = chunks(s, start, len);
+            if (c > L) {
+                const int parts = (c + L - 1) / L;
+                again += (parts - 1) * L;
+                segs += parts;
+                parts_most = max(parts_most, parts);
+            }
+        }
+        for (int o = 16; o > 0; o >>= 1) {
+            again += __shfl_xor_sync(0xffffffffu, again, o);
+            segs += __shfl_xor_sync(0xffffffffu, segs, o);
+            parts_most = max(parts_most, __shfl_xor_sync(0xffffffffu, parts_most, o));
+        }
+        const float longest = static_cast<float>(min(L, most));
+        float t = fmaxf(longest, sum * each * 1.03f + 1.f);
+        if (again > 0)
+            t += kStateCost * fmaxf(longest, again * each * 1.03f + 1.f) + kSplitCost +
+                 kLinkCost * parts_most;
+        if (segs > seg_cap) t = INFINITY;
+        if (lane == 0) cost[warp] = t;
+    }
+    __syncthreads();
+    int L = most > 0 ? most : 1;  // not split
+    if (seg_cap > 0) {
+        float best = must || forced > 0 ? INFINITY
+                                        : 0.97f * fmaxf(static_cast<float>(most), sum * each * 1.03f + 1.f);
+        for (int i = 0; i < 32; ++i)
+            if (cost[i] < best) {
+                best = cost[i];
+                L = candidate(i);
+            }
+    }
+    const int shift = max(0, 32 - __clz(min(L, most)) - 10);  // bucket: chunks >> shift
+    for (int i = tid; i < kBuckets; i += kPlanThreads) hist[i] = 0;
+    if (tid == 0) slots = n_splits = n_states = 0;
+    __syncthreads();
+    auto bucket = [&](int c) { return kBuckets - 1 - (c >> shift); };  // longest first
+    for (int s = tid; s < p.n_seqs; s += kPlanThreads) {
+        const int c = chunks(s, start, len);
+        int parts = c > L ? (c + L - 1) / L : 1, at = 0;
+        if (parts > 1) at = atomicAdd(&slots, parts);
+        base[s] = at;
+        if (parts > 1) {
+            atomicAdd(&hist[bucket(L)], parts - 1);
+            atomicAdd(&hist[bucket(c - (parts - 1) * L)], 1);
+        } else {
+            atomicAdd(&hist[bucket(c)], 1);
+        }
+    }
+    __syncthreads();
+    // Exclusive scan of the buckets (as many as threads).
+    int x = hist[tid];
+    const int mine = x;
+    for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+    }
+    __syncthreads();
+    if (lane == 31) ws[warp] = x;
+    __syncthreads();
+    int before = 0;
+    for (int i = 0; i < warp; ++i) before += ws[i];
+    __syncthreads();
+    hist[tid] = before + x - mine;
+    __syncthreads();
+    for (int s = tid; s < p.n_seqs; s += kPlanThreads) {
+        const int c = chunks(s, start, len);
+        const int parts = c > L ? (c + L - 1) / L : 1;
+        if (parts == 1) {
+            main[atomicAdd(&hist[bucket(c)], 1)] = {static_cast<int32_t>(start),
+                                                    static_cast<int32_t>(len), s, s};
+            continue;
+        }
+        splits[atomicAdd(&n_splits, 1)] = {base[s], parts, s, 0};
+        for (int r = 0; r < parts; ++r) {  // in the order of time
+            const int part = p.reverse ? parts - 1 - r : r;
+            const int from = part * L, n = min(L, c - from);
+            const int32_t t0 = static_cast<int32_t>(start) + from * kC;
+            const int32_t tokens = min(n * kC, static_cast<int32_t>(len) - from * kC);
+            main[atomicAdd(&hist[bucket(n)], 1)] = {t0, tokens, r == 0 ? s : -2 - (base[s] + r),
+                                                    r == parts - 1 ? s : -1};
+            if (r < parts - 1)
+                states[atomicAdd(&n_states, 1)] = {t0, tokens, -1, -2 - (base[s] + r + 1)};
+        }
+    }
+    __syncthreads();
+    if (tid == 0) {
+        plan->main = {p.n_seqs + slots - n_splits, grid};
+        plan->states = {n_states, grid};
+        plan->splits = n_splits;
+        plan->seg_tokens = L * kC;
+    }
+}
+
+// S_{r+1} = w^(tokens of r) S_r + B_r, in place: slot base + r + 1 holds B_r. Four
+// elements a thread, every link's load issued ahead of the products.
+__global__ void __launch_bounds__(256)
+la_scan(const LaCore p, const Plan* plan, const Split* splits, float* scratch) {
+    const int size = p.d_b * p.d_c, tiles = (size + 1023) / 1024;
+    const int64_t jobs = static_cast<int64_t>(plan->splits) * p.heads * tiles;
+    for (int64_t job = blockIdx.x; job < jobs; job += gridDim.x) {
+        const int tile = static_cast<int>(job % tiles);
+        const int h = static_cast<int>(job / tiles % p.heads);
+        const Split sp = splits[job / tiles / p.heads];
+        const int e = tile * 1024 + 4 * threadIdx.x;
+        if (e >= size) continue;
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+        const StateAt in = state_at(p, sp.seq, h, p.state_in, scratch);
+        if (in.ptr != nullptr) {
+            const float* src = in.ptr + (e / p.d_c) * in.row + (e % p.d_c) * in.col;
+            x = make_float4(src[0], src[in.col], src[2 * in.col], src[3 * in.col]);
+        }
+        int64_t start, end;
+        la_span(p, sp.seq, start, end);
+        const float g = p.log_decay[h];
+        const int last = static_cast<int>(end - start) - (sp.parts - 1) * plan->seg_tokens;
+        const float w = power(g, plan->seg_tokens);
+        float* slot = scratch + (static_cast<int64_t>(sp.base + 1) * p.heads + h) * size + e;
+        const int64_t step = static_cast<int64_t>(p.heads) * size;
+#pragma unroll 4
+        for (int r = 0; r < sp.parts - 1; ++r, slot += step) {
+            const float f = p.reverse && r == 0 ? power(g, last) : w;
+            const float4 b = *reinterpret_cast<const float4*>(slot);
+            x = make_float4(fmaf(f, x.x, b.x), fmaf(f, x.y, b.y), fmaf(f, x.z, b.z),
+                            fmaf(f, x.w, b.w));
+            *reinterpret_cast<float4*>(slot) = x;
+        }
+    }
+}
+
 PFN_cuTensorMapEncodeTiled_v12000 encoder() {
     static PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
         void* ptr = nullptr;
@@ -1040,7 +1323,7 @@ bool la_tc_supports(const LaCore& p) {
            static_cast<int64_t>(p.n_seqs) * p.heads < (int64_t{1} << 30);
 }
 
-cudaError_t launch_la_tc(const LaCore& p, cudaStream_t stream) {
+cudaError_t launch_la_tc(const LaCore& p, bool split, bool must, int forced, cudaStream_t stream) {
     CUtensorMap ma, mb, mc, mo;
     const int64_t tokens = la_tokens(p);
     if (!tile_map(&ma, p.a, tokens, p.heads_a, p.d_b, kC) ||
@@ -1048,14 +1331,57 @@ cudaError_t launch_la_tc(const LaCore& p, cudaStream_t stream) {
         !tile_map(&mc, p.c, tokens, p.heads_c, p.d_c, kC) ||
         !tile_map(&mo, p.out, tokens, p.heads, p.d_c, 32, p.out_f32 != 0))
         return cudaErrorInvalidValue;
-    auto* kernel = p.reverse ? la_tc<true> : la_tc<false>;
-    const cudaError_t e = cudaFuncSetAttribute(
-        kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmemBytes));
-    if (e != cudaSuccess) return e;
-    const int64_t items = static_cast<int64_t>(p.n_seqs) * p.heads;
-    const int grid = static_cast<int>(std::min<int64_t>(items, sm_count()));
-    kernel<<<grid, kThreads, kSmemBytes, stream>>>(p, ma, mb, mc, mo, static_cast<int>(items));
-    return cudaGetLastError();
+    auto* full = p.reverse ? la_tc<true, false> : la_tc<false, false>;
+    auto* states = p.reverse ? la_tc<true, true> : la_tc<false, true>;
+    cudaError_t e;
+    for (auto* k : {full, states})
+        if ((e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                      static_cast<int>(kSmemBytes))) != cudaSuccess)
+            return e;
+    // What splitting could bring: no sequence is longer than `longest` chunks, and the
+    // work fills every SM for `each` chunks or fewer.
+    const int sms = sm_count();
+    const int64_t longest = ((p.cu_seqlens ? tokens : p.seq_len) + kC - 1) / kC;
+    const int64_t most = p.cu_seqlens ? tokens / kC + p.n_seqs : longest * p.n_seqs;
+    const double each = static_cast<double>(most) * p.heads / sms;
+    const int l_min = forced > 0 ? forced : std::max(2, static_cast<int>(each / 4));
+    split = split && (must || longest > 2 * l_min + 2) && longest > l_min;
+    const int64_t jobs = static_cast<int64_t>(p.n_seqs) * p.heads;
+    if (!split && jobs <= sms) {  // one job a CTA
+        full<<<static_cast<int>(jobs), kThreads, kSmemBytes, stream>>>(p, ma, mb, mc, mo, nullptr,
+                                                                       nullptr, nullptr);
+        return cudaGetLastError();
+    }
+    const size_t size = sizeof(float) * p.heads * p.d_b * p.d_c;
+    // A split sequence of c > L chunks has ceil(c / L) < 2 c / L segments.
+    const int64_t cap = split ? std::min<int64_t>(2 * most / l_min + 2, kStateBudget / size) : 0;
+    auto up = [](size_t x) { return (x + 255) & ~static_cast<size_t>(255); };
+    const size_t o_main = up(sizeof(Plan)), o_states = o_main + up(sizeof(Entry) * (p.n_seqs + cap)),
+                 o_splits = o_states + up(sizeof(Entry) * cap),
+                 o_base = o_splits + up(sizeof(Split) * (cap / 2 + 1)),
+                 o_slots = o_base + up(sizeof(int32_t) * p.n_seqs), bytes = o_slots + cap * size;
+    cudaMemPool_t pool;
+    if ((e = library_pool(&pool, true)) != cudaSuccess) return e;
+    void* mem = nullptr;
+    if ((e = cudaMallocFromPoolAsync(&mem, bytes, pool, stream)) != cudaSuccess) return e;
+    uint8_t* at = static_cast<uint8_t*>(mem);
+    Plan* plan = reinterpret_cast<Plan*>(at);
+    Entry* main_list = reinterpret_cast<Entry*>(at + o_main);
+    Entry* state_list = reinterpret_cast<Entry*>(at + o_states);
+    Split* splits = reinterpret_cast<Split*>(at + o_splits);
+    float* slots = reinterpret_cast<float*>(at + o_slots);
+    la_plan<<<1, kPlanThreads, 0, stream>>>(p, plan, main_list, state_list, splits,
+                                            reinterpret_cast<int32_t*>(at + o_base), sms, l_min,
+                                            static_cast<int>(cap), forced, must);
+    if (split) {
+        states<<<sms, kThreads, kSmemBytes, stream>>>(p, ma, mb, mc, mo, &plan->states, state_list,
+                                                      slots);
+        la_scan<<<4 * sms, 256, 0, stream>>>(p, plan, splits, slots);
+    }
+    full<<<sms, kThreads, kSmemBytes, stream>>>(p, ma, mb, mc, mo, &plan->main, main_list, slots);
+    e = cudaGetLastError();
+    const cudaError_t f = cudaFreeAsync(mem, stream);
+    return e != cudaSuccess ? e : f;
 }
 
 cudaError_t take_la_error(int* flag) {

@@ -450,3 +450,44 @@ def test_the_layer_together():
     for got, ref in zip((out, dq, dk, dv, dqw, dkw), (want, *grads)):
         ref = ref.detach()
         assert float((got.double() - ref).norm() / ref.norm()) < 1.4e-3
+
+
+@pytest.mark.parametrize("split", [0, 1, 2, 5])
+@pytest.mark.parametrize("state", [True, False])
+@pytest.mark.parametrize("shape", [(128, 128), (40, 72)])
+def test_segments(shape, state, split):
+    """Long sequences in segments: the states before them from a first pass and a
+    scan, forward and backward in time; the last segment short, one position,
+    or whole."""
+    x = make([700, 5, 0, 1281, 1, 640, 129], 2, 2, *shape, torch.bfloat16, seed=split, state=state,
+             g=[-0.003, -0.6])
+    check_forward(x, "tensor_split", split=split)
+    check_backward(x, "tensor_split", split=split)
+
+
+@pytest.mark.parametrize("algo", ["auto", "tensor", "cuda_core", "tensor_split"])
+def test_kernel_families_agree_with_the_definition(algo):
+    x = make([300, 0, 513, 64], 2, 4, 128, 128, torch.bfloat16, seed=14)
+    check_forward(x, algo)
+    check_backward(x, algo)
+    y = make([2049], 2, 2, 64, 64, torch.bfloat16, seed=15, packed=False)
+    check_forward(y, algo)
+    check_backward(y, algo)
+
+
+@pytest.mark.parametrize("algo", ["tensor", "tensor_split"])
+@pytest.mark.parametrize("shape,dtype", [((128, 128), torch.float32), ((128, 128), torch.float16),
+                                         ((136, 128), torch.bfloat16), ((60, 64), torch.bfloat16)])
+def test_tensor_families_refuse_what_they_do_not_take(shape, dtype, algo):
+    x = make([64], 1, 1, *shape, dtype)
+    with pytest.raises(_lib.GdrError) as e:
+        LinearAttention(algo=algo).chunked(x["q"], x["k"], x["v"], x["g"], cu_seqlens=x["cu"])
+    assert e.value.status == _lib.GDR_ERR_UNSUPPORTED
+
+
+def test_many_sequences_on_few_heads():
+    """More jobs than SMs, handed out from the list: every length from 0 to 399."""
+    lens = list(range(400))
+    x = make(lens, 1, 2, 128, 128, torch.bfloat16, seed=16)
+    check_forward(x)
+    check_backward(x)
