@@ -108,6 +108,10 @@ cudaError_t run_core(const gdr_la_params& a, const LaCore& p, bool chunked, cuda
     if (tc && a.algo != GDR_ALGO_CUDA_CORE)
         return launch_la_tc(p, a.algo != GDR_ALGO_TENSOR, a.algo == GDR_ALGO_TENSOR_SPLIT,
                             a.split_chunks, s);
+    // Short sequences step as fast as a chunk does; the others go in chunks.
+    const int64_t tokens = la_tokens(p);
+    if (la_mma_supports(p) && tokens > 4 * static_cast<int64_t>(p.n_seqs))
+        return launch_la_mma(p, s);
     return launch_la_recurrent(p, s);
 }
 

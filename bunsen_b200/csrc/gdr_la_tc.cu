@@ -50,11 +50,10 @@
 #include <cmath>
 
 #include "gdr_la.cuh"
+#include "gdr_la_plan.cuh"
 #include "gdr_sm100.cuh"
 
 namespace gdr {
-
-cudaError_t library_pool(cudaMemPool_t* pool, bool create);
 
 // Device-side failures since the last gdr_device_error: bit 0, a bounded wait
 // ran out.
@@ -64,7 +63,7 @@ namespace {
 
 using namespace sm100;
 
-constexpr int kC = 128, kD = 128;
+constexpr int kC = kLaChunk, kD = 128;
 constexpr int kThreads = 896;
 constexpr uint32_t kTile = 32768;         // 128 positions x 128 bf16, two 64-wide halves
 constexpr uint32_t kHalf = kTile / 2;
@@ -72,11 +71,10 @@ constexpr uint32_t kStage = 3 * kTile;    // a, b, c
 constexpr uint32_t kOffSb = 2 * kStage, kOffMisc = kOffSb + kTile;
 constexpr uint32_t kSmemBytes = kOffMisc + 512;
 constexpr uint32_t kColU = 0, kColP = 128, kColO = 256, kColW = 384, kColWBuf = 48;
-constexpr int64_t kStateBudget = int64_t{2} << 30;  // scratch states of a split call, bytes
 constexpr int kWaitRounds = 1 << 24;  // of two tries: seconds
 
 // What a CTA works on next: the positions [start, start + len) of a sequence with
-// head h, from state `in` to state `out` (see state_at); len < 0: nothing more.
+// head h, from state `in` to state `out` (see la_state); len < 0: nothing more.
 struct Job {
     int start, len, h, in, out;
 };
@@ -340,53 +338,8 @@ __device__ __forceinline__ uint32_t pack_bf16(uint64_t p) {
 }
 __device__ __forceinline__ uint64_t widen(uint32_t p) { return pair(low_f32(p), high_f32(p)); }
 
-// w^n for 0 <= n <= 128, 1 for n = 0 (minus infinity included): the exponent's
-// rounding error goes in as a factor, e^(p + d) = e^p (1 + d).
-__device__ __forceinline__ float power(float g, int n) {
-    if (n <= 0) return 1.f;
-    const float p = g * n;
-    if (p < -104.f) return 0.f;  // below the smallest f32
-    const float e = expf(p);
-    return fmaf(e, fmaf(g, static_cast<float>(n), -p), e);
-}
-
-// w^n in two parts, hi + lo.
-__device__ __forceinline__ float2 power2(float g, int n) {
-    const double f = exp(static_cast<double>(g) * n);
-    const float hi = static_cast<float>(f);
-    return make_float2(hi, static_cast<float>(f - hi));
-}
-
 // Heads whose decay's powers to w^-128 are far from overflow (e^51).
 __device__ __forceinline__ bool is_gentle(float g) { return g >= -0.4f && g <= 0.4f; }
-
-// A list of work in device memory, made by la_plan: entries of positions and states,
-// each for every head, the longest first. null: one job a CTA, its sequence and
-// head by its index.
-struct Work {
-    int32_t count;    // entries
-    int32_t next;     // the next job not handed out (entry x heads + head)
-};
-struct Entry {
-    int32_t start, len, in, out;
-};
-
-// States by index: the call's own of sequence x >= 0, none (-1: zeros, or not
-// wanted), or segment -2 - x's in the scratch. Null, or row `r` columns `c` apart.
-struct StateAt {
-    const float* ptr;
-    int64_t row, col;
-};
-__device__ __forceinline__ StateAt state_at(const LaCore& p, int x, int h, const float* own,
-                                            const float* scratch) {
-    const int64_t size = static_cast<int64_t>(p.d_b) * p.d_c;
-    const float* base = x >= 0 ? own : x == -1 ? nullptr : scratch;
-    const bool turned = x >= 0 && p.state_t;
-    return {base != nullptr
-                ? base + (static_cast<int64_t>(x >= 0 ? x : -2 - x) * p.heads + h) * size
-                : nullptr,
-            turned ? 1 : p.d_c, turned ? p.d_b : 1};
-}
 
 // Chunk c of an item, in the order they run: its length, and its first row.
 template <bool kRev>
@@ -406,7 +359,7 @@ template <bool kRev, bool kStateOnly>
 __global__ void __launch_bounds__(kThreads, 1)
 la_tc(const LaCore p, const __grid_constant__ CUtensorMap ma,
       const __grid_constant__ CUtensorMap mb, const __grid_constant__ CUtensorMap mc,
-      const __grid_constant__ CUtensorMap mo, Work* work, const Entry* entries, float* scratch) {
+      const __grid_constant__ CUtensorMap mo, LaWork* work, const LaEntry* entries, float* scratch) {
     extern __shared__ __align__(1024) uint8_t sm[];  // (checked below: swizzled tiles need it)
     Bars& B = *reinterpret_cast<Bars*>(sm + kOffMisc);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -480,7 +433,7 @@ la_tc(const LaCore p, const __grid_constant__ CUtensorMap ma,
                     const int e = id / heads;
                     it.h = id - e * heads;
                     if (work != nullptr) {
-                        const Entry x = entries[e];
+                        const LaEntry x = entries[e];
                         it.start = x.start, it.len = x.len, it.in = x.in, it.out = x.out;
                     } else {
                         int64_t start, end;
@@ -712,12 +665,12 @@ la_tc(const LaCore p, const __grid_constant__ CUtensorMap ma,
             const Job it = take(k % kJobs);
             if (it.len < 0) break;
             const int nch = (it.len + kC - 1) / kC;
-            const float g = p.log_decay[it.h], w = power(g, 1);
+            const float g = p.log_decay[it.h], w = la_power(g, 1);
             const bool gentle = is_gentle(g);
             const uint64_t step = pair(w * w, w * w);
-            const float w16 = power(g, 16);
+            const float w16 = la_power(g, 16);
             // Steep, the diagonal block's second half.
-            const float steep = p.sigma * p.tau * power(g, kRev ? max(16 - lane, 0)
+            const float steep = p.sigma * p.tau * la_power(g, kRev ? max(16 - lane, 0)
                                                                 : max(lane - 15, 0));
             float ahead = 0.f, fb[2];  // O's row factor; the blocks' first column factors
             int known = 0;             // the chunk length they are for
@@ -726,17 +679,17 @@ la_tc(const LaCore p, const __grid_constant__ CUtensorMap ma,
                 const uint32_t st = n & 1, ph = n & 1, ph2 = (n >> 1) & 1;
                 const int len = chunk_len<kRev>(it, nch, c);
                 if (len != known) {
-                    ahead = p.tau * power(g, kRev ? max(len - 1 - i, 0) : i + 1);
+                    ahead = p.tau * la_power(g, kRev ? max(len - 1 - i, 0) : i + 1);
                     // Steep, off the diagonal block: w^{i-j} splits in two
                     // exponents that are not negative, rows' and columns'.
-                    const float edge = p.sigma * p.tau * power(g, kRev ? 32 - lane : lane + 1);
+                    const float edge = p.sigma * p.tau * la_power(g, kRev ? 32 - lane : lane + 1);
 #pragma unroll
                     for (int x = 0; x < 2; ++x) {
                         const int cb = 2 * half + x;
                         const int e = kRev ? len - 1 - 32 * cb : 32 * cb + 32;
                         const int apart = kRev ? cb - quarter : quarter - cb;
                         fb[x] = (gentle ? p.sigma : edge) *
-                                power(gentle && e >= 0 ? -g : g,
+                                la_power(gentle && e >= 0 ? -g : g,
                                       gentle ? abs(e) : 32 * (apart - 1));
                     }
                     known = len;
@@ -871,7 +824,7 @@ la_tc(const LaCore p, const __grid_constant__ CUtensorMap ma,
             const float g = p.log_decay[it.h];
             const bool mine = col < p.d_c;
             {
-                const StateAt in = state_at(p, it.in, it.h, p.state_in, scratch);
+                const LaState in = la_state(p, it.in, it.h, p.state_in, scratch);
                 if (in.ptr != nullptr && mine) {
                     const float* src = in.ptr + col * in.col + b0 * in.row;
 #pragma unroll
@@ -901,7 +854,7 @@ la_tc(const LaCore p, const __grid_constant__ CUtensorMap ma,
                 }
                 const int len = chunk_len<kRev>(it, nch, c);
                 if (len != known) {
-                    const float2 f = power2(g, len);
+                    const float2 f = la_power2(g, len);
                     hi2 = pair(f.x, f.x);
                     lo2 = pair(f.y, f.y);
                     known = len;
@@ -922,7 +875,7 @@ la_tc(const LaCore p, const __grid_constant__ CUtensorMap ma,
                         s[8 * blk + j] = fma2(s[8 * blk + j], hi2, fma2(s[8 * blk + j], lo2, u[j]));
                 }
             }
-            const StateAt out = state_at(p, it.out, it.h, p.state_out, scratch);
+            const LaState out = la_state(p, it.out, it.h, p.state_out, scratch);
             if (ok && out.ptr != nullptr && mine) {
                 float* dst = const_cast<float*>(out.ptr) + col * out.col + b0 * out.row;
 #pragma unroll
@@ -957,7 +910,7 @@ la_tc(const LaCore p, const __grid_constant__ CUtensorMap ma,
             // Of position j = 32 q + jj, jj = 8 k + 2 (t % 4) + e, in a whole chunk:
             // w^(127 - j) = w^(96 - 32 q) w^(31 - jj), backward w^(32 q) w^(jj + 1).
             const int j0 = 2 * (lane & 3);
-            const float mine = power(g, lane);  // w^lane, for the other lanes
+            const float mine = la_power(g, lane);  // w^lane, for the other lanes
             auto small = [&](int n) { return __shfl_sync(0xffffffffu, mine, n & 31); };
             uint64_t wt[4];
 #pragma unroll
@@ -966,7 +919,7 @@ la_tc(const LaCore p, const __grid_constant__ CUtensorMap ma,
                 wt[k] = kRev ? pair(small(j) * small(1), small(j + 1) * small(1))
                              : pair(small(31 - j), small(30 - j));
             }
-            const float w32 = power(g, 32), w64 = power(g, 64), w96 = power(g, 96);
+            const float w32 = la_power(g, 32), w64 = la_power(g, 64), w96 = la_power(g, 96);
 #pragma unroll 1
             for (int c = 0; c < nch; ++c, ++n) {
                 const int st = n & 1;
@@ -1066,211 +1019,6 @@ la_tc(const LaCore p, const __grid_constant__ CUtensorMap ma,
     if (warp == 26) tmem_dealloc(B.tmem, 512);
 }
 
-// ---- sequences in segments ------------------------------------------------------
-// A state passes through positions as S -> w^n S + B, B what they reach from zero.
-// So a long sequence, which one CTA would walk alone, goes in segments of L chunks:
-// one pass finds the B of every segment but the last (in the order of time), a
-// scan the states before the segments, and the main pass runs all segments at once.
-// The first pass reads b and c again: it is worth it where the longest
-// sequences would bound the call. la_plan decides from the lengths, which only
-// the device has.
-struct Split {
-    int32_t base, parts, seq, unused;  // segment r's state: slot base + r, r >= 1
-};
-struct Plan {
-    Work main, states;
-    int32_t splits, seg_tokens;
-    int32_t pad[2];
-};
-
-constexpr int kPlanThreads = 1024, kBuckets = 1024;
-// Costs in chunks of the main pass (3.8 us a chunk at one CTA an SM): a chunk of the
-// first pass, and what two more passes and a scan cost at all.
-constexpr float kStateCost = 0.55f, kSplitCost = 3.f, kLinkCost = 0.05f;
-
-// The block's sum (op 0) or maximum (op 1) of x.
-__device__ int block_reduce(int x, bool maximum, int* ws) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    for (int o = 16; o > 0; o >>= 1) {
-        const int y = __shfl_xor_sync(0xffffffffu, x, o);
-        x = maximum ? max(x, y) : x + y;
-    }
-    __syncthreads();
-    if (lane == 0) ws[warp] = x;
-    __syncthreads();
-    x = ws[lane];
-    for (int o = 16; o > 0; o >>= 1) {
-        const int y = __shfl_xor_sync(0xffffffffu, x, o);
-        x = maximum ? max(x, y) : x + y;
-    }
-    return x;
-}
-
-// The work lists: every sequence, or its segments, the longest first (by buckets of
-// chunk counts), and the first pass's segments. seg_cap: state slots; 0: no
-// splitting. forced: a given segment length.
-__global__ void __launch_bounds__(kPlanThreads)
-la_plan(const LaCore p, Plan* plan, Entry* main, Entry* states, Split* splits, int32_t* base,
-        int grid, int l_min, int seg_cap, int forced, bool must) {
-    __shared__ int ws[32], hist[kBuckets], slots, n_splits, n_states;
-    __shared__ float cost[32];
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    auto chunks = [&](int s, int64_t& start, int64_t& len) {
-        int64_t end;
-        la_span(p, s, start, end);
-        len = end - start;
-        return static_cast<int>((len + kC - 1) / kC);
-    };
-    int64_t start, len;
-    int sum = 0, most = 0;
-    for (int s = tid; s < p.n_seqs; s += kPlanThreads) {
-        const int c = chunks(s, start, len);
-        sum += c;
-        most = max(most, c);
-    }
-    sum = block_reduce(sum, false, ws);
-    most = block_reduce(most, true, ws);
-    // Candidate lengths from l_min to the longest sequence, one a warp.
-    const float each = static_cast<float>(p.heads) / grid;
-    auto candidate = [&](int i) {
-        return forced > 0 ? forced
-                          : max(l_min, static_cast<int>(l_min * powf(fmaxf(1.f, static_cast<float>(most) / l_min),
-                                                                     i / 31.f)));
-    };
-    {
-        const int L = candidate(warp);
-        int again = 0, parts_most = 0, segs = 0;
-        for (int s = lane; s < p.n_seqs; s += 32) {
-            const int c = chunks(s, start, len);
-            if (c > L) {
-                const int parts = (c + L - 1) / L;
-                again += (parts - 1) * L;
-                segs += parts;
-                parts_most = max(parts_most, parts);
-            }
-        }
-        for (int o = 16; o > 0; o >>= 1) {
-            again += __shfl_xor_sync(0xffffffffu, again, o);
-            segs += __shfl_xor_sync(0xffffffffu, segs, o);
-            parts_most = max(parts_most, __shfl_xor_sync(0xffffffffu, parts_most, o));
-        }
-        const float longest = static_cast<float>(min(L, most));
-        float t = fmaxf(longest, sum * each * 1.03f + 1.f);
-        if (again > 0)
-            t += kStateCost * fmaxf(longest, again * each * 1.03f + 1.f) + kSplitCost +
-                 kLinkCost * parts_most;
-        if (segs > seg_cap) t = INFINITY;
-        if (lane == 0) cost[warp] = t;
-    }
-    __syncthreads();
-    int L = most > 0 ? most : 1;  // not split
-    if (seg_cap > 0) {
-        float best = must || forced > 0 ? INFINITY
-                                        : 0.97f * fmaxf(static_cast<float>(most), sum * each * 1.03f + 1.f);
-        for (int i = 0; i < 32; ++i)
-            if (cost[i] < best) {
-                best = cost[i];
-                L = candidate(i);
-            }
-    }
-    const int shift = max(0, 32 - __clz(min(L, most)) - 10);  // bucket: chunks >> shift
-    for (int i = tid; i < kBuckets; i += kPlanThreads) hist[i] = 0;
-    if (tid == 0) slots = n_splits = n_states = 0;
-    __syncthreads();
-    auto bucket = [&](int c) { return kBuckets - 1 - (c >> shift); };  // longest first
-    for (int s = tid; s < p.n_seqs; s += kPlanThreads) {
-        const int c = chunks(s, start, len);
-        int parts = c > L ? (c + L - 1) / L : 1, at = 0;
-        if (parts > 1) at = atomicAdd(&slots, parts);
-        base[s] = at;
-        if (parts > 1) {
-            atomicAdd(&hist[bucket(L)], parts - 1);
-            atomicAdd(&hist[bucket(c - (parts - 1) * L)], 1);
-        } else {
-            atomicAdd(&hist[bucket(c)], 1);
-        }
-    }
-    __syncthreads();
-    // Exclusive scan of the buckets (as many as threads).
-    int x = hist[tid];
-    const int mine = x;
-    for (int o = 1; o < 32; o <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, x, o);
-        if (lane >= o) x += y;
-    }
-    __syncthreads();
-    if (lane == 31) ws[warp] = x;
-    __syncthreads();
-    int before = 0;
-    for (int i = 0; i < warp; ++i) before += ws[i];
-    __syncthreads();
-    hist[tid] = before + x - mine;
-    __syncthreads();
-    for (int s = tid; s < p.n_seqs; s += kPlanThreads) {
-        const int c = chunks(s, start, len);
-        const int parts = c > L ? (c + L - 1) / L : 1;
-        if (parts == 1) {
-            main[atomicAdd(&hist[bucket(c)], 1)] = {static_cast<int32_t>(start),
-                                                    static_cast<int32_t>(len), s, s};
-            continue;
-        }
-        splits[atomicAdd(&n_splits, 1)] = {base[s], parts, s, 0};
-        for (int r = 0; r < parts; ++r) {  // in the order of time
-            const int part = p.reverse ? parts - 1 - r : r;
-            const int from = part * L, n = min(L, c - from);
-            const int32_t t0 = static_cast<int32_t>(start) + from * kC;
-            const int32_t tokens = min(n * kC, static_cast<int32_t>(len) - from * kC);
-            main[atomicAdd(&hist[bucket(n)], 1)] = {t0, tokens, r == 0 ? s : -2 - (base[s] + r),
-                                                    r == parts - 1 ? s : -1};
-            if (r < parts - 1)
-                states[atomicAdd(&n_states, 1)] = {t0, tokens, -1, -2 - (base[s] + r + 1)};
-        }
-    }
-    __syncthreads();
-    if (tid == 0) {
-        plan->main = {p.n_seqs + slots - n_splits, grid};
-        plan->states = {n_states, grid};
-        plan->splits = n_splits;
-        plan->seg_tokens = L * kC;
-    }
-}
-
-// S_{r+1} = w^(tokens of r) S_r + B_r, in place: slot base + r + 1 holds B_r. Four
-// elements a thread, every link's load issued ahead of the products.
-__global__ void __launch_bounds__(256)
-la_scan(const LaCore p, const Plan* plan, const Split* splits, float* scratch) {
-    const int size = p.d_b * p.d_c, tiles = (size + 1023) / 1024;
-    const int64_t jobs = static_cast<int64_t>(plan->splits) * p.heads * tiles;
-    for (int64_t job = blockIdx.x; job < jobs; job += gridDim.x) {
-        const int tile = static_cast<int>(job % tiles);
-        const int h = static_cast<int>(job / tiles % p.heads);
-        const Split sp = splits[job / tiles / p.heads];
-        const int e = tile * 1024 + 4 * threadIdx.x;
-        if (e >= size) continue;
-        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-        const StateAt in = state_at(p, sp.seq, h, p.state_in, scratch);
-        if (in.ptr != nullptr) {
-            const float* src = in.ptr + (e / p.d_c) * in.row + (e % p.d_c) * in.col;
-            x = make_float4(src[0], src[in.col], src[2 * in.col], src[3 * in.col]);
-        }
-        int64_t start, end;
-        la_span(p, sp.seq, start, end);
-        const float g = p.log_decay[h];
-        const int last = static_cast<int>(end - start) - (sp.parts - 1) * plan->seg_tokens;
-        const float w = power(g, plan->seg_tokens);
-        float* slot = scratch + (static_cast<int64_t>(sp.base + 1) * p.heads + h) * size + e;
-        const int64_t step = static_cast<int64_t>(p.heads) * size;
-#pragma unroll 4
-        for (int r = 0; r < sp.parts - 1; ++r, slot += step) {
-            const float f = p.reverse && r == 0 ? power(g, last) : w;
-            const float4 b = *reinterpret_cast<const float4*>(slot);
-            x = make_float4(fmaf(f, x.x, b.x), fmaf(f, x.y, b.y), fmaf(f, x.z, b.z),
-                            fmaf(f, x.w, b.w));
-            *reinterpret_cast<float4*>(slot) = x;
-        }
-    }
-}
-
 PFN_cuTensorMapEncodeTiled_v12000 encoder() {
     static PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
         void* ptr = nullptr;
@@ -1305,13 +1053,6 @@ bool tile_map(CUtensorMap* map, const void* base, int64_t tokens, int heads, int
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-int sm_count() {
-    int dev = 0, n = 0;
-    cudaGetDevice(&dev);
-    cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
-    return n > 0 ? n : 148;
-}
-
 }  // namespace
 
 bool la_tc_supports(const LaCore& p) {
@@ -1338,49 +1079,23 @@ cudaError_t launch_la_tc(const LaCore& p, bool split, bool must, int forced, cud
         if ((e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                       static_cast<int>(kSmemBytes))) != cudaSuccess)
             return e;
-    // What splitting could bring: no sequence is longer than `longest` chunks, and the
-    // work fills every SM for `each` chunks or fewer.
-    const int sms = sm_count();
-    const int64_t longest = ((p.cu_seqlens ? tokens : p.seq_len) + kC - 1) / kC;
-    const int64_t most = p.cu_seqlens ? tokens / kC + p.n_seqs : longest * p.n_seqs;
-    const double each = static_cast<double>(most) * p.heads / sms;
-    const int l_min = forced > 0 ? forced : std::max(2, static_cast<int>(each / 4));
-    split = split && (must || longest > 2 * l_min + 2) && longest > l_min;
+    // A chunk takes 3.8 us at one CTA an SM; the states' pass 0.85 of that (it waits for
+    // the same operand), and its launches and the scan some 6 chunks.
+    const int sms = la_sm_count();
+    LaLists lists;
+    e = la_prepare(p, sms, 1, {split, must, forced, 0.85f, 6.f}, lists, stream);
+    if (e != cudaSuccess) return e;
+    if (lists.split) {
+        states<<<sms, kThreads, kSmemBytes, stream>>>(p, ma, mb, mc, mo, &lists.plan->states,
+                                                      lists.states, lists.slots);
+        la_scan_states(p, lists, stream);
+    }
     const int64_t jobs = static_cast<int64_t>(p.n_seqs) * p.heads;
-    if (!split && jobs <= sms) {  // one job a CTA
-        full<<<static_cast<int>(jobs), kThreads, kSmemBytes, stream>>>(p, ma, mb, mc, mo, nullptr,
-                                                                       nullptr, nullptr);
-        return cudaGetLastError();
-    }
-    const size_t size = sizeof(float) * p.heads * p.d_b * p.d_c;
-    // A split sequence of c > L chunks has ceil(c / L) < 2 c / L segments.
-    const int64_t cap = split ? std::min<int64_t>(2 * most / l_min + 2, kStateBudget / size) : 0;
-    auto up = [](size_t x) { return (x + 255) & ~static_cast<size_t>(255); };
-    const size_t o_main = up(sizeof(Plan)), o_states = o_main + up(sizeof(Entry) * (p.n_seqs + cap)),
-                 o_splits = o_states + up(sizeof(Entry) * cap),
-                 o_base = o_splits + up(sizeof(Split) * (cap / 2 + 1)),
-                 o_slots = o_base + up(sizeof(int32_t) * p.n_seqs), bytes = o_slots + cap * size;
-    cudaMemPool_t pool;
-    if ((e = library_pool(&pool, true)) != cudaSuccess) return e;
-    void* mem = nullptr;
-    if ((e = cudaMallocFromPoolAsync(&mem, bytes, pool, stream)) != cudaSuccess) return e;
-    uint8_t* at = static_cast<uint8_t*>(mem);
-    Plan* plan = reinterpret_cast<Plan*>(at);
-    Entry* main_list = reinterpret_cast<Entry*>(at + o_main);
-    Entry* state_list = reinterpret_cast<Entry*>(at + o_states);
-    Split* splits = reinterpret_cast<Split*>(at + o_splits);
-    float* slots = reinterpret_cast<float*>(at + o_slots);
-    la_plan<<<1, kPlanThreads, 0, stream>>>(p, plan, main_list, state_list, splits,
-                                            reinterpret_cast<int32_t*>(at + o_base), sms, l_min,
-                                            static_cast<int>(cap), forced, must);
-    if (split) {
-        states<<<sms, kThreads, kSmemBytes, stream>>>(p, ma, mb, mc, mo, &plan->states, state_list,
-                                                      slots);
-        la_scan<<<4 * sms, 256, 0, stream>>>(p, plan, splits, slots);
-    }
-    full<<<sms, kThreads, kSmemBytes, stream>>>(p, ma, mb, mc, mo, &plan->main, main_list, slots);
+    full<<<lists.plan != nullptr ? sms : static_cast<int>(jobs), kThreads, kSmemBytes, stream>>>(
+        p, ma, mb, mc, mo, lists.plan != nullptr ? &lists.plan->main : nullptr, lists.main,
+        lists.slots);
     e = cudaGetLastError();
-    const cudaError_t f = cudaFreeAsync(mem, stream);
+    const cudaError_t f = la_release(lists, stream);
     return e != cudaSuccess ? e : f;
 }
 
