@@ -240,8 +240,9 @@ gdr_status make_rope(const gdr_qk_norm_rope_params* params, const void* q, const
         return GDR_ERR_INVALID;
     if (!(a.eps >= 0.0) || !std::isfinite(a.eps)) return GDR_ERR_INVALID;
     if (a.head_dim > gdr::norm_rope_max_d()) return GDR_ERR_UNSUPPORTED;
-    if (a.tokens * (static_cast<int64_t>(a.heads_q) + a.heads_k) >= (int64_t{1} << 33))
-        return GDR_ERR_UNSUPPORTED;  // grid limit
+    if (a.tokens >= (int64_t{1} << 31) ||
+        a.tokens * (static_cast<int64_t>(a.heads_q) + a.heads_k) >= (int64_t{1} << 31))
+        return GDR_ERR_UNSUPPORTED;  // rows are counted in 32 bits
     if (a.tokens > 0 && !(q && k && positions && cos && sin && q_out && k_out))
         return GDR_ERR_INVALID;
     p.tokens = a.tokens;

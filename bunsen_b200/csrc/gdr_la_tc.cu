@@ -49,6 +49,7 @@
 #include <algorithm>
 #include <cmath>
 
+#include "gdr_f32x2.cuh"
 #include "gdr_la.cuh"
 #include "gdr_la_plan.cuh"
 #include "gdr_sm100.cuh"
@@ -312,25 +313,6 @@ __device__ __forceinline__ void take_registers() {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegs));
 }
 
-// Pairs of f32 in one 64-bit register: one instruction for two products or sums.
-__device__ __forceinline__ uint64_t pair(float x, float y) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
-    return r;
-}
-__device__ __forceinline__ void unpair(uint64_t p, float& x, float& y) {
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(p));
-}
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-    uint64_t r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
 __device__ __forceinline__ uint32_t pack_bf16(uint64_t p) {
     float x, y;
     unpair(p, x, y);

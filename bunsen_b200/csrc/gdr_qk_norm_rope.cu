@@ -10,18 +10,21 @@
 // Every sum and product is f32; the one rounding is the output's own.
 //
 // Bound by HBM: one read and one write of q and k (for the gradient two reads
-// and one write). The vector kernels give a lane 8 consecutive features (one
-// 16-byte access for 16-bit types), 8, 16 or 32 lanes to a row, so a warp
-// covers one to four rows per instruction, the row's sums by shuffles inside
-// its lanes, a rotation partner by one shuffle (or in the lane itself when
-// interleaved). A warp takes kRows rows of one token per lane group, all loads
-// issued before any is used; the token's angles are read once for them. Other
-// shapes (odd widths, unaligned rows) take one warp per row, scalar accesses.
+// and one write). The vector kernels give a lane 8 features, both of every pair it
+// rotates among them (two runs of four: 8-byte accesses for 16-bit types), 8,
+// 16 or 32 lanes to a row, so a warp covers one to four rows per instruction,
+// the row's sums by shuffles inside its lanes; products by f32 pairs. (With 8
+// consecutive features a lane, partners by shuffle and single products it was
+// bound by instructions: 150 us for 32768 x 32 heads of 128 against TIMEUS.) A warp takes kRows rows of one token per lane group, the next rows'
+// loads issued before these are computed; the token's angles are read once for
+// them. Other shapes (odd widths, unaligned rows) take one warp per row, scalar
+// accesses.
 //
 // The weights' gradient is summed without atomics, so equal calls give equal
 // bits: a fixed grid, each lane's sums over its rows in registers, each
 // block's in shared memory in warp order, then one kernel over the blocks.
 #include "gdr_common.cuh"
+#include "gdr_f32x2.cuh"
 #include "gdr_qk_norm_rope.cuh"
 
 namespace gdr {
@@ -34,53 +37,64 @@ namespace {
 
 constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr int kMaxD = 256;
+constexpr int kWaves = 4;  // of CTAs of the outputs' kernels
 
-template <typename T>
-__device__ __forceinline__ void load8(const T* src, float (&x)[8]) {
-    if constexpr (sizeof(T) == 4) {
-        const float4 a = reinterpret_cast<const float4*>(src)[0];
-        const float4 b = reinterpret_cast<const float4*>(src)[1];
-        x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-        x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-    } else {
-        const uint4 a = *reinterpret_cast<const uint4*>(src);
-        const T* e = reinterpret_cast<const T*>(&a);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = to_f32(e[i]);
-    }
-}
-
-template <typename T>
-__device__ __forceinline__ void store8(T* dst, const float (&x)[8]) {
-    if constexpr (sizeof(T) == 4) {
-        reinterpret_cast<float4*>(dst)[0] = make_float4(x[0], x[1], x[2], x[3]);
-        reinterpret_cast<float4*>(dst)[1] = make_float4(x[4], x[5], x[6], x[7]);
-    } else {
-        uint4 a;
-        T* e = reinterpret_cast<T*>(&a);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) e[i] = from_f32<T>(x[i]);
-        *reinterpret_cast<uint4*>(dst) = a;
-    }
-}
-
-// A raw row piece as loaded, so that several are in flight before one is used.
+// The 8 features of a lane: two runs of four, at `o0` and `o1`, so that both
+// features of a rotated pair are one lane's: 4 li and rot / 2 + 4 li of the rotated
+// part, 8 li and 8 li + 4 behind it or where pairs are neighbours.
 template <typename T>
 struct Raw {
-    uint4 v[sizeof(T) == 4 ? 2 : 1];
+    uint2 v[sizeof(T) == 4 ? 4 : 2];  // as loaded, so that several rows are in flight
 };
 template <typename T>
-__device__ __forceinline__ Raw<T> load_raw(const T* src) {
+__device__ __forceinline__ Raw<T> load_raw(const T* row, int o0, int o1) {
     Raw<T> r;
-    r.v[0] = reinterpret_cast<const uint4*>(src)[0];
-    if constexpr (sizeof(T) == 4) r.v[1] = reinterpret_cast<const uint4*>(src)[1];
+    if constexpr (sizeof(T) == 4) {
+        const uint4 a = *reinterpret_cast<const uint4*>(row + o0);
+        const uint4 b = *reinterpret_cast<const uint4*>(row + o1);
+        r.v[0] = make_uint2(a.x, a.y), r.v[1] = make_uint2(a.z, a.w);
+        r.v[2] = make_uint2(b.x, b.y), r.v[3] = make_uint2(b.z, b.w);
+    } else {
+        r.v[0] = *reinterpret_cast<const uint2*>(row + o0);
+        r.v[1] = *reinterpret_cast<const uint2*>(row + o1);
+    }
     return r;
 }
+// As pairs of f32.
 template <typename T>
-__device__ __forceinline__ void unpack(const Raw<T>& r, float (&x)[8]) {
+__device__ __forceinline__ void unpack(const Raw<T>& r, uint64_t (&x)[4]) {
     const T* e = reinterpret_cast<const T*>(r.v);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = to_f32(e[i]);
+    for (int i = 0; i < 4; ++i) x[i] = pair(to_f32(e[2 * i]), to_f32(e[2 * i + 1]));
+}
+template <typename T>
+__device__ __forceinline__ void store(T* row, int o0, int o1, const uint64_t (&x)[4]) {
+    Raw<T> r;
+    T* e = reinterpret_cast<T*>(r.v);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        float u, v;
+        unpair(x[i], u, v);
+        e[2 * i] = from_f32<T>(u);
+        e[2 * i + 1] = from_f32<T>(v);
+    }
+    if constexpr (sizeof(T) == 4) {
+        *reinterpret_cast<uint4*>(row + o0) = make_uint4(r.v[0].x, r.v[0].y, r.v[1].x, r.v[1].y);
+        *reinterpret_cast<uint4*>(row + o1) = make_uint4(r.v[2].x, r.v[2].y, r.v[3].x, r.v[3].y);
+    } else {
+        *reinterpret_cast<uint2*>(row + o0) = r.v[0];
+        *reinterpret_cast<uint2*>(row + o1) = r.v[1];
+    }
+}
+__device__ __forceinline__ void load_pairs(const float* row, int o0, int o1, uint64_t (&x)[4]) {
+    const float4 a = *reinterpret_cast<const float4*>(row + o0);
+    const float4 b = *reinterpret_cast<const float4*>(row + o1);
+    x[0] = pair(a.x, a.y), x[1] = pair(a.z, a.w), x[2] = pair(b.x, b.y), x[3] = pair(b.z, b.w);
+}
+__device__ __forceinline__ float sum_pair(uint64_t x) {
+    float u, v;
+    unpair(x, u, v);
+    return u + v;
 }
 
 template <int G>
@@ -90,125 +104,53 @@ __device__ __forceinline__ float group_sum(float x) {
     return x;
 }
 
-// The angles of a lane's 8 features: cos and sin for each, or, interleaved,
-// for its 4 pairs (the other 4 unused). Lanes past the rotated part: none.
+// The angles of a lane's four pairs, as its features' products want them: neighbours
+// (u, v) -> (u, v) (c, c) + (v, u) (-s, s); else pairs of the two runs.
+template <bool kInter>
 struct Angles {
-    float c[8], s[8];
+    uint64_t c[kInter ? 4 : 2], s[kInter ? 4 : 2], n[kInter ? 1 : 2];
 };
-
-__device__ __forceinline__ void load_angles(const NormRope& p, int64_t pos, int e0, Angles& a) {
-    const int half = p.rot / 2;
-    if (e0 >= p.rot) return;
-    if (p.interleaved) {
-        const float4 c = *reinterpret_cast<const float4*>(p.cos + pos * half + e0 / 2);
-        const float4 s = *reinterpret_cast<const float4*>(p.sin + pos * half + e0 / 2);
-        a.c[0] = c.x; a.c[1] = c.y; a.c[2] = c.z; a.c[3] = c.w;
-        a.s[0] = s.x; a.s[1] = s.y; a.s[2] = s.z; a.s[3] = s.w;
+template <bool kInter>
+__device__ __forceinline__ Angles<kInter> angles(const float4& c, const float4& s) {
+    Angles<kInter> a;
+    if constexpr (kInter) {
+        a.c[0] = pair(c.x, c.x), a.c[1] = pair(c.y, c.y), a.c[2] = pair(c.z, c.z), a.c[3] = pair(c.w, c.w);
+        a.s[0] = pair(-s.x, s.x), a.s[1] = pair(-s.y, s.y), a.s[2] = pair(-s.z, s.z), a.s[3] = pair(-s.w, s.w);
     } else {
-        const int i = e0 < half ? e0 : e0 - half;
-        load8(p.cos + pos * half + i, a.c);
-        load8(p.sin + pos * half + i, a.s);
+        a.c[0] = pair(c.x, c.y), a.c[1] = pair(c.z, c.w);
+        a.s[0] = pair(s.x, s.y), a.s[1] = pair(s.z, s.w);
+        a.n[0] = pair(-s.x, -s.y), a.n[1] = pair(-s.z, -s.w);
     }
+    return a;
 }
-
-// Rotates a lane's 8 features in place (sign -1: by the opposite angles).
-// Every lane of the warp calls it: the partner features come by shuffle.
-__device__ __forceinline__ void rotate8(const NormRope& p, int e0, const Angles& a, float sign,
-                                        float (&x)[8]) {
-    if (p.interleaved) {
-        if (e0 < p.rot) {
+template <bool kInter>
+__device__ __forceinline__ void rotate(const Angles<kInter>& a, uint64_t (&x)[4]) {
+    if constexpr (kInter) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float u = x[2 * i], v = x[2 * i + 1], s = sign * a.s[i];
-                x[2 * i] = u * a.c[i] - v * s;
-                x[2 * i + 1] = v * a.c[i] + u * s;
-            }
+        for (int i = 0; i < 4; ++i) {
+            float u, v;
+            unpair(x[i], u, v);
+            x[i] = fma2(x[i], a.c[i], mul2(pair(v, u), a.s[i]));
         }
-        return;
-    }
-    const int half = p.rot / 2, lane = threadIdx.x & 31;
-    const bool low = e0 < half;
-    const int partner = e0 >= p.rot ? lane : low ? lane + half / 8 : lane - half / 8;
-    const float s = low ? -sign : sign;
+    } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const float other = __shfl_sync(0xffffffffu, x[i], partner);
-        if (e0 < p.rot) x[i] = x[i] * a.c[i] + s * other * a.s[i];
+        for (int i = 0; i < 2; ++i) {
+            const uint64_t u = x[i], v = x[2 + i];
+            x[i] = fma2(u, a.c[i], mul2(v, a.n[i]));
+            x[2 + i] = fma2(v, a.c[i], mul2(u, a.s[i]));
+        }
     }
 }
 
-// Which rows a warp's unit of work covers: `per` heads of q, or of k, of one
-// token.
-struct Unit {
-    int64_t token;
-    int head0, heads;  // first head of the unit, heads of the tensor
-    bool is_k;
-};
-__device__ __forceinline__ Unit unit_of(const NormRope& p, int64_t unit, int per) {
-    const int nq = (p.heads_q + per - 1) / per, nk = (p.heads_k + per - 1) / per;
-    Unit u;
-    u.token = unit / (nq + nk);
-    int b = static_cast<int>(unit - u.token * (nq + nk));
-    u.is_k = b >= nq;
-    if (u.is_k) b -= nq;
-    u.head0 = b * per;
-    u.heads = u.is_k ? p.heads_k : p.heads_q;
-    return u;
+__device__ __forceinline__ bool in_tables(const NormRope& p, int pos) {
+    return pos >= 0 && pos < p.table_rows;
 }
-
-__device__ __forceinline__ bool position_of(const NormRope& p, int64_t token, int64_t& pos) {
-    pos = p.positions[token];
-    if (pos >= 0 && pos < p.table_rows) return true;
+__device__ __forceinline__ void report_position() {
     if ((threadIdx.x & 31) == 0) atomicOr(&g_rope_error, 2);
-    return false;
-}
-
-template <typename T, int G, int kRows>
-__global__ void __launch_bounds__(kThreads)
-norm_rope_vec(const NormRope p, int64_t units) {
-    constexpr int kPer = (32 / G) * kRows;
-    const int lane = threadIdx.x & 31, li = lane % G, sub = lane / G, e0 = 8 * li;
-    const int64_t unit = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) >> 5;
-    if (unit >= units) return;
-    const Unit u = unit_of(p, unit, kPer);
-    int64_t pos;
-    if (!position_of(p, u.token, pos)) return;
-    const T* x = static_cast<const T*>(u.is_k ? p.k : p.q) +
-                 u.token * (u.is_k ? p.k_token : p.q_token);
-    const int64_t hstride = u.is_k ? p.k_head : p.q_head;
-    T* y = static_cast<T*>(u.is_k ? p.k_out : p.q_out) + u.token * u.heads * p.d;
-    const float* weight = u.is_k ? p.k_weight : p.q_weight;
-    const bool live = e0 < p.d;
-    Raw<T> raw[kRows];
-#pragma unroll
-    for (int i = 0; i < kRows; ++i) {
-        raw[i] = Raw<T>{};
-        const int h = u.head0 + i * (32 / G) + sub;
-        if (live && h < u.heads) raw[i] = load_raw(x + h * hstride + e0);
-    }
-    Angles a;
-    load_angles(p, pos, e0, a);
-    float wt[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) wt[i] = 1.f;
-    if (weight != nullptr && live) load8(weight + e0, wt);
-#pragma unroll
-    for (int i = 0; i < kRows; ++i) {
-        const int h = u.head0 + i * (32 / G) + sub;
-        float v[8], ss = 0.f;
-        unpack(raw[i], v);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) ss = fmaf(v[j], v[j], ss);
-        const float r = 1.f / sqrtf(group_sum<G>(ss) / p.d + p.eps);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] *= r * wt[j];
-        rotate8(p, e0, a, 1.f, v);
-        if (live && h < u.heads) store8(y + static_cast<int64_t>(h) * p.d + e0, v);
-    }
 }
 
 // The weights' sums of a block into its row of `part` [gridDim.x][2][d]: the
-// warps' sums in warp order (row groups of a warp first).
+// warps' sums in warp order.
 __device__ __forceinline__ void block_weights(const NormRope& p, float (*acc)[kMaxD], float* part) {
     __syncthreads();
     for (int i = threadIdx.x; i < 2 * p.d; i += kThreads) {
@@ -219,82 +161,115 @@ __device__ __forceinline__ void block_weights(const NormRope& p, float (*acc)[kM
     }
 }
 
-template <typename T, int G, int kRows>
-__global__ void __launch_bounds__(kThreads)
-norm_rope_grad_vec(const NormRope p, int64_t units, float* part) {
-    constexpr int kPer = (32 / G) * kRows;
-    __shared__ float acc[2 * kWarps][kMaxD];
+// The outputs, or (kGrad) the gradients. A warp works on q or on k throughout (in
+// proportion to their heads; its weights stay in registers), a unit of kRows x
+// (32 / G) heads of one token at a time, every load before the first use.
+// `q_warps` of all warps work on q. Rows past the last head are the last again,
+// not stored.
+template <typename T, int G, int kRows, bool kInter, bool kGrad>
+__global__ void __launch_bounds__(kThreads, kGrad ? 3 : 4)
+norm_rope_vec(const NormRope p, uint32_t q_warps, float* part) {
+    constexpr int kSub = 32 / G, kPer = kSub * kRows;
+    __shared__ float acc[kGrad ? 2 * kWarps : 1][kMaxD];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int li = lane % G, sub = lane / G, e0 = 8 * li;
-    const bool live = e0 < p.d;
-    float wsum[2][8];
+    const int li = lane % G, sub = lane / G;
+    const bool live = 8 * li < p.d, turned = 8 * li < p.rot;
+    int o0 = 8 * li, o1 = 8 * li + 4;
+    if (turned && !kInter) o0 = 4 * li, o1 = p.rot / 2 + 4 * li;
+    if (!live) o0 = o1 = 0;
+    const uint32_t me = blockIdx.x * kWarps + warp;
+    const bool is_k = me >= q_warps;
+    const int heads = is_k ? p.heads_k : p.heads_q;
+    const uint32_t each = (heads + kPer - 1) / kPer;  // units of a token
+    const uint32_t units = static_cast<uint32_t>(p.tokens) * each;
+    const uint32_t step = is_k ? gridDim.x * kWarps - q_warps : q_warps;
+    const T* x = static_cast<const T*>(is_k ? p.k : p.q);
+    const T* dy = static_cast<const T*>(is_k ? p.dk_out : p.dq_out);
+    T* y = static_cast<T*>(is_k ? p.k_out : p.q_out);
+    const int64_t token_stride = is_k ? p.k_token : p.q_token, head_stride = is_k ? p.k_head : p.q_head;
+    const float* weight = is_k ? p.k_weight : p.q_weight;
+    uint64_t wt[4], wsum[4];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) wsum[0][j] = wsum[1][j] = 0.f;
-    const int64_t step = static_cast<int64_t>(gridDim.x) * kWarps;
-    for (int64_t unit = static_cast<int64_t>(blockIdx.x) * kWarps + warp; unit < units;
-         unit += step) {
-        const Unit u = unit_of(p, unit, kPer);
-        int64_t pos;
-        if (!position_of(p, u.token, pos)) continue;
-        const T* x = static_cast<const T*>(u.is_k ? p.k : p.q) +
-                     u.token * (u.is_k ? p.k_token : p.q_token);
-        const int64_t hstride = u.is_k ? p.k_head : p.q_head;
-        const int64_t row0 = u.token * u.heads;
-        const T* dy = static_cast<const T*>(u.is_k ? p.dk_out : p.dq_out);
-        T* dx = static_cast<T*>(u.is_k ? p.k_out : p.q_out);
-        const float* weight = u.is_k ? p.k_weight : p.q_weight;
-        Raw<T> rx[kRows], rd[kRows];
+    for (int j = 0; j < 4; ++j) wt[j] = pair(1.f, 1.f), wsum[j] = 0;
+    if (weight != nullptr) load_pairs(weight, o0, o1, wt);
+    const float inv_d = 1.f / p.d;
+#pragma unroll 1
+    for (uint32_t u = is_k ? me - q_warps : me; u < units; u += step) {
+        const uint32_t token = u / each;
+        const int head0 = static_cast<int>(u - token * each) * kPer + sub;
+        const T* row = x + token * token_stride;
+        const int64_t flat = static_cast<int64_t>(token) * heads;
+        Raw<T> rx[kRows], rd[kGrad ? kRows : 1];
 #pragma unroll
         for (int i = 0; i < kRows; ++i) {
-            rx[i] = Raw<T>{};
-            rd[i] = Raw<T>{};
-            const int h = u.head0 + i * (32 / G) + sub;
-            if (live && h < u.heads) {
-                rx[i] = load_raw(x + h * hstride + e0);
-                rd[i] = load_raw(dy + (row0 + h) * p.d + e0);
-            }
+            const int h = min(head0 + i * kSub, heads - 1);
+            rx[i] = load_raw(row + h * head_stride, o0, o1);
+            if constexpr (kGrad) rd[i] = load_raw(dy + (flat + h) * p.d, o0, o1);
         }
-        Angles a;
-        load_angles(p, pos, e0, a);
-        float wt[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) wt[i] = 1.f;
-        if (weight != nullptr && live) load8(weight + e0, wt);
+        const int pos = p.positions[token];
+        if (!in_tables(p, pos)) {
+            report_position();
+            continue;
+        }
+        float4 c = make_float4(1.f, 1.f, 1.f, 1.f), sn = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (turned) {
+            const int64_t at = static_cast<int64_t>(pos) * (p.rot / 2) + 4 * li;
+            c = *reinterpret_cast<const float4*>(p.cos + at);
+            sn = *reinterpret_cast<const float4*>(p.sin + at);
+            if (kGrad) sn = make_float4(-sn.x, -sn.y, -sn.z, -sn.w);  // the opposite angles
+        }
+        const Angles<kInter> a = angles<kInter>(c, sn);
 #pragma unroll
         for (int i = 0; i < kRows; ++i) {
-            const int h = u.head0 + i * (32 / G) + sub;
-            float v[8], g[8], ss = 0.f, dot = 0.f;
+            uint64_t v[4], ss = 0;
             unpack(rx[i], v);
-            unpack(rd[i], g);
-            rotate8(p, e0, a, -1.f, g);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                ss = fmaf(v[j], v[j], ss);
-                dot = fmaf(v[j] * wt[j], g[j], dot);
-            }
-            const float r = 1.f / sqrtf(group_sum<G>(ss) / p.d + p.eps);
-            const float back = group_sum<G>(dot) / p.d * (r * r);
+            for (int j = 0; j < 4; ++j) ss = fma2(v[j], v[j], ss);
+            const bool mine = live && head0 + i * kSub < heads;
+            if constexpr (!kGrad) {
+                const float r =
+                    rsqrtf(fmaf(group_sum<G>(live ? sum_pair(ss) : 0.f), inv_d, p.eps));
+                const uint64_t rr = pair(r, r);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float t = v[j] * r * g[j];
-                if (u.is_k) wsum[1][j] += t;
-                else wsum[0][j] += t;
-                v[j] = r * (wt[j] * g[j] - v[j] * back);
+                for (int j = 0; j < 4; ++j) v[j] = mul2(v[j], mul2(wt[j], rr));
+                rotate(a, v);
+            } else {
+                uint64_t g[4], t[4], dot = 0;
+                unpack(rd[i], g);
+                rotate(a, g);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    t[j] = mul2(v[j], g[j]);
+                    dot = fma2(t[j], wt[j], dot);
+                }
+                const float r =
+                    rsqrtf(fmaf(group_sum<G>(live ? sum_pair(ss) : 0.f), inv_d, p.eps));
+                const float back =
+                    -group_sum<G>(live ? sum_pair(dot) : 0.f) * inv_d * (r * r * r);
+                const float r_own = mine ? r : 0.f;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    wsum[j] = fma2(t[j], pair(r_own, r_own), wsum[j]);
+                    v[j] = fma2(v[j], pair(back, back), mul2(g[j], mul2(wt[j], pair(r, r))));
+                }
             }
-            if (live && h < u.heads) store8(dx + (row0 + h) * p.d + e0, v);
+            if (mine) store(y + (flat + head0 + i * kSub) * p.d, o0, o1, v);
         }
     }
-    if (part == nullptr) return;
+    if constexpr (kGrad) {
+        if (part == nullptr) return;
+        for (int e = lane; e < p.d; e += 32) acc[2 * warp + !is_k][e] = 0.f;
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
+        for (int j = 0; j < 8; ++j) {
+            float u, v;
+            unpair(wsum[j >> 1], u, v);
+            float t = j & 1 ? v : u;
 #pragma unroll
-        for (int w = 0; w < 2; ++w) {
-            float x = wsum[w][j];
-#pragma unroll
-            for (int o = G; o < 32; o <<= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-            if (sub == 0 && live) acc[2 * warp + w][e0 + j] = x;
+            for (int o = G; o < 32; o <<= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+            if (sub == 0 && live) acc[2 * warp + is_k][(j < 4 ? o0 : o1 - 4) + j] = t;
         }
-    block_weights(p, acc, part);
+        block_weights(p, acc, part);
+    }
 }
 
 // Any width up to 256, any strides: one warp per row, lane l holding features
@@ -310,15 +285,21 @@ norm_rope_any(const NormRope p, int64_t rows, float* part) {
     for (int j = 0; j < kE; ++j) wsum[0][j] = wsum[1][j] = 0.f;
     const int64_t step = static_cast<int64_t>(gridDim.x) * kWarps;
     for (int64_t row = static_cast<int64_t>(blockIdx.x) * kWarps + warp; row < rows; row += step) {
-        const Unit u = unit_of(p, row, 1);
-        int64_t pos;
-        if (!position_of(p, u.token, pos)) continue;
-        const T* x = u.is_k ? static_cast<const T*>(p.k) + u.token * p.k_token + u.head0 * p.k_head
-                            : static_cast<const T*>(p.q) + u.token * p.q_token + u.head0 * p.q_head;
-        const int64_t flat = (u.token * u.heads + u.head0) * p.d;
-        const T* dy = kGrad ? static_cast<const T*>(u.is_k ? p.dk_out : p.dq_out) + flat : nullptr;
-        T* y = static_cast<T*>(u.is_k ? p.k_out : p.q_out) + flat;
-        const float* weight = u.is_k ? p.k_weight : p.q_weight;
+        const int64_t token = row / (p.heads_q + p.heads_k);
+        int h = static_cast<int>(row - token * (p.heads_q + p.heads_k));
+        const bool is_k = h >= p.heads_q;
+        if (is_k) h -= p.heads_q;
+        const int64_t pos = p.positions[token];
+        if (!in_tables(p, static_cast<int>(pos))) {
+            report_position();
+            continue;
+        }
+        const T* x = is_k ? static_cast<const T*>(p.k) + token * p.k_token + h * p.k_head
+                          : static_cast<const T*>(p.q) + token * p.q_token + h * p.q_head;
+        const int64_t flat = (token * (is_k ? p.heads_k : p.heads_q) + h) * p.d;
+        const T* dy = kGrad ? static_cast<const T*>(is_k ? p.dk_out : p.dq_out) + flat : nullptr;
+        T* y = static_cast<T*>(is_k ? p.k_out : p.q_out) + flat;
+        const float* weight = is_k ? p.k_weight : p.q_weight;
         auto wt = [&](int e) { return weight != nullptr ? weight[e] : 1.f; };
         float v[kE], ss = 0.f;
 #pragma unroll
@@ -353,7 +334,7 @@ norm_rope_any(const NormRope p, int64_t rows, float* part) {
             if (e >= p.d) continue;
             if (kGrad) {
                 const float t = v[j] * r * g[j];
-                if (u.is_k) wsum[1][j] += t;
+                if (is_k) wsum[1][j] += t;
                 else wsum[0][j] += t;
                 y[e] = from_f32<T>(r * (wt(e) * g[j] - v[j] * back));
             } else {
@@ -372,36 +353,30 @@ norm_rope_any(const NormRope p, int64_t rows, float* part) {
     }
 }
 
-// d_weight[e] = sum over the blocks' rows of `part`, 8 warps each a run of
-// blocks, joined in order.
+// d_weight[e] = sum over the blocks' rows of `part`: 8 columns a CTA, 32 runs of rows
+// joined in order.
 __global__ void __launch_bounds__(kThreads)
 sum_weights(const float* part, int blocks, int d, float* dq_weight, float* dk_weight) {
-    __shared__ float run[kWarps][32];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int i = blockIdx.x * 32 + lane;  // of 2 d
-    const int each = (blocks + kWarps - 1) / kWarps;
+    __shared__ float run[kThreads];
+    const int c = threadIdx.x & 7, r = threadIdx.x >> 3;
+    const int i = blockIdx.x * 8 + c;  // of 2 d
     float s = 0.f;
     if (i < 2 * d)
-        for (int b = warp * each; b < min(blocks, (warp + 1) * each); ++b)
-            s += part[static_cast<int64_t>(b) * 2 * d + i];
-    run[warp][lane] = s;
+#pragma unroll 4
+        for (int b = r; b < blocks; b += kThreads / 8) s += part[static_cast<int64_t>(b) * 2 * d + i];
+    run[threadIdx.x] = s;
     __syncthreads();
-    if (warp != 0 || i >= 2 * d) return;
+    if (r != 0 || i >= 2 * d) return;
     s = 0.f;
-    for (int w = 0; w < kWarps; ++w) s += run[w][lane];
+    for (int w = 0; w < kThreads / 8; ++w) s += run[8 * w + c];
     float* out = i < d ? dq_weight : dk_weight;
     if (out != nullptr) out[i < d ? i : i - d] = s;
 }
 
-int64_t unit_count(const NormRope& p, int per) {
-    return p.tokens * ((p.heads_q + per - 1) / per + (p.heads_k + per - 1) / per);
-}
-
-// 16-byte accesses need these; else the scalar kernel.
+// Accesses of four features need these; else the scalar kernel.
 bool vectors(const NormRope& p) {
-    const int es = p.dtype == GDR_DTYPE_F32 ? 4 : 2, e16 = 16 / es;
-    if (p.d % 8 || (p.interleaved ? p.rot % 8 : (p.rot / 2) % 8)) return false;
-    if (p.q_token % e16 || p.q_head % e16 || p.k_token % e16 || p.k_head % e16) return false;
+        if (p.d % 8 || p.rot % 8) return false;
+    if (p.q_token % 4 || p.q_head % 4 || p.k_token % 4 || p.k_head % 4) return false;
     uintptr_t a = 0;
     for (const void* x : {p.q, p.k, static_cast<const void*>(p.q_out),
                           static_cast<const void*>(p.k_out), p.dq_out, p.dk_out,
@@ -412,55 +387,91 @@ bool vectors(const NormRope& p) {
     return (a & 15) == 0;
 }
 
-template <typename T, int G, int kRows>
-void start_vec(const NormRope& p, float* part, int blocks, cudaStream_t s) {
-    const int64_t units = unit_count(p, (32 / G) * kRows);
+// What a call launches.
+struct Launch {
+    int blocks;
+    uint32_t q_warps;  // vector kernels
+};
+
+int sm_count() {
+    int dev = 0, n = 0;
+    cudaGetDevice(&dev);
+    cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+    return n > 0 ? n : 148;
+}
+
+// Rows a lane group takes at once: four, or in the gradient (two tensors' rows, and
+// the next unit's) two; one where that leaves SMs without work.
+int lanes_of(const NormRope& p) { return p.d <= 64 ? 8 : p.d <= 128 ? 16 : 32; }
+int rows_of(const NormRope& p) {
+    const int rows = p.dq_out != nullptr ? 2 : 4;
+    const int64_t units = p.tokens * (p.heads_q + p.heads_k) / (32 / lanes_of(p) * rows);
+    return units < 2 * kWarps * sm_count() ? 1 : rows;
+}
+
+Launch launch_of(const NormRope& p) {
+    const int64_t rows = p.tokens * (p.heads_q + p.heads_k);
+    const int per = vectors(p) ? 32 / lanes_of(p) * rows_of(p) : 1;
+    const int64_t want = (rows / per + kWarps) / kWarps;
+    const int64_t most = static_cast<int64_t>(sm_count()) * (p.dq_out != nullptr ? 3 : kWaves * 4);
+    Launch l;
+    l.blocks = static_cast<int>(want < 1 ? 1 : want < most ? want : most);
+    const int64_t warps = static_cast<int64_t>(l.blocks) * kWarps;
+    int64_t q = warps * p.heads_q / (p.heads_q + p.heads_k);
+    l.q_warps = static_cast<uint32_t>(q < 1 ? 1 : q > warps - 1 ? warps - 1 : q);
+    return l;
+}
+
+template <typename T, int G, bool kInter>
+void start_rows(const NormRope& p, float* part, Launch l, cudaStream_t s) {
+    const bool one = rows_of(p) == 1;
     if (p.dq_out != nullptr)
-        norm_rope_grad_vec<T, G, kRows><<<blocks, kThreads, 0, s>>>(p, units, part);
+        (one ? norm_rope_vec<T, G, 1, kInter, true> : norm_rope_vec<T, G, 2, kInter, true>)
+            <<<l.blocks, kThreads, 0, s>>>(p, l.q_warps, part);
     else
-        norm_rope_vec<T, G, kRows>
-            <<<static_cast<unsigned>((units + kWarps - 1) / kWarps), kThreads, 0, s>>>(p, units);
+        (one ? norm_rope_vec<T, G, 1, kInter, false> : norm_rope_vec<T, G, 4, kInter, false>)
+            <<<l.blocks, kThreads, 0, s>>>(p, l.q_warps, nullptr);
+}
+
+template <typename T, int G>
+void start_pairs(const NormRope& p, float* part, Launch l, cudaStream_t s) {
+    p.interleaved ? start_rows<T, G, true>(p, part, l, s) : start_rows<T, G, false>(p, part, l, s);
 }
 
 template <typename T>
-void start(const NormRope& p, float* part, int blocks, cudaStream_t s) {
+void start(const NormRope& p, float* part, Launch l, cudaStream_t s) {
     if (!vectors(p)) {
-        const int64_t rows = unit_count(p, 1);
+        const int64_t rows = p.tokens * (p.heads_q + p.heads_k);
         if (p.dq_out != nullptr)
-            norm_rope_any<T, true><<<blocks, kThreads, 0, s>>>(p, rows, part);
+            norm_rope_any<T, true><<<l.blocks, kThreads, 0, s>>>(p, rows, part);
         else
-            norm_rope_any<T, false><<<blocks, kThreads, 0, s>>>(p, rows, nullptr);
+            norm_rope_any<T, false><<<l.blocks, kThreads, 0, s>>>(p, rows, nullptr);
         return;
     }
-    // Four rows per lane group, or one when that leaves SMs without work.
-    const bool few = unit_count(p, (p.d <= 64 ? 4 : p.d <= 128 ? 2 : 1) * 4) < 148 * kWarps;
-    if (p.d <= 64) few ? start_vec<T, 8, 1>(p, part, blocks, s) : start_vec<T, 8, 4>(p, part, blocks, s);
-    else if (p.d <= 128) few ? start_vec<T, 16, 1>(p, part, blocks, s) : start_vec<T, 16, 4>(p, part, blocks, s);
-    else few ? start_vec<T, 32, 1>(p, part, blocks, s) : start_vec<T, 32, 4>(p, part, blocks, s);
+    switch (lanes_of(p)) {
+        case 8: start_pairs<T, 8>(p, part, l, s); break;
+        case 16: start_pairs<T, 16>(p, part, l, s); break;
+        default: start_pairs<T, 32>(p, part, l, s);
+    }
 }
 
 }  // namespace
 
 int norm_rope_max_d() { return kMaxD; }
 
-// Blocks of a gradient call (its weights' partial sums: one row of 2 d each)
-// and of the scalar forward kernel.
-int norm_rope_blocks(const NormRope& p) {
-    const int64_t warps = (unit_count(p, 1) + 3) / 4;
-    const int64_t want = (warps + kWarps - 1) / kWarps;
-    return static_cast<int>(want < 148 * 4 ? (want > 0 ? want : 1) : 148 * 4);
-}
+// Blocks of a gradient call: its weights' partial sums are one row of 2 d each.
+int norm_rope_blocks(const NormRope& p) { return launch_of(p).blocks; }
 
 cudaError_t launch_norm_rope(const NormRope& p, float* part, cudaStream_t s) {
-    const int blocks = norm_rope_blocks(p);
+    const Launch l = launch_of(p);
     switch (p.dtype) {
-        case GDR_DTYPE_BF16: start<__nv_bfloat16>(p, part, blocks, s); break;
-        case GDR_DTYPE_F16: start<__half>(p, part, blocks, s); break;
-        default: start<float>(p, part, blocks, s); break;
+        case GDR_DTYPE_BF16: start<__nv_bfloat16>(p, part, l, s); break;
+        case GDR_DTYPE_F16: start<__half>(p, part, l, s); break;
+        default: start<float>(p, part, l, s); break;
     }
     if (part != nullptr)
-        sum_weights<<<(2 * p.d + 31) / 32, kThreads, 0, s>>>(part, blocks, p.d, p.dq_weight,
-                                                             p.dk_weight);
+        sum_weights<<<(2 * p.d + 7) / 8, kThreads, 0, s>>>(part, l.blocks, p.d, p.dq_weight,
+                                                           p.dk_weight);
     return cudaGetLastError();
 }
 

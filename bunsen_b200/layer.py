@@ -111,39 +111,42 @@ def state_reorder(src, sources, out=None):
 
 def _rope_args(q, k, positions, cos, sin, q_weight, k_weight, eps, interleaved):
     """The checks and the call's struct, the tensors it points at and the
-    leading shape of ``qk_norm_rope``."""
-    if q.dtype not in _DTYPES or k.dtype != q.dtype:
+    device of ``qk_norm_rope``."""
+    qs, ks, dtype, dev = q.shape, k.shape, q.dtype, q.device
+    if dtype not in _DTYPES or k.dtype != dtype:
         raise TypeError("q and k share one dtype, f32, bf16 or f16")
-    if q.dim() < 3 or k.dim() != q.dim() or k.shape[:-2] != q.shape[:-2] \
-            or k.shape[-1] != q.shape[-1]:
+    if len(qs) < 3 or len(ks) != len(qs) or ks[:-2] != qs[:-2] or ks[-1] != qs[-1]:
         raise ValueError(f"q is [..., H_q, d] and k [..., H_k, d] with the same leading dims; got "
-                         f"{tuple(q.shape)} and {tuple(k.shape)}")
-    lead, d = q.shape[:-2], q.shape[-1]
-    if positions.shape != lead or positions.dtype not in (torch.int32, torch.int64):
-        raise ValueError(f"positions are int32 or int64 {tuple(lead)}, one for each token")
-    if cos.dim() != 2 or sin.shape != cos.shape or not 0 < 2 * cos.shape[1] <= d \
-            or cos.shape[0] == 0:
+                         f"{tuple(qs)} and {tuple(ks)}")
+    d = qs[-1]
+    if positions.shape != qs[:-2] or positions.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"positions are int32 or int64 {tuple(qs[:-2])}, one for each token")
+    table = cos.shape
+    if len(table) != 2 or sin.shape != table or not 0 < 2 * table[1] <= d or table[0] == 0:
         raise ValueError("cos and sin are [positions, rotary_dim / 2], rotary_dim at most d")
     for w in (q_weight, k_weight):
-        if w is not None and tuple(w.shape) != (d,):
+        if w is not None and w.shape != (d,):
             raise ValueError(f"the weights are [d] = ({d},)")
-    dev = q.device
     if dev.type != "cuda":
         raise RuntimeError("libgdr runs on CUDA tensors only")
     for x in (k, positions, cos, sin, q_weight, k_weight):
         if x is not None and x.device != dev:
             raise ValueError(f"every tensor is on q's device {dev}; got one on {x.device}")
     q, k = _token_rows(q), _token_rows(k)
-    if positions.dtype != torch.int32:  # far positions stay outside the tables
+    if positions.dtype is not torch.int32:  # far positions stay outside the tables
         positions = positions.clamp(-1, 2**31 - 1).to(torch.int32)
     positions = positions.contiguous()
-    cos, sin = cos.to(torch.float32).contiguous(), sin.to(torch.float32).contiguous()
-    q_weight, k_weight = (None if w is None else w.to(torch.float32).contiguous()
-                          for w in (q_weight, k_weight))
-    p = _lib.GdrQkNormRopeParams(
-        q.shape[0], q.stride(0), q.stride(1), k.stride(0), k.stride(1), q.shape[1], k.shape[1], d,
-        2 * cos.shape[1], cos.shape[0], int(interleaved), _DTYPES[q.dtype], float(eps))
-    return p, (q, k, positions, cos, sin, q_weight, k_weight), lead, dev
+    cos, sin, q_weight, k_weight = _f32(cos), _f32(sin), _f32(q_weight), _f32(k_weight)
+    (tokens, h_q, _), (q0, q1, _), (k0, k1, _) = q.shape, q.stride(), k.stride()
+    p = _lib.GdrQkNormRopeParams(tokens, q0, q1, k0, k1, h_q, k.shape[1], d, 2 * table[1], table[0],
+                                 int(interleaved), _DTYPES[dtype], float(eps))
+    return p, (q, k, positions, cos, sin, q_weight, k_weight), dev
+
+
+def _f32(x):
+    if x is None or (x.dtype is torch.float32 and x.is_contiguous()):
+        return x
+    return x.to(torch.float32).contiguous()
 
 
 def _token_rows(x):
@@ -163,7 +166,7 @@ def qk_norm_rope(q, k, positions, cos, sin, q_weight=None, k_weight=None, eps=1e
     ``interleaved``. One pass; q and k may be strided parts of one tensor.
     Returns new contiguous ``(q, k)`` in q's dtype. A position outside the
     tables leaves its rows unwritten; ``gdr_device_error`` reports it."""
-    p, x, lead, dev = _rope_args(q, k, positions, cos, sin, q_weight, k_weight, eps, interleaved)
+    p, x, dev = _rope_args(q, k, positions, cos, sin, q_weight, k_weight, eps, interleaved)
     q_out = torch.empty(q.shape, dtype=q.dtype, device=dev)
     k_out = torch.empty(k.shape, dtype=k.dtype, device=dev)
     on_device(dev, "gdr_qk_norm_rope", ctypes.byref(p), *(_ptr(t) for t in x), q_out.data_ptr(),
@@ -177,7 +180,7 @@ def qk_norm_rope_backward(dq_out, dk_out, q, k, positions, cos, sin, q_weight=No
     dq_weight, dk_weight)``, dq and dk contiguous in q's dtype, the weights' in
     f32 (None for a weight that is None), summed over all rows in a fixed order. A row
     whose position is outside the tables is left unwritten and adds nothing."""
-    p, x, lead, dev = _rope_args(q, k, positions, cos, sin, q_weight, k_weight, eps, interleaved)
+    p, x, dev = _rope_args(q, k, positions, cos, sin, q_weight, k_weight, eps, interleaved)
     for g, y in ((dq_out, q), (dk_out, k)):
         if g.shape != y.shape or g.dtype != y.dtype or g.device != dev:
             raise ValueError("dq_out and dk_out are shaped, typed and placed like q and k")

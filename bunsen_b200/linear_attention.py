@@ -89,51 +89,50 @@ class LinearAttention:
     # -- plumbing ------------------------------------------------------------
     def _check(self, q, k, v, log_decay, state, cu_seqlens):
         """The shape contract; returns the device and the number of sequences."""
+        qs, vs, dtype, dev = q.shape, v.shape, q.dtype, q.device
         rank = 4 if cu_seqlens is None else 3
-        if q.dim() != rank:
+        if len(qs) != rank:
             raise ValueError(f"q is {'[B, T, H, Dk]' if rank == 4 else '[T, H, Dk]'}; "
-                             f"got {tuple(q.shape)}")
-        if k.shape != q.shape:
-            raise ValueError(f"k {tuple(k.shape)} must match q {tuple(q.shape)}")
-        if v.dim() != rank or v.shape[:-2] != q.shape[:-2]:
-            raise ValueError(f"v {tuple(v.shape)} must share q's leading dims "
-                             f"{tuple(q.shape[:-2])}")
-        h_qk, h_v = q.shape[-2], v.shape[-2]
+                             f"got {tuple(qs)}")
+        if k.shape != qs:
+            raise ValueError(f"k {tuple(k.shape)} must match q {tuple(qs)}")
+        if len(vs) != rank or vs[:-2] != qs[:-2]:
+            raise ValueError(f"v {tuple(vs)} must share q's leading dims {tuple(qs[:-2])}")
+        h_qk, h_v = qs[-2], vs[-2]
         if h_qk == 0 or h_v == 0 or h_v % h_qk != 0:
             raise ValueError(f"{h_qk} key heads must divide {h_v} value heads")
-        if q.dtype not in _DTYPES:
-            raise TypeError(f"q, k, v in f32, bf16 or f16, not {q.dtype}")
-        if k.dtype != q.dtype or v.dtype != q.dtype:
+        if dtype not in _DTYPES:
+            raise TypeError(f"q, k, v in f32, bf16 or f16, not {dtype}")
+        if k.dtype != dtype or v.dtype != dtype:
             raise TypeError("q, k and v share one dtype")
-        if tuple(log_decay.shape) != (h_v,):
+        if log_decay.shape != (h_v,):
             raise ValueError(f"log_decay is [H_v] = ({h_v},); got {tuple(log_decay.shape)}")
         if cu_seqlens is None:
-            n = q.shape[0]
+            n = qs[0]
         else:
             if cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1:
                 raise ValueError("cu_seqlens holds n_seqs + 1 offsets")
             n = cu_seqlens.numel() - 1
         if state is not None:
-            want = (n, h_v, q.shape[-1], v.shape[-1])
-            if tuple(state.shape) != want:
-                raise ValueError(f"the state is [N, H_v, d_k, d_v] = {want}; "
+            if state.shape != (n, h_v, qs[-1], vs[-1]):
+                raise ValueError(f"the state is [N, H_v, d_k, d_v] = {(n, h_v, qs[-1], vs[-1])}; "
                                  f"got {tuple(state.shape)}")
         if self.scale is not None and not math.isfinite(self.scale):
             raise ValueError("scale is finite")
-        dev = q.device
         if dev.type != "cuda":
             raise RuntimeError("libgdr runs on CUDA tensors only")
         _same_device(dev, k, v, log_decay, state)
         return dev, n
 
     def _params(self, q, v, cu_seqlens, n):
-        dense = cu_seqlens is None
+        vs = v.shape
         h_qk, d_k = q.shape[-2:]
-        h_v, d_v = v.shape[-2:]
-        return _lib.GdrLaParams(n if dense else 0, q.shape[1] if dense else q.shape[0],
-                                0 if dense else n, h_qk, h_v, d_k, d_v, _DTYPES[q.dtype],
-                                _ALGOS[self.algo], self.split_chunks,
-                                d_k ** -0.5 if self.scale is None else self.scale)
+        scale = d_k ** -0.5 if self.scale is None else self.scale
+        if cu_seqlens is None:
+            return _lib.GdrLaParams(n, vs[1], 0, h_qk, vs[2], d_k, vs[3], _DTYPES[q.dtype],
+                                    _ALGOS[self.algo], self.split_chunks, scale)
+        return _lib.GdrLaParams(0, vs[0], n, h_qk, vs[1], d_k, vs[2], _DTYPES[q.dtype],
+                                _ALGOS[self.algo], self.split_chunks, scale)
 
     def _forward(self, fn, q, k, v, log_decay, state, cu_seqlens, out, state_out):
         dev, n = self._check(q, k, v, log_decay, state, cu_seqlens)
@@ -144,11 +143,12 @@ class LinearAttention:
             out = torch.empty_like(v)
         else:
             _output(out, v.shape, q.dtype, dev, "out")
-        want = (n, v.shape[-2], q.shape[-1], v.shape[-1])
         if state_out is None:
-            state_out = torch.empty(want, dtype=torch.float32, device=dev)
+            state_out = torch.empty((n, v.shape[-2], q.shape[-1], v.shape[-1]),
+                                    dtype=torch.float32, device=dev)
         else:
-            _output(state_out, want, torch.float32, dev, "state_out")
+            _output(state_out, (n, v.shape[-2], q.shape[-1], v.shape[-1]), torch.float32, dev,
+                    "state_out")
         p = self._params(q, v, cu_seqlens, n)
         on_device(dev, fn, ctypes.byref(p), q.data_ptr(), k.data_ptr(), v.data_ptr(),
                   log_decay.data_ptr(), _ptr(state), out.data_ptr(), state_out.data_ptr(),
@@ -157,12 +157,15 @@ class LinearAttention:
 
 
 def _f32(x):
-    return None if x is None else x.to(torch.float32).contiguous()
+    if x is None or (x.dtype is torch.float32 and x.is_contiguous()):
+        return x
+    return x.to(torch.float32).contiguous()
 
 
 def _offsets(cu_seqlens, dev):
-    if cu_seqlens is None:
-        return None
+    if cu_seqlens is None or (cu_seqlens.dtype is torch.int32 and cu_seqlens.device == dev
+                              and cu_seqlens.is_contiguous()):
+        return cu_seqlens
     return cu_seqlens.to(device=dev, dtype=torch.int32).contiguous()
 
 
@@ -173,6 +176,5 @@ def _same_device(dev, *tensors):
 
 
 def _output(x, shape, dtype, dev, name):
-    if tuple(x.shape) != tuple(shape) or x.dtype != dtype or x.device != dev \
-            or not x.is_contiguous():
+    if x.shape != shape or x.dtype != dtype or x.device != dev or not x.is_contiguous():
         raise ValueError(f"{name} is a contiguous {dtype} {tuple(shape)} on {dev}")

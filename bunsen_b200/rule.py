@@ -42,15 +42,21 @@ def _stream(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+_current_stream = torch._C._cuda_getCurrentRawStream  # by device index: the raw handle
+
+
 def on_device(device: torch.device, fn: str, *args) -> None:
     """Calls libgdr's ``fn`` with ``args`` and the current stream of ``device``,
     with that device current (the library launches on the current one)."""
     call = getattr(_lib.load(), fn)
-    if device.index == torch.cuda.current_device():
-        _lib.check(fn, call(*args, _stream(device)))
+    index = device.index
+    if index == torch.cuda.current_device():
+        status = call(*args, _current_stream(index))
     else:
         with torch.cuda.device(device):
-            _lib.check(fn, call(*args, _stream(device)))
+            status = call(*args, _current_stream(index))
+    if status:
+        _lib.check(fn, status)
 
 
 def _layer_io(gates, norm, q, v, g, beta):

@@ -365,7 +365,8 @@ gdr_status gdr_la_backward(const gdr_la_params* params, const void* q, const voi
  * contiguous; outputs are contiguous and must not overlap inputs. cos and sin
  * are f32 [table_rows, rotary_dim / 2]. A position outside the tables leaves
  * its rows unwritten and is reported by gdr_device_error as GDR_ERR_INVALID.
- * head_dim up to 256 (else GDR_ERR_UNSUPPORTED). */
+ * head_dim up to 256, fewer than 2^31 head vectors (else
+ * GDR_ERR_UNSUPPORTED). */
 typedef struct gdr_qk_norm_rope_params {
     int64_t tokens;
     int64_t q_token_stride;
