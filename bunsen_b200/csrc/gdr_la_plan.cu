@@ -76,26 +76,31 @@ la_plan(const LaCore p, LaPlan* plan, LaEntry* main, LaEntry* states, LaSplit* s
     };
     {
         const int L = candidate(warp);
-        int again = 0, parts_most = 0, segs = 0;
+        int again = 0, parts_most = 0, segs = 0, whole = 0;  // whole: segments of L chunks
         for (int s = lane; s < p.n_seqs; s += 32) {
             const int c = chunks(s, start, len);
             if (c > L) {
                 const int parts = (c + L - 1) / L;
                 again += (parts - 1) * L;
                 segs += parts;
+                whole += c / L;
                 parts_most = max(parts_most, parts);
             }
         }
         for (int o = 16; o > 0; o >>= 1) {
             again += __shfl_xor_sync(0xffffffffu, again, o);
             segs += __shfl_xor_sync(0xffffffffu, segs, o);
+            whole += __shfl_xor_sync(0xffffffffu, whole, o);
             parts_most = max(parts_most, __shfl_xor_sync(0xffffffffu, parts_most, o));
         }
+        // A pass takes the work's share of a CTA, and at least the most whole segments
+        // that fall to one.
         const float longest = static_cast<float>(min(L, most));
-        float t = fmaxf(longest, sum * each * 1.03f + 1.f);
+        float t = fmaxf(longest * ceilf(whole * each), sum * each * 1.03f + 1.f);
+        t = fmaxf(t, longest);
         if (again > 0)
-            t += how.state_cost * fmaxf(longest, again * each * 1.03f + 1.f) + how.fixed_cost +
-                 kLinkCost * parts_most;
+            t += how.state_cost * fmaxf(longest * ceilf(again * each / L), again * each * 1.03f) +
+                 how.fixed_cost + kLinkCost * parts_most;
         if (segs > seg_cap) t = INFINITY;
         if (lane == 0) cost[warp] = t;
     }

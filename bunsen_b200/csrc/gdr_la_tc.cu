@@ -71,7 +71,7 @@ constexpr uint32_t kHalf = kTile / 2;
 constexpr uint32_t kStage = 3 * kTile;    // a, b, c
 constexpr uint32_t kOffSb = 2 * kStage, kOffMisc = kOffSb + kTile;
 constexpr uint32_t kSmemBytes = kOffMisc + 512;
-constexpr uint32_t kColU = 0, kColP = 128, kColO = 256, kColW = 384, kColWBuf = 48;
+constexpr uint32_t kColU = 0, kColP = 128, kColO = 256, kColWBuf = 48;
 constexpr int kWaitRounds = 1 << 24;  // of two tries: seconds
 
 // What a CTA works on next: the positions [start, start + len) of a sequence with
@@ -81,11 +81,13 @@ struct Job {
 };
 constexpr int kJobs = 4;  // in flight between the loading warp and the other roles
 
+constexpr int kRingMost = 8;
+
 struct Bars {
     uint64_t a_full[2], b_full[2], c_full[2], a_free[2], c_read[2], o_staged[2];
     uint64_t in_full[2], o_full[2], u_full[2];
     uint64_t sc_full, pa_ready, sb_ready, o_free, u_free, fix[2], drain[2];
-    uint64_t wv_full[2], wv_free[2];
+    uint64_t wv_full[kRingMost], wv_free[kRingMost];
     uint64_t job_full[kJobs], job_free[kJobs];
     uint32_t tmem;
     Job jobs[kJobs];
@@ -182,6 +184,18 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint64_t (&v)[8]
     tmem_st16(taddr, r);
 }
 
+// 32 lanes x 8 columns, as pairs of columns, arrived.
+__device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint64_t (&v)[4]) {
+    asm volatile(
+        "{\n\t.reg .b32 r<8>;\n\t"
+        "tcgen05.ld.sync.aligned.32x32b.x8.b32 {r0, r1, r2, r3, r4, r5, r6, r7}, [%4];\n\t"
+        "tcgen05.wait::ld.sync.aligned;\n\t"
+        "mov.b64 %0, {r0, r1};\n\tmov.b64 %1, {r2, r3};\n\t"
+        "mov.b64 %2, {r4, r5};\n\tmov.b64 %3, {r6, r7};\n\t}"
+        : "=l"(v[0]), "=l"(v[1]), "=l"(v[2]), "=l"(v[3])
+        : "r"(taddr)
+        : "memory");
+}
 // 32 lanes x 16 columns, as pairs of columns, arrived. (The loads take some 30
 // cycles; several in flight gained nothing.)
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint64_t (&v)[8]) {
@@ -303,7 +317,8 @@ __device__ __forceinline__ float low_f32(uint32_t p) { return __uint_as_float(p 
 __device__ __forceinline__ float high_f32(uint32_t p) { return __uint_as_float(p & 0xffff0000u); }
 
 // Moves registers between the roles: the launch gives each thread 72, 504 for
-// the seven warpgroups' lanes together: 2 x 72 + 2 x 96 + 2 x 64 + 40.
+// the seven warpgroups' lanes together: 2 x 72 + 2 x 96 + 2 x 64 + 40, and in the
+// states' pass 2 x 24 + 2 x 104 + 2 x 96 + 40.
 template <int kRegs>
 __device__ __forceinline__ void give_registers() {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegs));
@@ -357,9 +372,11 @@ la_tc(const LaCore p, const __grid_constant__ CUtensorMap ma,
             mbar_init(&B.o_full[i], 1);
             mbar_init(&B.u_full[i], 1);
             mbar_init(&B.fix[i], 8);
+            mbar_init(&B.drain[i], 1);
+        }
+        for (int i = 0; i < kRingMost; ++i) {
             mbar_init(&B.wv_full[i], 8);
             mbar_init(&B.wv_free[i], 1);
-            mbar_init(&B.drain[i], 1);
         }
         for (int i = 0; i < kJobs; ++i) {
             mbar_init(&B.job_full[i], 1);
@@ -383,6 +400,8 @@ la_tc(const LaCore p, const __grid_constant__ CUtensorMap ma,
     // All 512 columns are this CTA's, so they begin at 0: a constant, as the
     // tiles' addresses are, keeps the products' operands in uniform registers.
     constexpr uint32_t tm = 0;
+    // Buffers of (w c)^T: the room beside U^T, or what the scores and O leave.
+    constexpr uint32_t kRing = kStateOnly ? kRingMost : 2, kColW = kStateOnly ? 128 : 384;
     if (B.tmem != 0 || (smem_u32(sm) & 1023) != 0) ok = false;  // never: nothing would be right
     // The job of a slot that is full, and the slot given back (its warp converged).
     auto take = [&](uint32_t slot) {
@@ -533,12 +552,12 @@ la_tc(const LaCore p, const __grid_constant__ CUtensorMap ma,
         {
             constexpr uint32_t kKMn = idesc_bf16(128, 128, 0, 1, 0);
             const uint32_t base = smem_u32(sm);
-            auto update = [&](uint32_t st, uint32_t q) {  // 32 positions, in buffer q % 2
-                product_ts3(tm + kColU, tm + kColW + (q & 1) * kColWBuf,
+            auto update = [&](uint32_t st, uint32_t q, uint32_t buf) {  // 32 positions
+                product_ts3(tm + kColU, tm + kColW + buf * kColWBuf,
                             sdesc_sw128(base + st * kStage + kTile + q * 4096, kHalf, 1024), kKMn,
                             q);
             };
-            uint32_t n = 0, tails = 0;
+            uint32_t n = 0, w = 0, tails = 0;
 #pragma unroll 1
             for (uint32_t k = 0; ok; ++k) {
                 if (!(ok = warp_wait(&B.job_full[k % kJobs], k / kJobs & 1))) break;
@@ -555,13 +574,13 @@ la_tc(const LaCore p, const __grid_constant__ CUtensorMap ma,
                     }
                     if (n > 0 && !(ok = warp_wait(&B.u_free, (n & 1) ^ 1))) break;
 #pragma unroll 1
-                    for (uint32_t q = 0; q < 4; ++q) {
-                        // (Buffer q % 2 for the (2 n + q / 2)th time.)
-                        if (!ok || !(ok = warp_wait(&B.wv_full[q & 1], (q >> 1) & 1))) break;
+                    for (uint32_t q = 0; q < 4; ++q, ++w) {
+                        const uint32_t buf = w % kRing;
+                        if (!(ok = warp_wait(&B.wv_full[buf], w / kRing & 1))) break;
                         tc_fence_after();
                         if (elect_one()) {
-                            update(st, q);
-                            umma_commit(&B.wv_free[q & 1]);
+                            update(st, q, buf);
+                            umma_commit(&B.wv_free[buf]);
                             if (q == 3) umma_commit(&B.u_full[st]);
                         }
                     }
@@ -623,6 +642,7 @@ la_tc(const LaCore p, const __grid_constant__ CUtensorMap ma,
         __syncwarp();
     }
     } else if (warp < 8) {
+        if constexpr (kStateOnly) give_registers<24>();
         // ---- scores and outputs -------------------------------------------------------
         // Where w^-128 is far from overflow, the powers come out of the sums:
         //   out_i = tau w^{i+1} [ a_i . S + sum_{j<=i} sigma w^{-(j+1)} (a_i.b_j) c_j ]
@@ -790,11 +810,13 @@ la_tc(const LaCore p, const __grid_constant__ CUtensorMap ma,
             }
         }
     } else if (warp < 16) {
-        take_registers<96>();
+        take_registers<kStateOnly ? 104 : 96>();
         // ---- the state -----------------------------------------------------------
         const int col = 32 * (warp & 3) + lane;  // this thread's column of S (row of U^T),
         const int half = (warp - 8) >> 2, b0 = 64 * half;  // and its rows b0 .. b0 + 63
-        uint8_t* sb = sm + kOffSb + half * kHalf + col * 128;
+        // Its row of Sb: 16 bytes at x are at (row's first) ^ x.
+        const uint32_t sb =
+            smem_u32(sm + kOffSb) + half * kHalf + col * 128 + ((col & 7) << 4);
         uint32_t n = 0;  // chunks begun
         uint64_t s[32];  // pairs of its rows
 #pragma unroll 1
@@ -825,11 +847,14 @@ la_tc(const LaCore p, const __grid_constant__ CUtensorMap ma,
                 if constexpr (!kStateOnly) {
                     // The bf16 copy, once the last chunk's product has read its own.
                     if (n > 0 && !(ok = group_wait(&B.in_full[(n - 1) & 1], ((n - 1) >> 1) & 1, 2, warp == 9))) break;
+                    uint32_t to = sb;
+                    asm volatile("" : "+r"(to));  // (eight addresses kept would be registers)
 #pragma unroll
                     for (int m = 0; m < 8; ++m)
-                        *reinterpret_cast<uint4*>(sb + ((m ^ (col & 7)) << 4)) =
-                            make_uint4(pack_bf16(s[4 * m]), pack_bf16(s[4 * m + 1]),
-                                       pack_bf16(s[4 * m + 2]), pack_bf16(s[4 * m + 3]));
+                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to ^ (m << 4)),
+                                     "r"(pack_bf16(s[4 * m])), "r"(pack_bf16(s[4 * m + 1])),
+                                     "r"(pack_bf16(s[4 * m + 2])), "r"(pack_bf16(s[4 * m + 3]))
+                                     : "memory");
                     fence_proxy_async();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&B.sb_ready);
@@ -844,17 +869,17 @@ la_tc(const LaCore p, const __grid_constant__ CUtensorMap ma,
                 if (!(ok = group_wait(&B.u_full[n & 1], (n >> 1) & 1, 2, warp == 9))) break;
                 tc_fence_after();
 #pragma unroll
-                for (int blk = 0; blk < 4; ++blk) {
-                    uint64_t u[8];
-                    tmem_ld16(quad + kColU + b0 + 16 * blk, u);
-                    if (blk == 3) {
+                for (int blk = 0; blk < 8; ++blk) {
+                    uint64_t u[4];
+                    tmem_ld8(quad + kColU + b0 + 8 * blk, u);
+                    if (blk == 7) {
                         tc_fence_before();
                         __syncwarp();
                         if (lane == 0) mbar_arrive(&B.u_free);
                     }
 #pragma unroll
-                    for (int j = 0; j < 8; ++j)
-                        s[8 * blk + j] = fma2(s[8 * blk + j], hi2, fma2(s[8 * blk + j], lo2, u[j]));
+                    for (int j = 0; j < 4; ++j)
+                        s[4 * blk + j] = fma2(s[4 * blk + j], hi2, fma2(s[4 * blk + j], lo2, u[j]));
                 }
             }
             const LaState out = la_state(p, it.out, it.h, p.state_out, scratch);
@@ -870,7 +895,8 @@ la_tc(const LaCore p, const __grid_constant__ CUtensorMap ma,
             }
         }
     } else {
-        give_registers<64>();
+        if constexpr (kStateOnly) take_registers<96>();
+        else give_registers<64>();
         // ---- the update's operand ----------------------------------------------------
         // (w c)^T, features on the TMEM lanes: 8 x 8 blocks of the c tile come
         // transposed from ldmatrix, thread t holding feature t / 4 (and + 8)
@@ -921,10 +947,9 @@ la_tc(const LaCore p, const __grid_constant__ CUtensorMap ma,
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&B.fix[st]);
                 }
-#pragma unroll 1
-                for (int q = 0; q < 4; ++q, ++w) {
-                    const int buf = w & 1;
-                    uint32_t x[8];
+                // A quarter's values; in the states' pass, which has registers for them,
+                // the next one's on their way.
+                auto fetch = [&](int q, uint32_t (&x)[8]) {
 #pragma unroll
                     for (int g2 = 0; g2 < 2; ++g2)
                         asm volatile(
@@ -935,6 +960,20 @@ la_tc(const LaCore p, const __grid_constant__ CUtensorMap ma,
                             : "r"(src0 + st * kStage + (32 * q + 16 * g2) * 128 +
                                   ((chunk0 ^ (lane & 7)) << 4))
                             : "memory");
+                };
+                uint32_t next[8];
+                if constexpr (kStateOnly) fetch(0, next);
+#pragma unroll 1
+                for (int q = 0; q < 4; ++q, ++w) {
+                    const uint32_t buf = w % kRing;
+                    uint32_t x[8];
+                    if constexpr (kStateOnly) {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) x[i] = next[i];
+                        if (q < 3) fetch(q + 1, next);
+                    } else {
+                        fetch(q, x);
+                    }
                     if (q == 3) {
                         __syncwarp();
                         if (lane == 0) mbar_arrive(&B.c_read[st]);
@@ -969,7 +1008,9 @@ la_tc(const LaCore p, const __grid_constant__ CUtensorMap ma,
                             x[2 * k + 1] &= keep;
                         }
                     }
-                    if (w >= 2 && !(ok = group_wait(&B.wv_free[buf], ((w >> 1) & 1) ^ 1, 3, warp == 18))) break;
+                    if (w >= kRing &&
+                        !(ok = group_wait(&B.wv_free[buf], (w / kRing & 1) ^ 1, 3, warp == 18)))
+                        break;
                     tc_fence_after();
                     uint32_t mid[8], lo[8];
 #pragma unroll
