@@ -124,22 +124,6 @@ __device__ __forceinline__ bool elect_one() {
         : "=r"(p));
     return p != 0;
 }
-// The same for the eight warps of a role together, in step: one of them waits for
-// the phase, the others at a hardware barrier, which costs them no issue
-// slots (24 warps trying took more than half of all instructions). The
-// barrier carries the outcome, so that all of them go on or none.
-__device__ __forceinline__ bool group_wait(uint64_t* bar, uint32_t parity, uint32_t id, bool waits) {
-    uint32_t failed = 0;
-    if (waits) failed = !lane_wait(bar, parity);
-    uint32_t any;
-    asm volatile(
-        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\t"
-        "barrier.cta.red.or.pred q, %2, 256, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
-        : "=r"(any)
-        : "r"(failed), "r"(id)
-        : "memory");
-    return any == 0;
-}
 __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
@@ -663,7 +647,7 @@ la_tc(const LaCore p, const __grid_constant__ CUtensorMap ma,
         uint32_t n = 0;
 #pragma unroll 1
         for (uint32_t k = 0; !kStateOnly && ok; ++k) {
-            if (!(ok = group_wait(&B.job_full[k % kJobs], k / kJobs & 1, 1, warp == 0))) break;
+            if (!(ok = warp_wait(&B.job_full[k % kJobs], k / kJobs & 1))) break;
             const Job it = take(k % kJobs);
             if (it.len < 0) break;
             const int nch = (it.len + kC - 1) / kC;
@@ -696,7 +680,7 @@ la_tc(const LaCore p, const __grid_constant__ CUtensorMap ma,
                     }
                     known = len;
                 }
-                if (!(ok = group_wait(&B.sc_full, ph, 1, warp == 0))) break;
+                if (!(ok = warp_wait(&B.sc_full, ph))) break;
                 tc_fence_after();
 #pragma unroll 1
                 for (int cb = first; cb < last; ++cb) {
@@ -752,7 +736,7 @@ la_tc(const LaCore p, const __grid_constant__ CUtensorMap ma,
                 for (int cb = 2 * half; cb < 2 * half + 2; ++cb)
                     if (cb < first || cb >= last) tmem_st16(pcol + 16 * (cb & 1), zero);
                 if (!gentle) {
-                    if (!(ok = group_wait(&B.in_full[st], ph2, 1, warp == 0))) break;
+                    if (!(ok = warp_wait(&B.in_full[st], ph2))) break;
                     tc_fence_after();
 #pragma unroll 1
                     for (int blk = 0; blk < 4; ++blk) {
@@ -764,15 +748,15 @@ la_tc(const LaCore p, const __grid_constant__ CUtensorMap ma,
                         tmem_st16(at, o);
                     }
                 }
-                if (!(ok = group_wait(&B.c_full[st], ph2, 1, warp == 0))) break;
+                if (!(ok = warp_wait(&B.c_full[st], ph2))) break;
                 tmem_wait_st();
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&B.pa_ready);
 
                 // The output: scaled, converted, staged where a was (f32: and c).
-                if (!(ok = group_wait(&B.o_full[st], ph2, 1, warp == 0))) break;
-                if (p.out_f32 && !(ok = group_wait(&B.c_read[st], ph2, 1, warp == 0))) break;
+                if (!(ok = warp_wait(&B.o_full[st], ph2))) break;
+                if (p.out_f32 && !(ok = warp_wait(&B.c_read[st], ph2))) break;
                 tc_fence_after();
                 const float last_factor = gentle ? ahead : 1.f;
                 const uint64_t scale = pair(last_factor, last_factor);
@@ -821,7 +805,7 @@ la_tc(const LaCore p, const __grid_constant__ CUtensorMap ma,
         uint64_t s[32];  // pairs of its rows
 #pragma unroll 1
         for (uint32_t k = 0; ok; ++k) {
-            if (!(ok = group_wait(&B.job_full[k % kJobs], k / kJobs & 1, 2, warp == 9))) break;
+            if (!(ok = warp_wait(&B.job_full[k % kJobs], k / kJobs & 1))) break;
             const Job it = take(k % kJobs);
             if (it.len < 0) break;
             const int nch = (it.len + kC - 1) / kC;
@@ -846,7 +830,7 @@ la_tc(const LaCore p, const __grid_constant__ CUtensorMap ma,
             for (int c = 0; c < nch; ++c, ++n) {
                 if constexpr (!kStateOnly) {
                     // The bf16 copy, once the last chunk's product has read its own.
-                    if (n > 0 && !(ok = group_wait(&B.in_full[(n - 1) & 1], ((n - 1) >> 1) & 1, 2, warp == 9))) break;
+                    if (n > 0 && !(ok = warp_wait(&B.in_full[(n - 1) & 1], ((n - 1) >> 1) & 1))) break;
                     uint32_t to = sb;
                     asm volatile("" : "+r"(to));  // (eight addresses kept would be registers)
 #pragma unroll
@@ -866,7 +850,7 @@ la_tc(const LaCore p, const __grid_constant__ CUtensorMap ma,
                     lo2 = pair(f.y, f.y);
                     known = len;
                 }
-                if (!(ok = group_wait(&B.u_full[n & 1], (n >> 1) & 1, 2, warp == 9))) break;
+                if (!(ok = warp_wait(&B.u_full[n & 1], (n >> 1) & 1))) break;
                 tc_fence_after();
 #pragma unroll
                 for (int blk = 0; blk < 8; ++blk) {
@@ -910,7 +894,7 @@ la_tc(const LaCore p, const __grid_constant__ CUtensorMap ma,
         uint32_t n = 0, w = 0;
 #pragma unroll 1
         for (uint32_t k = 0; ok; ++k) {
-            if (!(ok = group_wait(&B.job_full[k % kJobs], k / kJobs & 1, 3, warp == 18))) break;
+            if (!(ok = warp_wait(&B.job_full[k % kJobs], k / kJobs & 1))) break;
             const Job it = take(k % kJobs);
             if (it.len < 0) break;
             const int nch = (it.len + kC - 1) / kC;
@@ -932,9 +916,9 @@ la_tc(const LaCore p, const __grid_constant__ CUtensorMap ma,
             for (int c = 0; c < nch; ++c, ++n) {
                 const int st = n & 1;
                 const int len = chunk_len<kRev>(it, nch, c);
-                if (!(ok = group_wait(&B.c_full[st], (n >> 1) & 1, 3, warp == 18))) break;
+                if (!(ok = warp_wait(&B.c_full[st], (n >> 1) & 1))) break;
                 if (len < kC) {
-                    if (!(ok = group_wait(&B.b_full[st], (n >> 1) & 1, 3, warp == 18))) break;
+                    if (!(ok = warp_wait(&B.b_full[st], (n >> 1) & 1))) break;
                     // The rows past the sequence hold another's (or anything):
                     // zeros, so that no product of theirs is NaN.
                     uint8_t* bt = sm + st * kStage + kTile;
@@ -1009,7 +993,7 @@ la_tc(const LaCore p, const __grid_constant__ CUtensorMap ma,
                         }
                     }
                     if (w >= kRing &&
-                        !(ok = group_wait(&B.wv_free[buf], (w / kRing & 1) ^ 1, 3, warp == 18)))
+                        !(ok = warp_wait(&B.wv_free[buf], (w / kRing & 1) ^ 1)))
                         break;
                     tc_fence_after();
                     uint32_t mid[8], lo[8];
@@ -1106,7 +1090,7 @@ cudaError_t launch_la_tc(const LaCore& p, bool split, bool must, int forced, cud
     // the same operand), and its launches and the scan some 6 chunks.
     const int sms = la_sm_count();
     LaLists lists;
-    e = la_prepare(p, sms, 1, {split, must, forced, 0.85f, 6.f}, lists, stream);
+    e = la_prepare(p, sms, 1, {split, must, forced, 0.5f, 9.f}, lists, stream);
     if (e != cudaSuccess) return e;
     if (lists.split) {
         states<<<sms, kThreads, kSmemBytes, stream>>>(p, ma, mb, mc, mo, &lists.plan->states,
