@@ -31,6 +31,7 @@ cudaError_t take_device_error(int* flag);
 cudaError_t take_layer_error(int* flag);
 cudaError_t take_rope_error(int* flag);
 cudaError_t take_la_error(int* flag);
+cudaError_t take_la_parts_error(int* flag);
 cudaError_t library_pool(cudaMemPool_t* pool, bool create);
 int conv_max_taps();
 cudaError_t launch_causal_conv1d(int dtype, int32_t n_seqs, int64_t tokens, int32_t seq_len,
@@ -685,12 +686,13 @@ gdr_status gdr_selftest_wait_timeout(int64_t limit_ns, void* stream) {
 }
 
 gdr_status gdr_device_error(void) {
-    int flag = 0, layer = 0, rope = 0, la = 0;
+    int flag = 0, layer = 0, rope = 0, la = 0, parts = 0;
     if (gdr::take_device_error(&flag) != cudaSuccess) return GDR_ERR_CUDA;
     if (gdr::take_layer_error(&layer) != cudaSuccess) return GDR_ERR_CUDA;
     if (gdr::take_rope_error(&rope) != cudaSuccess) return GDR_ERR_CUDA;
     if (gdr::take_la_error(&la) != cudaSuccess) return GDR_ERR_CUDA;
-    flag |= layer | rope | la;
+    if (gdr::take_la_parts_error(&parts) != cudaSuccess) return GDR_ERR_CUDA;
+    flag |= layer | rope | la | parts;
     if (flag & 1) return GDR_ERR_TIMEOUT;
     return (flag & 2) ? GDR_ERR_INVALID : GDR_OK;
 }

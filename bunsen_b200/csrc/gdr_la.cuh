@@ -57,8 +57,8 @@ __device__ __forceinline__ void la_span(const LaCore& p, int s, int64_t& start, 
 
 // Kernels of the core (each its own file) and what they take.
 cudaError_t launch_la_recurrent(const LaCore& p, cudaStream_t stream);
-bool la_mma_supports(const LaCore& p);
-cudaError_t launch_la_mma(const LaCore& p, cudaStream_t stream);
+bool la_parts_supports(const LaCore& p);
+cudaError_t launch_la_parts(const LaCore& p, cudaStream_t stream);
 bool la_tc_supports(const LaCore& p);
 // split: long sequences may go in segments (scratch from the library's pool);
 // must: they do even where it looks slower; forced: segment length in chunks, or 0.

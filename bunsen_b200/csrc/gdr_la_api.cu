@@ -110,8 +110,8 @@ cudaError_t run_core(const gdr_la_params& a, const LaCore& p, bool chunked, cuda
                             a.split_chunks, s);
     // Short sequences step as fast as a chunk does; the others go in chunks.
     const int64_t tokens = la_tokens(p);
-    if (la_mma_supports(p) && tokens > 4 * static_cast<int64_t>(p.n_seqs))
-        return launch_la_mma(p, s);
+    if (la_parts_supports(p) && tokens > 4 * static_cast<int64_t>(p.n_seqs))
+        return launch_la_parts(p, s);
     return launch_la_recurrent(p, s);
 }
 

@@ -1,0 +1,604 @@
+// The decayed linear attention core (gdr_la.cuh) in chunks at f32 accuracy, on the tensor
+// cores: f32 and f16 operands, and bf16 ones of widths gdr_la_tc.cu does not take;
+// d_b up to 128, d_c up to 256.
+//
+// The same sums as gdr_la_tc.cu in chunks of C = 64 positions:
+//   out_i = tau [ w^{i+1} a_i . S + sum_{j<=i} sigma w^{i-j} (a_i.b_j) c_j ]
+//   S'    = w^C S + sum_j sigma w^{C-1-j} b_j c_j^T
+// (backward in time their mirror image). Every operand goes in as bf16 parts, x = x0 +
+// x1 + x2 with 8 bits each (f16: two parts exactly, bf16: one), which keep f32's range
+// at any magnitude; of a product the parts x_i y_j with i + j <= 2 leave 2^-24 of it,
+// six products for f32. tcgen05.mma at 4096 bf16 products a cycle and SM makes that 680
+// f32 ones; three tf32 products by mma.sync make 163, FFMA 117.
+//
+// One CTA an SM takes a (sequence or segment, head) and 128 columns of the state:
+//   16 warps convert: a and b to parts in shared memory, c and the weighted c to TMEM with
+//            the columns of c on the lanes, the state's copy to shared memory; they turn
+//            scores into P, write the outputs, and hold the state, 32 values a thread
+//   1 warp   issues the products
+// The products of a chunk, N positions or rows of b on the columns of TMEM:
+//   scores = A B^T          128 x 64 (the lower 64 lanes are not read)
+//   O1^T   = S^T A^T        128 x 64, the state's copy as the first operand
+//   O2^T   = C^T P^T        128 x 64
+//   U^T    = (w C)^T B      128 x d_b
+// c never is in shared memory: a thread reads one column of it, 16 positions,
+// neighbouring lanes neighbouring columns, and that is how TMEM wants it; outputs go out
+// the same way. What the next chunk needs is read from HBM into registers while
+// the products run; a and c are converted beside the update's product, b, w c and
+// the state's copy beside the scores'.
+//
+// TMEM (512 columns): scores 64, O1 64, O2 64, U 128, c three parts of 32, w c the same.
+// Bound by the tensor cores: 5400 cycles a chunk at f32 and 128 x 128, 3.1 us.
+#include <cuda_fp16.h>
+
+#include <algorithm>
+#include <type_traits>
+
+#include "gdr_la.cuh"
+#include "gdr_la_plan.cuh"
+#include "gdr_la_sm100.cuh"
+
+namespace gdr {
+
+// As g_la_error in gdr_la_tc.cu.
+__device__ int g_la_parts_error;
+
+namespace {
+
+using namespace sm100;
+
+constexpr int kC = 64, kCols = 128;
+constexpr int kWarps = 16, kThreads = 32 * (kWarps + 4);
+constexpr uint32_t kRows64 = 64 * 128, kRows128 = 128 * 128;  // bytes of a tile 64 wide
+constexpr uint32_t kColSc = 0, kColO1 = 64, kColO2 = 128, kColU = 192, kColC = 320, kColW = 416;
+
+template <typename T, int kDb, bool kStateOnly>
+struct Layout {
+    static constexpr int kIn = sizeof(T) == 4 ? 3 : std::is_same_v<T, __half> ? 2 : 1;
+    // P and the state's copy, and the parts' products: outputs of 16 bits need 16.
+    static constexpr int kPs = sizeof(T) == 4 ? 3 : 2;
+    static constexpr int kHalves = kDb / 64;
+    static constexpr uint32_t kTileAb = kHalves * kRows64, kTileS = kHalves * kRows128;
+    static constexpr uint32_t kA = 0, kB = kA + kIn * kTileAb;
+    static constexpr uint32_t kS = kB + kIn * kTileAb;
+    static constexpr uint32_t kP = kS + (kStateOnly ? 0 : kPs * kTileS);
+    static constexpr uint32_t kMisc = kP + (kStateOnly ? 0 : kPs * kRows64);
+    static constexpr uint32_t kBytes = kMisc + 1024;
+};
+
+struct Misc {
+    float pw[kC + 8];  // w^0 .. w^kC
+    uint64_t ab_ready, s_ready, p_ready, sc_full, o_full, u_full[2], drain;
+    uint32_t tmem;
+    int next;
+};
+static_assert(sizeof(Misc) <= 1024, "its room");
+
+// Two f32 in kParts bf16 parts each.
+template <int kParts>
+__device__ __forceinline__ void split(uint64_t v, uint32_t (&out)[kParts]) {
+#pragma unroll
+    for (int i = 0; i < kParts; ++i) {
+        out[i] = pack_bf16(v);
+        if (i + 1 < kParts) v = fma2(widen(out[i]), pair(-1.f, -1.f), v);
+    }
+}
+
+// D (+)= A B over 16 kSteps of K, both K-major in shared memory in tiles 64 wide, kJump*
+// bytes apart. (Addresses step inside the assembly: four instructions a product.)
+template <int kHalves, uint32_t kJumpA, uint32_t kJumpB>
+__device__ __forceinline__ void product_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+                                           uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, t;\n\t.reg .b64 a, b;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\tsetp.eq.b32 t, 0, 0;\n\t"
+        "mov.b64 a, %1;\n\tmov.b64 b, %2;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t"
+        "add.s64 a, a, 2;\n\tadd.s64 b, b, 2;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, t;\n\t"
+        "add.s64 a, a, 2;\n\tadd.s64 b, b, 2;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, t;\n\t"
+        "add.s64 a, a, 2;\n\tadd.s64 b, b, 2;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, t;\n\t"
+        "}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+    if constexpr (kHalves == 2)
+        product_ss<1, 0, 0>(d, a + kJumpA / 16, b + kJumpB / 16, idesc, 1);
+}
+// D (+)= A B over 64 of K: A in TMEM, B's steps kStep bytes apart.
+template <uint32_t kStep>
+__device__ __forceinline__ void product_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc,
+                                           uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, t;\n\t.reg .b32 a;\n\t.reg .b64 b;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\tsetp.eq.b32 t, 0, 0;\n\tmov.b32 a, %1;\n\tmov.b64 b, %2;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [a], b, %3, p;\n\t"
+        "add.u32 a, a, 8;\n\tadd.s64 b, b, %5;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [a], b, %3, t;\n\t"
+        "add.u32 a, a, 8;\n\tadd.s64 b, b, %5;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [a], b, %3, t;\n\t"
+        "add.u32 a, a, 8;\n\tadd.s64 b, b, %5;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [a], b, %3, t;\n\t"
+        "}" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(accumulate), "n"(kStep / 16)
+        : "memory");
+}
+// The parts (i, j) of a product with i + j <= kOrder, the smallest first.
+template <int kX, int kY, int kOrder, typename F>
+__device__ __forceinline__ void each_part(F&& f) {
+    bool first = true;
+#pragma unroll
+    for (int o = kOrder; o >= 0; --o)
+#pragma unroll
+        for (int i = 0; i <= o; ++i)
+            if (i < kX && o - i < kY) {
+                f(i, o - i, first ? 0u : 1u);
+                first = false;
+            }
+}
+
+// Eight neighbours of a row, as read.
+template <typename T>
+struct Eight {
+    T v[8];
+};
+template <typename T>
+__device__ __forceinline__ Eight<T> load8(const T* at, int left, bool vec) {
+    Eight<T> e{};
+    if (left <= 0) return e;
+    if (vec) {  // (d is a multiple of 8 then, and rows begin on 16 bytes)
+        constexpr int kV = sizeof(Eight<T>) / 16;
+#pragma unroll
+        for (int i = 0; i < kV; ++i)
+            reinterpret_cast<uint4*>(e.v)[i] = reinterpret_cast<const uint4*>(at)[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i < left) e.v[i] = at[i];
+    }
+    return e;
+}
+
+template <typename T, int kDb, bool kRev, bool kStateOnly>
+__global__ void __launch_bounds__(kThreads, 1)
+la_parts(const LaCore p, LaWork* work, const LaEntry* entries, float* scratch, bool vec) {
+    using L = Layout<T, kDb, kStateOnly>;
+    constexpr int kIn = L::kIn, kPs = L::kPs, kOrder = kPs - 1, kHalves = L::kHalves;
+    constexpr int kEights = kC * kDb / 8 / (32 * kWarps);  // of a and of b, a thread
+    constexpr int kMine = kDb / 4;                         // the state's rows of a thread
+    extern __shared__ __align__(1024) uint8_t sm[];
+    Misc& M = *reinterpret_cast<Misc*>(sm + L::kMisc);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    if (tid == 0) {
+        mbar_init(&M.ab_ready, kWarps);
+        mbar_init(&M.s_ready, kWarps);
+        mbar_init(&M.p_ready, kWarps / 2);
+        mbar_init(&M.sc_full, 1);
+        mbar_init(&M.o_full, 1);
+        mbar_init(&M.u_full[0], 1);
+        mbar_init(&M.u_full[1], 1);
+        mbar_init(&M.drain, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == kWarps) {
+        tmem_alloc(&M.tmem, 512);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    bool ok = M.tmem == 0 && (smem_u32(sm) & 1023) == 0;  // (all columns: they begin at 0)
+    const int blocks = (p.d_c + kCols - 1) / kCols;
+    const int jobs = (work != nullptr ? work->count : p.n_seqs) * p.heads * blocks;
+    const int quarter = warp & 3, part = warp >> 2;
+    const uint32_t quad = static_cast<uint32_t>(quarter) << 21;  // this warp's lanes
+    uint32_t n = 0;                                              // chunks before
+    // The jobs, one after the other: body(entry, head, first column, chunks).
+    auto each_job = [&](auto&& body) {
+        int id = blockIdx.x;
+#pragma unroll 1
+        while (id < jobs) {
+            const int e = id / blocks / p.heads;
+            LaEntry it;
+            if (work != nullptr) {
+                it = entries[e];
+            } else {
+                int64_t start, end;
+                la_span(p, e, start, end);
+                it = {static_cast<int32_t>(start), static_cast<int32_t>(end - start), e, e};
+            }
+            const int nch = (it.len + kC - 1) / kC;
+            body(it, id / blocks % p.heads, id % blocks * kCols, nch);
+            n += nch;
+            if (tid == 0) M.next = work != nullptr ? atomicAdd(&work->next, 1) : jobs;
+            if (!__syncthreads_and(ok)) break;
+            id = M.next;
+            __syncthreads();
+        }
+    };
+    // The launch gives each thread 96 registers, 480 for the five warpgroups' lanes together:
+    // 4 x 112 + 32.
+    if (warp >= kWarps) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 32;");
+        each_job([&](const LaEntry& it, int, int, int nch) {
+            // ---- the products ------------------------------------------------------
+            constexpr uint32_t kKK = idesc_bf16(128, kC, 0, 0, 0);
+            constexpr uint32_t kKMn = idesc_bf16(128, kDb, 0, 1, 0);
+            const uint32_t base = smem_u32(sm);
+            auto update = [&](uint32_t b_at, uint32_t w_at, uint32_t u_at) {
+                each_part<3, kIn, 2>([&](int i, int j, uint32_t acc) {
+                    product_ts<2048>(u_at, w_at + 32 * i,
+                                     sdesc_sw128(b_at + j * L::kTileAb, kRows64, 1024), kKMn, acc);
+                });
+            };
+            __syncthreads();  // (the converting warps' one at a job's start)
+#pragma unroll 1
+            for (int c = 0; warp == kWarps && ok && c < nch; ++c) {
+                const uint32_t ph = (n + c) & 1;
+                if (!(ok = warp_wait(&M.ab_ready, ph))) break;
+                tc_fence_after();
+                if constexpr (kStateOnly) {
+                    if (elect_one()) {
+                        update(base + ph * L::kB, kColC + 96 * ph, 128 * ph);
+                        umma_commit(&M.u_full[ph]);
+                    }
+                } else {
+                    if (elect_one()) {
+                        each_part<kIn, kIn, kOrder>([&](int i, int j, uint32_t acc) {
+                            product_ss<kHalves, kRows64, kRows64>(
+                                kColSc, sdesc_sw128(base + L::kA + i * L::kTileAb, 16, 1024),
+                                sdesc_sw128(base + L::kB + j * L::kTileAb, 16, 1024), kKK, acc);
+                        });
+                        umma_commit(&M.sc_full);
+                    }
+                    if (!(ok = warp_wait(&M.s_ready, ph))) break;
+                    tc_fence_after();
+                    if (elect_one())
+                        each_part<kPs, kIn, kOrder>([&](int i, int j, uint32_t acc) {
+                            product_ss<kHalves, kRows128, kRows64>(
+                                kColO1, sdesc_sw128(base + L::kS + i * L::kTileS, 16, 1024),
+                                sdesc_sw128(base + L::kA + j * L::kTileAb, 16, 1024), kKK, acc);
+                        });
+                    if (!(ok = warp_wait(&M.p_ready, ph))) break;
+                    tc_fence_after();
+                    if (elect_one()) {
+                        each_part<kIn, kPs, kOrder>([&](int i, int j, uint32_t acc) {
+                            product_ts<32>(kColO2, kColC + 32 * i,
+                                           sdesc_sw128(base + L::kP + j * kRows64, 16, 1024), kKK,
+                                           acc);
+                        });
+                        umma_commit(&M.o_full);
+                        update(base + L::kB, kColW, kColU);
+                        umma_commit(&M.u_full[0]);
+                    }
+                }
+            }
+        });
+        if (warp == kWarps) {  // nothing of this CTA's may be in flight when it ends
+            if (elect_one()) umma_commit(&M.drain);
+            warp_wait(&M.drain, 0);
+        }
+        __syncwarp();
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 112;");
+        each_job([&](const LaEntry& it, int h, int n0, int nch) {
+            // ---- conversions, outputs, the state -----------------------------------------
+            const int col = 32 * quarter + lane;  // this thread's column of c, of 128
+            const bool mine = n0 + col < p.d_c;
+            const int ha = h / (p.heads / p.heads_a), hb = h / (p.heads / p.heads_b),
+                      hc = h / (p.heads / p.heads_c);
+            Eight<T> va[kEights], vb[kEights];
+            T vc[16];  // positions 16 part .. + 15
+            auto fetch = [&](int c, bool first, bool second) {  // a and c, b
+                const int x = kRev ? nch - 1 - c : c;
+                const int64_t row = static_cast<int64_t>(it.start) + x * kC;
+                const int len = min(kC, it.len - x * kC);
+#pragma unroll
+                for (int i = 0; i < kEights; ++i) {
+                    const int at = tid + 32 * kWarps * i, r = at / (kDb / 8), d = at % (kDb / 8) * 8;
+                    const int left = r < len ? p.d_b - d : 0;
+                    if (!kStateOnly && first)
+                        va[i] = load8(static_cast<const T*>(p.a) +
+                                          ((row + r) * p.heads_a + ha) * p.d_b + d, left, vec);
+                    if (second)
+                        vb[i] = load8(static_cast<const T*>(p.b) +
+                                          ((row + r) * p.heads_b + hb) * p.d_b + d, left, vec);
+                }
+                if (!first) return;
+                const int64_t step = static_cast<int64_t>(p.heads_c) * p.d_c;
+                const T* src = static_cast<const T*>(p.c) + (row * p.heads_c + hc) * p.d_c + n0 +
+                               col + 16 * part * step;
+                const int live = mine ? len - 16 * part : 0;
+#pragma unroll
+                for (int j = 0; j < 16; ++j, src += step) vc[j] = j < live ? *src : T(0.f);
+            };
+            // Parts of a or b: rows of 128 bytes, 16 of them exchanged by the row's number.
+            auto put = [&](uint32_t at, const Eight<T>(&v)[kEights]) {
+#pragma unroll
+                for (int i = 0; i < kEights; ++i) {
+                    const int x = tid + 32 * kWarps * i, r = x / (kDb / 8), d = x % (kDb / 8);
+                    uint32_t q[4][kIn];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        split<kIn>(pair(to_f32(v[i].v[2 * j]), to_f32(v[i].v[2 * j + 1])), q[j]);
+                    uint8_t* dst = sm + at + (d >> 3) * kRows64 + r * 128 + (((d ^ r) & 7) << 4);
+#pragma unroll
+                    for (int k = 0; k < kIn; ++k)
+                        *reinterpret_cast<uint4*>(dst + k * L::kTileAb) =
+                            make_uint4(q[0][k], q[1][k], q[2][k], q[3][k]);
+                }
+            };
+            auto put_c = [&]() {
+                uint32_t q[8][kIn];
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    split<kIn>(pair(to_f32(vc[2 * j]), to_f32(vc[2 * j + 1])), q[j]);
+#pragma unroll
+                for (int k = 0; k < kIn; ++k) {
+                    uint32_t r[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) r[j] = q[j][k];
+                    tmem_st8(quad + kColC + 32 * k + 8 * part, r);
+                }
+            };
+            auto put_w = [&](uint32_t at, int len) {  // sigma w^{len-1-j} c_j, or w^{j+1}
+                uint32_t q[8][3];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int x = 16 * part + 2 * j;
+                    const float w0 = p.sigma * M.pw[kRev ? x + 1 : max(len - 1 - x, 0)];
+                    const float w1 = p.sigma * M.pw[kRev ? x + 2 : max(len - 2 - x, 0)];
+                    split<3>(mul2(pair(to_f32(vc[2 * j]), to_f32(vc[2 * j + 1])), pair(w0, w1)), q[j]);
+                }
+#pragma unroll
+                for (int k = 0; k < 3; ++k) {
+                    uint32_t r[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) r[j] = q[j][k];
+                    tmem_st8(quad + at + 32 * k + 8 * part, r);
+                }
+            };
+            auto arrive = [&](uint64_t* bar) {  // all of this warp's writes before
+                tmem_wait_st();
+                tc_fence_before();
+                fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar);
+            };
+            if (nch > 0) fetch(0, true, true);
+            const float decay = p.log_decay[h];
+            if (tid <= kC) M.pw[tid] = la_power(decay, tid);
+            uint64_t s[kMine / 2];  // rows kMine part .. of the state, pairs
+            const LaState in = la_state(p, it.in, h, p.state_in, scratch);
+            {
+                const int b0 = kMine * part;
+                const float* src = in.ptr + (n0 + col) * in.col + b0 * in.row;
+                const bool any = in.ptr != nullptr && mine;
+#pragma unroll
+                for (int j = 0; j < kMine / 2; ++j, src += 2 * in.row)
+                    s[j] = pair(any && b0 + 2 * j < p.d_b ? src[0] : 0.f,
+                                any && b0 + 2 * j + 1 < p.d_b ? src[in.row] : 0.f);
+            }
+            __syncthreads();  // the powers
+            uint64_t hi2 = 0, lo2 = 0;  // w^len of a chunk, in two parts
+            int known = 0;
+            auto add_update = [&](uint32_t at) {
+#pragma unroll
+                for (int blk = 0; blk < kMine / 8; ++blk) {
+                    uint64_t u[4];
+                    tmem_ld8(quad + at + kMine * part + 8 * blk, u);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        s[4 * blk + j] = fma2(s[4 * blk + j], hi2, fma2(s[4 * blk + j], lo2, u[j]));
+                }
+                tc_fence_before();  // (before this warp's next arrival)
+            };
+            auto len_of = [&](int c) { return min(kC, it.len - (kRev ? nch - 1 - c : c) * kC); };
+            auto decay_of = [&](int len) {
+                if (len == known) return;
+                const float2 f = la_power2(decay, len);
+                hi2 = pair(f.x, f.x), lo2 = pair(f.y, f.y);
+                known = len;
+            };
+            if constexpr (kStateOnly) {
+                // The conversions of a chunk run beside the product of the one before.
+#pragma unroll 1
+                for (int c = 0; c < nch; ++c) {
+                    const uint32_t ph = (n + c) & 1;
+                    put(ph * L::kB, vb);
+                    put_w(kColC + 96 * ph, len_of(c));
+                    arrive(&M.ab_ready);
+                    if (c + 1 < nch) fetch(c + 1, true, true);
+                    if (c > 0) {
+                        if (!(ok = warp_wait(&M.u_full[ph ^ 1], ((n + c - 1) >> 1) & 1))) break;
+                        tc_fence_after();
+                        decay_of(len_of(c - 1));
+                        add_update(128 * (ph ^ 1));
+                    }
+                }
+                if (ok && nch > 0) {
+                    const uint32_t m = n + nch - 1;
+                    if ((ok = warp_wait(&M.u_full[m & 1], (m >> 1) & 1))) {
+                        tc_fence_after();
+                        decay_of(len_of(nch - 1));
+                        add_update(128 * (m & 1));
+                    }
+                }
+            } else {
+                if (nch > 0) {
+                    put(L::kA, va);
+                    put_c();
+                }
+#pragma unroll 1
+                for (int c = 0; c < nch; ++c) {
+                    const uint32_t ph = (n + c) & 1;
+                    const int x = kRev ? nch - 1 - c : c, len = len_of(c);
+                    put(L::kB, vb);
+                    arrive(&M.ab_ready);
+                    put_w(kColW, len);
+                    {
+                        const uint32_t row = L::kS + (kMine * part >> 6) * kRows128 + col * 128;
+                        const int first = kMine * part / 8;
+#pragma unroll
+                        for (int m = 0; m < kMine / 8; ++m) {
+                            uint32_t q[4][kPs];
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) split<kPs>(s[4 * m + j], q[j]);
+                            uint8_t* dst = sm + row + (((first + m) ^ col) & 7) * 16;
+#pragma unroll
+                            for (int k = 0; k < kPs; ++k)
+                                *reinterpret_cast<uint4*>(dst + k * L::kTileS) =
+                                    make_uint4(q[0][k], q[1][k], q[2][k], q[3][k]);
+                        }
+                    }
+                    arrive(&M.s_ready);
+                    if (c + 1 < nch) fetch(c + 1, true, false);
+                    if (quarter < 2) {
+                        // P: row i, 16 columns; what the mask leaves, decayed.
+                        const int i = 32 * quarter + lane;
+                        if (!(ok = warp_wait(&M.sc_full, ph))) break;
+                        tc_fence_after();
+#pragma unroll
+                        for (int m = 0; m < 2; ++m) {
+                            const int j0 = 16 * part + 8 * m;
+                            uint64_t u[4];
+                            tmem_ld8(quad + kColSc + j0, u);
+                            uint32_t q[4][kPs];
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                const int e0 = kRev ? j0 + 2 * j - i : i - j0 - 2 * j;
+                                const int e1 = kRev ? e0 + 1 : e0 - 1;
+                                float f0, f1;
+                                unpair(u[j], f0, f1);
+                                f0 = e0 >= 0 ? f0 * (p.sigma * M.pw[e0]) : 0.f;
+                                f1 = e1 >= 0 ? f1 * (p.sigma * M.pw[e1]) : 0.f;
+                                split<kPs>(pair(f0, f1), q[j]);
+                            }
+                            uint8_t* dst = sm + L::kP + i * 128 + (((j0 >> 3) ^ i) & 7) * 16;
+#pragma unroll
+                            for (int k = 0; k < kPs; ++k)
+                                *reinterpret_cast<uint4*>(dst + k * kRows64) =
+                                    make_uint4(q[0][k], q[1][k], q[2][k], q[3][k]);
+                        }
+                        arrive(&M.p_ready);
+                    }
+                    if (!(ok = warp_wait(&M.o_full, ph))) break;
+                    tc_fence_after();
+                    {
+                        const int64_t step = static_cast<int64_t>(p.heads) * p.d_c;
+                        int64_t at = (static_cast<int64_t>(it.start) + x * kC + 16 * part) * step +
+                                     static_cast<int64_t>(h) * p.d_c + n0 + col;
+                        const int live = mine ? len - 16 * part : 0;
+#pragma unroll
+                        for (int m = 0; m < 2; ++m) {
+                            uint64_t u[4], v[4];
+                            tmem_ld8(quad + kColO1 + 16 * part + 8 * m, u);
+                            tmem_ld8(quad + kColO2 + 16 * part + 8 * m, v);
+#pragma unroll
+                            for (int j = 0; j < 8; ++j, at += step) {
+                                const int i = 16 * part + 8 * m + j;
+                                float f[2], g[2];
+                                unpair(u[j >> 1], f[0], f[1]);
+                                unpair(v[j >> 1], g[0], g[1]);
+                                const float y =
+                                    p.tau * fmaf(M.pw[kRev ? max(len - 1 - i, 0) : i + 1], f[j & 1],
+                                                 g[j & 1]);
+                                if (8 * m + j < live) {
+                                    if (p.out_f32) static_cast<float*>(p.out)[at] = y;
+                                    else static_cast<T*>(p.out)[at] = from_f32<T>(y);
+                                }
+                            }
+                        }
+                    }
+                    if (c + 1 < nch) {
+                        fetch(c + 1, false, true);
+                        put(L::kA, va);
+                        put_c();
+                    }
+                    decay_of(len);
+                    if (!(ok = warp_wait(&M.u_full[0], ph))) break;
+                    tc_fence_after();
+                    add_update(kColU);
+                }
+            }
+            const LaState out = la_state(p, it.out, h, p.state_out, scratch);
+            if (ok && out.ptr != nullptr && mine) {
+                const int b0 = kMine * part;
+                float* dst = const_cast<float*>(out.ptr) + (n0 + col) * out.col + b0 * out.row;
+#pragma unroll
+                for (int j = 0; j < kMine / 2; ++j, dst += 2 * out.row) {
+                    float f[2];
+                    unpair(s[j], f[0], f[1]);
+                    if (b0 + 2 * j < p.d_b) dst[0] = f[0];
+                    if (b0 + 2 * j + 1 < p.d_b) dst[out.row] = f[1];
+                }
+            }
+        });
+    }
+    if (!ok && lane == 0) atomicOr(&g_la_parts_error, 1);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == kWarps) tmem_dealloc(M.tmem, 512);
+}
+
+template <typename T, int kDb, bool kRev>
+cudaError_t start(const LaCore& p, cudaStream_t stream) {
+    auto* full = la_parts<T, kDb, kRev, false>;
+    auto* states = la_parts<T, kDb, kRev, true>;
+    constexpr int kFull = static_cast<int>(Layout<T, kDb, false>::kBytes),
+                  kStates = static_cast<int>(Layout<T, kDb, true>::kBytes);
+    cudaError_t e = cudaFuncSetAttribute(full, cudaFuncAttributeMaxDynamicSharedMemorySize, kFull);
+    if (e == cudaSuccess)
+        e = cudaFuncSetAttribute(states, cudaFuncAttributeMaxDynamicSharedMemorySize, kStates);
+    if (e != cudaSuccess) return e;
+    const bool vec = p.d_b % 8 == 0 && ((reinterpret_cast<uintptr_t>(p.a) |
+                                         reinterpret_cast<uintptr_t>(p.b)) & 15) == 0;
+    const int grid = la_sm_count(), blocks = (p.d_c + kCols - 1) / kCols;
+    LaLists lists;
+    if ((e = la_prepare(p, grid, blocks, {true, false, 0, 0.3f, 3.f}, lists, stream)) != cudaSuccess)
+        return e;
+    if (lists.split) {
+        states<<<grid, kThreads, kStates, stream>>>(p, &lists.plan->states, lists.states,
+                                                    lists.slots, vec);
+        la_scan_states(p, lists, stream);
+    }
+    const int64_t jobs = static_cast<int64_t>(p.n_seqs) * p.heads * blocks;
+    full<<<lists.plan != nullptr ? grid : static_cast<int>(jobs), kThreads, kFull, stream>>>(
+        p, lists.plan != nullptr ? &lists.plan->main : nullptr, lists.main, lists.slots, vec);
+    e = cudaGetLastError();
+    const cudaError_t f = la_release(lists, stream);
+    return e != cudaSuccess ? e : f;
+}
+
+template <typename T>
+cudaError_t pick(const LaCore& p, cudaStream_t stream) {
+    if (p.d_b <= 64)
+        return p.reverse ? start<T, 64, true>(p, stream) : start<T, 64, false>(p, stream);
+    return p.reverse ? start<T, 128, true>(p, stream) : start<T, 128, false>(p, stream);
+}
+
+}  // namespace
+
+bool la_parts_supports(const LaCore& p) {
+    return p.d_b <= 128 && p.d_c <= kLaMaxD && la_tokens(p) < (int64_t{1} << 31) - 2 * kLaChunk &&
+           static_cast<int64_t>(p.n_seqs) * p.heads < (int64_t{1} << 28);
+}
+
+cudaError_t launch_la_parts(const LaCore& p, cudaStream_t stream) {
+    switch (p.dtype) {
+        case GDR_DTYPE_BF16: return pick<__nv_bfloat16>(p, stream);
+        case GDR_DTYPE_F16: return pick<__half>(p, stream);
+        default: return pick<float>(p, stream);
+    }
+}
+
+cudaError_t take_la_parts_error(int* flag) {
+    cudaError_t e = cudaMemcpyFromSymbol(flag, g_la_parts_error, sizeof(int));
+    if (e != cudaSuccess || *flag == 0) return e;
+    const int zero = 0;
+    return cudaMemcpyToSymbol(g_la_parts_error, &zero, sizeof(int));
+}
+
+}  // namespace gdr
