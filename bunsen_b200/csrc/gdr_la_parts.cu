@@ -63,24 +63,39 @@ struct Layout {
     static constexpr uint32_t kS = kB + kIn * kTileAb;
     static constexpr uint32_t kP = kS + (kStateOnly ? 0 : kPs * kTileS);
     static constexpr uint32_t kMisc = kP + (kStateOnly ? 0 : kPs * kRows64);
-    static constexpr uint32_t kBytes = kMisc + 1024;
+    static constexpr uint32_t kBytes = kMisc + 2048;
 };
 
 struct Misc {
-    float pw[kC + 8];  // w^0 .. w^kC
+    // Powers for a job's whole chunks, and for its short one:
+    alignas(16) float wt[2][kC];     // sigma w^{len-1-j}, the weights of c (backward w^{j+1})
+    alignas(16) float ahead[2][kC];  // tau w^{i+1}, of a_i . S (backward w^{len-1-i})
+    float2 f[2];                     // w^len, in two parts
+    float decay[kC];                 // sigma w^0 .. w^{kC-1}
     uint64_t ab_ready, s_ready, p_ready, sc_full, o_full, u_full[2], drain;
     uint32_t tmem;
     int next;
 };
-static_assert(sizeof(Misc) <= 1024, "its room");
+static_assert(sizeof(Misc) <= 2048, "its room");
 
-// Two f32 in kParts bf16 parts each.
-template <int kParts>
-__device__ __forceinline__ void split(uint64_t v, uint32_t (&out)[kParts]) {
+// 2 kN values in kParts bf16 parts each, put(k, part k of the pairs) part by part.
+// (Volatile: kN chains at once and no more, or the registers run out. Scalar
+// differences: pairs of f32 took more moves and registers than they saved.)
+template <int kParts, int kN, typename F>
+__device__ __forceinline__ void split(float (&v)[kN], F&& put) {
 #pragma unroll
-    for (int i = 0; i < kParts; ++i) {
-        out[i] = pack_bf16(v);
-        if (i + 1 < kParts) v = fma2(widen(out[i]), pair(-1.f, -1.f), v);
+    for (int k = 0; k < kParts; ++k) {
+        uint32_t r[kN / 2];
+#pragma unroll
+        for (int j = 0; j < kN / 2; ++j)
+            asm volatile("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r[j]) : "f"(v[2 * j + 1]), "f"(v[2 * j]));
+        put(k, r);
+        if (k + 1 < kParts)
+#pragma unroll
+            for (int j = 0; j < kN / 2; ++j) {
+                v[2 * j] -= low_f32(r[j]);
+                v[2 * j + 1] -= high_f32(r[j]);
+            }
     }
 }
 
@@ -138,6 +153,20 @@ __device__ __forceinline__ void each_part(F&& f) {
             }
 }
 
+// x, unknown to the compiler: what follows from it is computed where it is used and not
+// kept in registers over the chunks (as hoisted addresses it spilled).
+__device__ __forceinline__ int here(int x) {
+    asm volatile("" : "+r"(x));
+    return x;
+}
+
+// (Volatile: in the order written, so that one store's values at a time are in registers.)
+__device__ __forceinline__ void st_shared(uint32_t at, uint32_t x, uint32_t y, uint32_t z,
+                                          uint32_t w) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(x), "r"(y), "r"(z), "r"(w)
+                 : "memory");
+}
+
 // Eight neighbours of a row, as read.
 template <typename T>
 struct Eight {
@@ -159,6 +188,11 @@ __device__ __forceinline__ Eight<T> load8(const T* at, int left, bool vec) {
     }
     return e;
 }
+
+template <typename T, int kN>
+struct Operand {
+    Eight<T> v[kN];
+};
 
 template <typename T, int kDb, bool kRev, bool kStateOnly>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -192,6 +226,7 @@ la_parts(const LaCore p, LaWork* work, const LaEntry* entries, float* scratch, b
     const int blocks = (p.d_c + kCols - 1) / kCols;
     const int jobs = (work != nullptr ? work->count : p.n_seqs) * p.heads * blocks;
     const int quarter = warp & 3, part = warp >> 2;
+    const uint32_t base = smem_u32(sm);
     const uint32_t quad = static_cast<uint32_t>(quarter) << 21;  // this warp's lanes
     uint32_t n = 0;                                              // chunks before
     // The jobs, one after the other: body(entry, head, first column, chunks).
@@ -225,7 +260,6 @@ la_parts(const LaCore p, LaWork* work, const LaEntry* entries, float* scratch, b
             // ---- the products ------------------------------------------------------
             constexpr uint32_t kKK = idesc_bf16(128, kC, 0, 0, 0);
             constexpr uint32_t kKMn = idesc_bf16(128, kDb, 0, 1, 0);
-            const uint32_t base = smem_u32(sm);
             auto update = [&](uint32_t b_at, uint32_t w_at, uint32_t u_at) {
                 each_part<3, kIn, 2>([&](int i, int j, uint32_t acc) {
                     product_ts<2048>(u_at, w_at + 32 * i,
@@ -235,7 +269,7 @@ la_parts(const LaCore p, LaWork* work, const LaEntry* entries, float* scratch, b
             __syncthreads();  // (the converting warps' one at a job's start)
 #pragma unroll 1
             for (int c = 0; warp == kWarps && ok && c < nch; ++c) {
-                const uint32_t ph = (n + c) & 1;
+                const uint32_t ph = (n + c) & 1, base = here(smem_u32(sm));
                 if (!(ok = warp_wait(&M.ab_ready, ph))) break;
                 tc_fence_after();
                 if constexpr (kStateOnly) {
@@ -288,76 +322,101 @@ la_parts(const LaCore p, LaWork* work, const LaEntry* entries, float* scratch, b
             const bool mine = n0 + col < p.d_c;
             const int ha = h / (p.heads / p.heads_a), hb = h / (p.heads / p.heads_b),
                       hc = h / (p.heads / p.heads_c);
-            Eight<T> va[kEights], vb[kEights];
-            T vc[16];  // positions 16 part .. + 15
-            auto fetch = [&](int c, bool first, bool second) {  // a and c, b
+            // Operands on their way. (Fetched after the last chunk too, as zeros: behind
+            // conditions they took more registers.)
+            using Ab = Operand<T, kEights>;
+            using Column = Operand<T, 2>;
+            auto chunk_at = [&](int c, int64_t& row, int& len) {
                 const int x = kRev ? nch - 1 - c : c;
-                const int64_t row = static_cast<int64_t>(it.start) + x * kC;
-                const int len = min(kC, it.len - x * kC);
+                row = static_cast<int64_t>(it.start) + x * kC;
+                len = c < nch ? min(kC, it.len - x * kC) : 0;  // (after the last chunk: nothing)
+            };
+            auto fetch = [&](const void* base, int heads, int head, int c) {
+                Ab o;
+                int64_t row;
+                int len;
+                chunk_at(c, row, len);
+                const int tid = here(threadIdx.x), step = heads * p.d_b;
+                const T* src = static_cast<const T*>(base) + (row * heads + head) * p.d_b;
 #pragma unroll
                 for (int i = 0; i < kEights; ++i) {
                     const int at = tid + 32 * kWarps * i, r = at / (kDb / 8), d = at % (kDb / 8) * 8;
-                    const int left = r < len ? p.d_b - d : 0;
-                    if (!kStateOnly && first)
-                        va[i] = load8(static_cast<const T*>(p.a) +
-                                          ((row + r) * p.heads_a + ha) * p.d_b + d, left, vec);
-                    if (second)
-                        vb[i] = load8(static_cast<const T*>(p.b) +
-                                          ((row + r) * p.heads_b + hb) * p.d_b + d, left, vec);
+                    o.v[i] = load8(src + (r * step + d), r < len ? p.d_b - d : 0, here(vec));
                 }
-                if (!first) return;
-                const int64_t step = static_cast<int64_t>(p.heads_c) * p.d_c;
+                return o;
+            };
+            auto fetch_c = [&](int c) {
+                Column o;
+                int64_t row;
+                int len;
+                chunk_at(c, row, len);
+                const int step = p.heads_c * p.d_c;  // (64 of them are below 2^31)
                 const T* src = static_cast<const T*>(p.c) + (row * p.heads_c + hc) * p.d_c + n0 +
-                               col + 16 * part * step;
+                               32 * quarter + here(lane) + 16 * part * step;
                 const int live = mine ? len - 16 * part : 0;
 #pragma unroll
-                for (int j = 0; j < 16; ++j, src += step) vc[j] = j < live ? *src : T(0.f);
+                for (int j = 0; j < 16; ++j)
+                    o.v[j >> 3].v[j & 7] = j < live ? src[j * step] : T(0.f);
+                return o;
+            };
+            // The lines of a chunk to L2: its loads come when registers are free for them.
+            auto prefetch = [&](int c) {
+                int64_t row;
+                int len;
+                chunk_at(c, row, len);
+                const int tid = here(threadIdx.x), r = tid >> 3, x = (tid & 3) * 128 / static_cast<int>(sizeof(T));
+                if (r >= len) return;
+                auto line = [&](const void* base, int heads, int head, int d, int at) {
+                    if (at < d)
+                        asm volatile("prefetch.global.L2 [%0];" ::"l"(
+                            static_cast<const T*>(base) + ((row + r) * heads + head) * d + at));
+                };
+                if (tid & 4) {
+                    line(p.b, p.heads_b, hb, p.d_b, x);
+                } else {
+                    if (!kStateOnly) line(p.a, p.heads_a, ha, p.d_b, x);
+                    line(p.c, p.heads_c, hc, p.d_c, n0 + x);
+                }
             };
             // Parts of a or b: rows of 128 bytes, 16 of them exchanged by the row's number.
-            auto put = [&](uint32_t at, const Eight<T>(&v)[kEights]) {
+            auto put = [&](uint32_t at, const Ab& from) {
+                const int tid = here(threadIdx.x);
 #pragma unroll
                 for (int i = 0; i < kEights; ++i) {
                     const int x = tid + 32 * kWarps * i, r = x / (kDb / 8), d = x % (kDb / 8);
-                    uint32_t q[4][kIn];
+                    float v[8];
 #pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        split<kIn>(pair(to_f32(v[i].v[2 * j]), to_f32(v[i].v[2 * j + 1])), q[j]);
-                    uint8_t* dst = sm + at + (d >> 3) * kRows64 + r * 128 + (((d ^ r) & 7) << 4);
-#pragma unroll
-                    for (int k = 0; k < kIn; ++k)
-                        *reinterpret_cast<uint4*>(dst + k * L::kTileAb) =
-                            make_uint4(q[0][k], q[1][k], q[2][k], q[3][k]);
+                    for (int j = 0; j < 8; ++j) v[j] = to_f32(from.v[i].v[j]);
+                    const uint32_t dst = base + at + (d >> 3) * kRows64 + r * 128 + (((d ^ r) & 7) << 4);
+                    split<kIn>(v, [&](int k, const uint32_t(&r)[4]) {
+                        st_shared(dst + k * L::kTileAb, r[0], r[1], r[2], r[3]);
+                    });
                 }
             };
-            auto put_c = [&]() {
-                uint32_t q[8][kIn];
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    split<kIn>(pair(to_f32(vc[2 * j]), to_f32(vc[2 * j + 1])), q[j]);
-#pragma unroll
-                for (int k = 0; k < kIn; ++k) {
-                    uint32_t r[8];
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) r[j] = q[j][k];
-                    tmem_st8(quad + kColC + 32 * k + 8 * part, r);
-                }
-            };
-            auto put_w = [&](uint32_t at, int len) {  // sigma w^{len-1-j} c_j, or w^{j+1}
-                uint32_t q[8][3];
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const int x = 16 * part + 2 * j;
-                    const float w0 = p.sigma * M.pw[kRev ? x + 1 : max(len - 1 - x, 0)];
-                    const float w1 = p.sigma * M.pw[kRev ? x + 2 : max(len - 2 - x, 0)];
-                    split<3>(mul2(pair(to_f32(vc[2 * j]), to_f32(vc[2 * j + 1])), pair(w0, w1)), q[j]);
-                }
-#pragma unroll
-                for (int k = 0; k < 3; ++k) {
-                    uint32_t r[8];
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) r[j] = q[j][k];
+            // Eight pairs of this thread's column of c.
+            auto put_column = [&](uint32_t at, float(&v)[16], auto parts) {
+                split<decltype(parts)::value>(v, [&](int k, const uint32_t(&r)[8]) {
                     tmem_st8(quad + at + 32 * k + 8 * part, r);
+                });
+            };
+            auto put_c = [&](const Column& vc) {
+                float v[16];
+#pragma unroll
+                for (int j = 0; j < 16; ++j) v[j] = to_f32(vc.v[j >> 3].v[j & 7]);
+                put_column(kColC, v, std::integral_constant<int, kIn>{});
+            };
+            auto put_w = [&](uint32_t at, int len, const Column& vc) {
+                float v[16];
+                const float4* w = reinterpret_cast<const float4*>(&M.wt[len < kC][16 * part]);
+#pragma unroll
+                for (int j = 0; j < 16; j += 4) {
+                    const float4 f = w[j >> 2];
+                    v[j] = to_f32(vc.v[j >> 3].v[j & 7]) * f.x;
+                    v[j + 1] = to_f32(vc.v[j >> 3].v[(j & 7) + 1]) * f.y;
+                    v[j + 2] = to_f32(vc.v[j >> 3].v[(j & 7) + 2]) * f.z;
+                    v[j + 3] = to_f32(vc.v[j >> 3].v[(j & 7) + 3]) * f.w;
                 }
+                put_column(at, v, std::integral_constant<int, 3>{});
             };
             auto arrive = [&](uint64_t* bar) {  // all of this warp's writes before
                 tmem_wait_st();
@@ -366,9 +425,24 @@ la_parts(const LaCore p, LaWork* work, const LaEntry* entries, float* scratch, b
                 __syncwarp();
                 if (lane == 0) mbar_arrive(bar);
             };
-            if (nch > 0) fetch(0, true, true);
+            Ab va;
+            if (!kStateOnly) va = fetch(p.a, p.heads_a, ha, 0);
+            Ab vb = fetch(p.b, p.heads_b, hb, 0);
+            Column vc = fetch_c(0);  // positions 16 part .. + 15 of this thread's column
             const float decay = p.log_decay[h];
-            if (tid <= kC) M.pw[tid] = la_power(decay, tid);
+            {
+                const int len = tid < 4 * kC / 2 || it.len % kC == 0 ? kC : it.len % kC;
+                const int j = tid % kC, up = j + 1, down = max(len - 1 - j, 0);
+                if (tid < 4 * kC) {
+                    const bool wt = tid / kC % 2 == 0;
+                    const float f = la_power(decay, wt == kRev ? up : down);
+                    if (wt) M.wt[tid / (2 * kC)][j] = p.sigma * f;
+                    else M.ahead[tid / (2 * kC)][j] = p.tau * f;
+                } else if (tid < 5 * kC) {
+                    M.decay[j] = p.sigma * la_power(decay, j);
+                }
+                if (j == 0 && tid <= 2 * kC) M.f[tid / (2 * kC)] = la_power2(decay, len);
+            }
             uint64_t s[kMine / 2];  // rows kMine part .. of the state, pairs
             const LaState in = la_state(p, it.in, h, p.state_in, scratch);
             {
@@ -381,9 +455,9 @@ la_parts(const LaCore p, LaWork* work, const LaEntry* entries, float* scratch, b
                                 any && b0 + 2 * j + 1 < p.d_b ? src[in.row] : 0.f);
             }
             __syncthreads();  // the powers
-            uint64_t hi2 = 0, lo2 = 0;  // w^len of a chunk, in two parts
-            int known = 0;
-            auto add_update = [&](uint32_t at) {
+            auto add_update = [&](uint32_t at, int len) {
+                const float2 f = M.f[len < kC];
+                const uint64_t hi2 = pair(f.x, f.x), lo2 = pair(f.y, f.y);
 #pragma unroll
                 for (int blk = 0; blk < kMine / 8; ++blk) {
                     uint64_t u[4];
@@ -395,68 +469,60 @@ la_parts(const LaCore p, LaWork* work, const LaEntry* entries, float* scratch, b
                 tc_fence_before();  // (before this warp's next arrival)
             };
             auto len_of = [&](int c) { return min(kC, it.len - (kRev ? nch - 1 - c : c) * kC); };
-            auto decay_of = [&](int len) {
-                if (len == known) return;
-                const float2 f = la_power2(decay, len);
-                hi2 = pair(f.x, f.x), lo2 = pair(f.y, f.y);
-                known = len;
-            };
             if constexpr (kStateOnly) {
                 // The conversions of a chunk run beside the product of the one before.
 #pragma unroll 1
                 for (int c = 0; c < nch; ++c) {
                     const uint32_t ph = (n + c) & 1;
                     put(ph * L::kB, vb);
-                    put_w(kColC + 96 * ph, len_of(c));
+                    put_w(kColC + 96 * ph, len_of(c), vc);
                     arrive(&M.ab_ready);
-                    if (c + 1 < nch) fetch(c + 1, true, true);
+                    vb = fetch(p.b, p.heads_b, hb, c + 1);
+                    vc = fetch_c(c + 1);
                     if (c > 0) {
                         if (!(ok = warp_wait(&M.u_full[ph ^ 1], ((n + c - 1) >> 1) & 1))) break;
                         tc_fence_after();
-                        decay_of(len_of(c - 1));
-                        add_update(128 * (ph ^ 1));
+                        add_update(128 * (ph ^ 1), len_of(c - 1));
                     }
                 }
                 if (ok && nch > 0) {
                     const uint32_t m = n + nch - 1;
                     if ((ok = warp_wait(&M.u_full[m & 1], (m >> 1) & 1))) {
                         tc_fence_after();
-                        decay_of(len_of(nch - 1));
-                        add_update(128 * (m & 1));
+                        add_update(128 * (m & 1), len_of(nch - 1));
                     }
                 }
             } else {
-                if (nch > 0) {
-                    put(L::kA, va);
-                    put_c();
-                }
+                put(L::kA, va);
+                put_c(vc);
 #pragma unroll 1
                 for (int c = 0; c < nch; ++c) {
                     const uint32_t ph = (n + c) & 1;
                     const int x = kRev ? nch - 1 - c : c, len = len_of(c);
                     put(L::kB, vb);
                     arrive(&M.ab_ready);
-                    put_w(kColW, len);
+                    const Column vw = fetch_c(c);  // (again: the registers are not there to keep it)
                     {
+                        const int col = 32 * quarter + here(lane);
                         const uint32_t row = L::kS + (kMine * part >> 6) * kRows128 + col * 128;
                         const int first = kMine * part / 8;
 #pragma unroll
                         for (int m = 0; m < kMine / 8; ++m) {
-                            uint32_t q[4][kPs];
+                            float v[8];
 #pragma unroll
-                            for (int j = 0; j < 4; ++j) split<kPs>(s[4 * m + j], q[j]);
-                            uint8_t* dst = sm + row + (((first + m) ^ col) & 7) * 16;
-#pragma unroll
-                            for (int k = 0; k < kPs; ++k)
-                                *reinterpret_cast<uint4*>(dst + k * L::kTileS) =
-                                    make_uint4(q[0][k], q[1][k], q[2][k], q[3][k]);
+                            for (int j = 0; j < 4; ++j) unpair(s[4 * m + j], v[2 * j], v[2 * j + 1]);
+                            const uint32_t dst = base + row + (((first + m) ^ col) & 7) * 16;
+                            split<kPs>(v, [&](int k, const uint32_t(&r)[4]) {
+                                st_shared(dst + k * L::kTileS, r[0], r[1], r[2], r[3]);
+                            });
                         }
                     }
+                    put_w(kColW, len, vw);
                     arrive(&M.s_ready);
-                    if (c + 1 < nch) fetch(c + 1, true, false);
+                    prefetch(c + 1);
                     if (quarter < 2) {
                         // P: row i, 16 columns; what the mask leaves, decayed.
-                        const int i = 32 * quarter + lane;
+                        const int i = 32 * quarter + here(lane);
                         if (!(ok = warp_wait(&M.sc_full, ph))) break;
                         tc_fence_after();
 #pragma unroll
@@ -464,62 +530,66 @@ la_parts(const LaCore p, LaWork* work, const LaEntry* entries, float* scratch, b
                             const int j0 = 16 * part + 8 * m;
                             uint64_t u[4];
                             tmem_ld8(quad + kColSc + j0, u);
-                            uint32_t q[4][kPs];
+                            float v[8];
 #pragma unroll
                             for (int j = 0; j < 4; ++j) {
                                 const int e0 = kRev ? j0 + 2 * j - i : i - j0 - 2 * j;
                                 const int e1 = kRev ? e0 + 1 : e0 - 1;
-                                float f0, f1;
-                                unpair(u[j], f0, f1);
-                                f0 = e0 >= 0 ? f0 * (p.sigma * M.pw[e0]) : 0.f;
-                                f1 = e1 >= 0 ? f1 * (p.sigma * M.pw[e1]) : 0.f;
-                                split<kPs>(pair(f0, f1), q[j]);
+                                unpair(u[j], v[2 * j], v[2 * j + 1]);
+                                v[2 * j] = e0 >= 0 ? v[2 * j] * M.decay[e0] : 0.f;
+                                v[2 * j + 1] = e1 >= 0 ? v[2 * j + 1] * M.decay[e1] : 0.f;
                             }
-                            uint8_t* dst = sm + L::kP + i * 128 + (((j0 >> 3) ^ i) & 7) * 16;
-#pragma unroll
-                            for (int k = 0; k < kPs; ++k)
-                                *reinterpret_cast<uint4*>(dst + k * kRows64) =
-                                    make_uint4(q[0][k], q[1][k], q[2][k], q[3][k]);
+                            const uint32_t dst = base + L::kP + i * 128 + (((j0 >> 3) ^ i) & 7) * 16;
+                            split<kPs>(v, [&](int k, const uint32_t(&r)[4]) {
+                                st_shared(dst + k * kRows64, r[0], r[1], r[2], r[3]);
+                            });
                         }
                         arrive(&M.p_ready);
                     }
+                    const Ab na = fetch(p.a, p.heads_a, ha, c + 1);
                     if (!(ok = warp_wait(&M.o_full, ph))) break;
                     tc_fence_after();
                     {
-                        const int64_t step = static_cast<int64_t>(p.heads) * p.d_c;
-                        int64_t at = (static_cast<int64_t>(it.start) + x * kC + 16 * part) * step +
-                                     static_cast<int64_t>(h) * p.d_c + n0 + col;
+                        const int step = p.heads * p.d_c;
+                        const int col = 32 * quarter + here(lane);
+                        const int64_t at =
+                            static_cast<int64_t>(it.start + x * kC + 16 * part) * step +
+                            static_cast<int64_t>(h) * p.d_c + n0 + col;
                         const int live = mine ? len - 16 * part : 0;
+                        auto outputs = [&](auto* to) {
+                            const uint64_t tau = pair(p.tau, p.tau);
 #pragma unroll
-                        for (int m = 0; m < 2; ++m) {
-                            uint64_t u[4], v[4];
-                            tmem_ld8(quad + kColO1 + 16 * part + 8 * m, u);
-                            tmem_ld8(quad + kColO2 + 16 * part + 8 * m, v);
+                            for (int m = 0; m < 2; ++m) {
+                                uint64_t u[4], v[4];
+                                tmem_ld8(quad + kColO1 + 16 * part + 8 * m, u);
+                                tmem_ld8(quad + kColO2 + 16 * part + 8 * m, v);
+                                const ulonglong2* ahead = reinterpret_cast<const ulonglong2*>(
+                                    &M.ahead[len < kC][16 * part + 8 * m]);
 #pragma unroll
-                            for (int j = 0; j < 8; ++j, at += step) {
-                                const int i = 16 * part + 8 * m + j;
-                                float f[2], g[2];
-                                unpair(u[j >> 1], f[0], f[1]);
-                                unpair(v[j >> 1], g[0], g[1]);
-                                const float y =
-                                    p.tau * fmaf(M.pw[kRev ? max(len - 1 - i, 0) : i + 1], f[j & 1],
-                                                 g[j & 1]);
-                                if (8 * m + j < live) {
-                                    if (p.out_f32) static_cast<float*>(p.out)[at] = y;
-                                    else static_cast<T*>(p.out)[at] = from_f32<T>(y);
+                                for (int j = 0; j < 4; ++j) {
+                                    const uint64_t f = j & 1 ? ahead[j >> 1].y : ahead[j >> 1].x;
+                                    float y[2];
+                                    unpair(fma2(u[j], f, mul2(v[j], tau)), y[0], y[1]);
+#pragma unroll
+                                    for (int k = 0; k < 2; ++k)
+                                        if (8 * m + 2 * j + k < live)
+                                            to[(8 * m + 2 * j + k) * step] =
+                                                from_f32<std::remove_reference_t<decltype(*to)>>(y[k]);
                                 }
                             }
-                        }
+                        };
+                        if (here(p.out_f32)) outputs(static_cast<float*>(p.out) + at);
+                        else outputs(static_cast<T*>(p.out) + at);
                     }
-                    if (c + 1 < nch) {
-                        fetch(c + 1, false, true);
-                        put(L::kA, va);
-                        put_c();
+                    {
+                        const Column nc = fetch_c(c + 1);
+                        put(L::kA, na);
+                        put_c(nc);
+                        vb = fetch(p.b, p.heads_b, hb, c + 1);
                     }
-                    decay_of(len);
                     if (!(ok = warp_wait(&M.u_full[0], ph))) break;
                     tc_fence_after();
-                    add_update(kColU);
+                    add_update(kColU, len);
                 }
             }
             const LaState out = la_state(p, it.out, h, p.state_out, scratch);
