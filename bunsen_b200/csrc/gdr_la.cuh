@@ -35,6 +35,7 @@ struct LaCore {
     void* out;                  // [T, heads, d_c] in the operands' type, or f32
     int32_t out_f32;
     int32_t dtype;              // of a, b, c
+    int32_t scratch_t;          // states between segments are there as [d_c, d_b]
 };
 
 inline int64_t la_tokens(const LaCore& p) {
@@ -55,14 +56,20 @@ __device__ __forceinline__ void la_span(const LaCore& p, int s, int64_t& start, 
     end = y;
 }
 
+// Work lists of a call (gdr_la_plan.cuh). Two cores over the same positions in the same
+// direction, whose states are each other's transposes, may share them: given to
+// both launches, made by the first, with the states between segments.
+struct LaLists;
+
 // Kernels of the core (each its own file) and what they take.
 cudaError_t launch_la_recurrent(const LaCore& p, cudaStream_t stream);
 bool la_parts_supports(const LaCore& p);
-cudaError_t launch_la_parts(const LaCore& p, cudaStream_t stream);
+cudaError_t launch_la_parts(const LaCore& p, cudaStream_t stream, LaLists* shared = nullptr);
 bool la_tc_supports(const LaCore& p);
 // split: long sequences may go in segments (scratch from the library's pool);
 // must: they do even where it looks slower; forced: segment length in chunks, or 0.
-cudaError_t launch_la_tc(const LaCore& p, bool split, bool must, int forced, cudaStream_t stream);
+cudaError_t launch_la_tc(const LaCore& p, bool split, bool must, int forced, cudaStream_t stream,
+                         LaLists* shared = nullptr);
 cudaError_t take_la_error(int* flag);
 constexpr int kLaMaxD = 256;  // d_k, d_v of any kernel here
 

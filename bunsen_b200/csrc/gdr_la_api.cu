@@ -3,6 +3,7 @@
 #include <cmath>
 
 #include "gdr_la.cuh"
+#include "gdr_la_plan.cuh"
 #include "gdr_qk_norm_rope.cuh"
 
 namespace gdr {
@@ -100,19 +101,29 @@ void operands(LaCore& p, const void* x, int hx, const void* y, int hy, const voi
     p.d_c = d_c;
 }
 
-// The kernel that runs a core.
-cudaError_t run_core(const gdr_la_params& a, const LaCore& p, bool chunked, cudaStream_t s) {
-    if (!chunked || la_tokens(p) == 0) return launch_la_recurrent(p, s);
-    const bool tc = la_tc_supports(p);
-    if (!tc && a.algo >= GDR_ALGO_TENSOR) return cudaErrorNotSupported;
-    if (tc && a.algo != GDR_ALGO_CUDA_CORE)
-        return launch_la_tc(p, a.algo != GDR_ALGO_TENSOR, a.algo == GDR_ALGO_TENSOR_SPLIT,
-                            a.split_chunks, s);
-    // Short sequences step as fast as a chunk does; the others go in chunks.
+enum class Kernel { none, recurrent, tensor, parts };
+
+Kernel kernel_of(const gdr_la_params& a, const LaCore& p, bool chunked) {
     const int64_t tokens = la_tokens(p);
-    if (la_parts_supports(p) && tokens > 4 * static_cast<int64_t>(p.n_seqs))
-        return launch_la_parts(p, s);
-    return launch_la_recurrent(p, s);
+    if (!chunked || tokens == 0) return Kernel::recurrent;
+    const bool tc = la_tc_supports(p);
+    if (!tc && a.algo >= GDR_ALGO_TENSOR) return Kernel::none;
+    if (tc && a.algo != GDR_ALGO_CUDA_CORE) return Kernel::tensor;
+    // Short sequences step as fast as a chunk does; the others go in chunks.
+    return la_parts_supports(p) && tokens > 4 * static_cast<int64_t>(p.n_seqs) ? Kernel::parts
+                                                                               : Kernel::recurrent;
+}
+
+cudaError_t run_core(const gdr_la_params& a, const LaCore& p, bool chunked, cudaStream_t s,
+                     LaLists* shared = nullptr) {
+    switch (kernel_of(a, p, chunked)) {
+        case Kernel::none: return cudaErrorNotSupported;
+        case Kernel::tensor:
+            return launch_la_tc(p, a.algo != GDR_ALGO_TENSOR, a.algo == GDR_ALGO_TENSOR_SPLIT,
+                                a.split_chunks, s, shared);
+        case Kernel::parts: return launch_la_parts(p, s, shared);
+        default: return launch_la_recurrent(p, s);
+    }
 }
 
 gdr_status forward(bool chunked, const gdr_la_params* params, const void* q, const void* k,
@@ -184,37 +195,54 @@ gdr_status gdr_la_backward(const gdr_la_params* params, const void* q, const voi
             return GDR_ERR_CUDA;
     }
     // dv_t = D_t^T k_t, and the gradient of the initial state.
-    LaCore p = base;
-    operands(p, k, a.heads_qk, q, a.heads_qk, d_out, a.heads_v, a.d_k, a.d_v);
-    p.sigma = scale;
-    p.tau = 1.f;
-    p.reverse = 1;
-    p.state_in = d_state_out;
-    p.state_out = d_state_in;
-    p.out = dv;
-    e = run_core(a, p, true, s);
-    for (int which = 0; which < 2 && e == cudaSuccess && tokens > 0; ++which) {
-        p = base;
-        p.state_t = 1;
-        if (which == 0) {  // dq_t = scale S_t do_t
-            operands(p, d_out, a.heads_v, v, a.heads_v, k, a.heads_qk, a.d_v, a.d_k);
-            p.sigma = 1.f;
-            p.tau = scale;
-            p.state_in = state_in;
-        } else {  // dk_t = D_t v_t
-            operands(p, v, a.heads_v, d_out, a.heads_v, q, a.heads_qk, a.d_v, a.d_k);
-            p.sigma = scale;
-            p.tau = 1.f;
-            p.reverse = 1;
-            p.state_in = d_state_out;
-        }
-        void* grad = which == 0 ? dq : dk;
-        p.out = part != nullptr ? part : grad;
-        p.out_f32 = part != nullptr;
-        e = run_core(a, p, true, s);
-        if (e == cudaSuccess && part != nullptr)
-            e = launch_sum_group(a.dtype, part, grad, a.heads_qk, group, a.d_k, tokens, cu_seqlens,
-                                 base.n_seqs, s);
+    LaCore v_core = base;
+    operands(v_core, k, a.heads_qk, q, a.heads_qk, d_out, a.heads_v, a.d_k, a.d_v);
+    v_core.sigma = scale;
+    v_core.tau = 1.f;
+    v_core.reverse = 1;
+    v_core.state_in = d_state_out;
+    v_core.state_out = d_state_in;
+    v_core.out = dv;
+    // dk_t = D_t v_t, D transposed.
+    LaCore k_core = base;
+    operands(k_core, v, a.heads_v, d_out, a.heads_v, q, a.heads_qk, a.d_v, a.d_k);
+    k_core.sigma = scale;
+    k_core.tau = 1.f;
+    k_core.reverse = 1;
+    k_core.state_t = 1;
+    k_core.state_in = d_state_out;
+    // dq_t = scale S_t do_t.
+    LaCore q_core = base;
+    operands(q_core, d_out, a.heads_v, v, a.heads_v, k, a.heads_qk, a.d_v, a.d_k);
+    q_core.sigma = 1.f;
+    q_core.tau = scale;
+    q_core.state_t = 1;
+    q_core.state_in = state_in;
+    for (LaCore* c : {&k_core, &q_core}) {
+        c->out = part != nullptr ? part : c == &k_core ? dk : dq;
+        c->out_f32 = part != nullptr;
+    }
+    auto sum = [&](void* grad) {
+        return part == nullptr ? cudaSuccess
+                               : launch_sum_group(a.dtype, part, grad, a.heads_qk, group, a.d_k,
+                                                  tokens, cu_seqlens, base.n_seqs, s);
+    };
+    // dv and dk run over the same D: one of them finds its states between segments.
+    const Kernel kernel = kernel_of(a, v_core, true);
+    const bool same = (kernel == Kernel::tensor || kernel == Kernel::parts) &&
+                      kernel_of(a, k_core, true) == kernel && la_same_lists(v_core, k_core);
+    LaLists lists;
+    k_core.scratch_t = same;
+    e = run_core(a, v_core, true, s, same ? &lists : nullptr);
+    if (e == cudaSuccess && tokens > 0) {
+        e = run_core(a, k_core, true, s, same ? &lists : nullptr);
+        if (e == cudaSuccess) e = sum(dk);
+    }
+    const cudaError_t r = la_release(lists, s);
+    if (e == cudaSuccess) e = r;
+    if (e == cudaSuccess && tokens > 0) {
+        e = run_core(a, q_core, true, s);
+        if (e == cudaSuccess) e = sum(dq);
     }
     if (part != nullptr) {
         const cudaError_t f = cudaFreeAsync(part, s);

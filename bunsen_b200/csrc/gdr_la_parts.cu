@@ -614,7 +614,7 @@ la_parts(const LaCore p, LaWork* work, const LaEntry* entries, float* scratch, b
 }
 
 template <typename T, int kDb, bool kRev>
-cudaError_t start(const LaCore& p, cudaStream_t stream) {
+cudaError_t start(const LaCore& p, LaLists* shared, cudaStream_t stream) {
     auto* full = la_parts<T, kDb, kRev, false>;
     auto* states = la_parts<T, kDb, kRev, true>;
     constexpr int kFull = static_cast<int>(Layout<T, kDb, false>::kBytes),
@@ -626,27 +626,34 @@ cudaError_t start(const LaCore& p, cudaStream_t stream) {
     const bool vec = p.d_b % 8 == 0 && ((reinterpret_cast<uintptr_t>(p.a) |
                                          reinterpret_cast<uintptr_t>(p.b)) & 15) == 0;
     const int grid = la_sm_count(), blocks = (p.d_c + kCols - 1) / kCols;
-    LaLists lists;
-    if ((e = la_prepare(p, grid, blocks, {true, false, 0, 0.3f, 3.f}, lists, stream)) != cudaSuccess)
-        return e;
-    if (lists.split) {
-        states<<<grid, kThreads, kStates, stream>>>(p, &lists.plan->states, lists.states,
-                                                    lists.slots, vec);
-        la_scan_states(p, lists, stream);
+    // In chunks of 128: 13 us at one CTA an SM, 0.3 of that in the states' pass, whose start,
+    // the list's kernel and the scan are 2.
+    LaLists own;
+    LaLists& lists = shared != nullptr ? *shared : own;
+    if (lists.uses == 0) {
+        e = la_prepare(p, grid, blocks, {true, false, 0, 0.3f, 2.f}, shared != nullptr, lists, stream);
+        if (e != cudaSuccess) return e;
+        if (lists.split) {
+            states<<<grid, kThreads, kStates, stream>>>(p, &lists.plan->states, lists.states,
+                                                        lists.slots, vec);
+            la_scan_states(p, lists, stream);
+        }
     }
     const int64_t jobs = static_cast<int64_t>(p.n_seqs) * p.heads * blocks;
     full<<<lists.plan != nullptr ? grid : static_cast<int>(jobs), kThreads, kFull, stream>>>(
-        p, lists.plan != nullptr ? &lists.plan->main : nullptr, lists.main, lists.slots, vec);
+        p, lists.plan != nullptr ? &lists.plan->main[lists.uses] : nullptr, lists.main, lists.slots,
+        vec);
+    ++lists.uses;
     e = cudaGetLastError();
-    const cudaError_t f = la_release(lists, stream);
+    const cudaError_t f = la_release(own, stream);
     return e != cudaSuccess ? e : f;
 }
 
 template <typename T>
-cudaError_t pick(const LaCore& p, cudaStream_t stream) {
+cudaError_t pick(const LaCore& p, LaLists* shared, cudaStream_t stream) {
     if (p.d_b <= 64)
-        return p.reverse ? start<T, 64, true>(p, stream) : start<T, 64, false>(p, stream);
-    return p.reverse ? start<T, 128, true>(p, stream) : start<T, 128, false>(p, stream);
+        return p.reverse ? start<T, 64, true>(p, shared, stream) : start<T, 64, false>(p, shared, stream);
+    return p.reverse ? start<T, 128, true>(p, shared, stream) : start<T, 128, false>(p, shared, stream);
 }
 
 }  // namespace
@@ -656,11 +663,11 @@ bool la_parts_supports(const LaCore& p) {
            static_cast<int64_t>(p.n_seqs) * p.heads < (int64_t{1} << 28);
 }
 
-cudaError_t launch_la_parts(const LaCore& p, cudaStream_t stream) {
+cudaError_t launch_la_parts(const LaCore& p, cudaStream_t stream, LaLists* shared) {
     switch (p.dtype) {
-        case GDR_DTYPE_BF16: return pick<__nv_bfloat16>(p, stream);
-        case GDR_DTYPE_F16: return pick<__half>(p, stream);
-        default: return pick<float>(p, stream);
+        case GDR_DTYPE_BF16: return pick<__nv_bfloat16>(p, shared, stream);
+        case GDR_DTYPE_F16: return pick<__half>(p, shared, stream);
+        default: return pick<float>(p, shared, stream);
     }
 }
 

@@ -83,7 +83,7 @@ la_plan(const LaCore p, LaPlan* plan, LaEntry* main, LaEntry* states, LaSplit* s
                 const int parts = (c + L - 1) / L;
                 again += (parts - 1) * L;
                 segs += parts;
-                whole += c / L;
+                whole += (c + L / 3) / L;  // (a part of two thirds too)
                 parts_most = max(parts_most, parts);
             }
         }
@@ -170,7 +170,7 @@ la_plan(const LaCore p, LaPlan* plan, LaEntry* main, LaEntry* states, LaSplit* s
     }
     __syncthreads();
     if (tid == 0) {
-        plan->main = {p.n_seqs + slots - n_splits, grid};
+        plan->main[0] = plan->main[1] = {p.n_seqs + slots - n_splits, grid};
         plan->states = {n_states, grid};
         plan->splits = n_splits;
         plan->seg_tokens = L * kLaChunk;
@@ -227,8 +227,12 @@ int la_sm_count() {
     return n > 0 ? n : 148;
 }
 
-cudaError_t la_prepare(const LaCore& p, int grid, int blocks, LaSplitCost o, LaLists& out,
-                       cudaStream_t stream) {
+cudaError_t la_prepare(const LaCore& p, int grid, int blocks, LaSplitCost o, bool shared,
+                       LaLists& out, cudaStream_t stream) {
+    if (shared) {  // two passes over the segments for one that finds their states
+        o.state_cost *= 0.5f;
+        o.fixed_cost *= 0.5f;
+    }
     // What splitting could bring: no sequence is longer than `longest` chunks, and the
     // work fills every CTA for `each` chunks or fewer.
     const int64_t tokens = la_tokens(p);

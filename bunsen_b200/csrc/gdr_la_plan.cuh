@@ -46,7 +46,7 @@ __device__ __forceinline__ LaState la_state(const LaCore& p, int x, int h, const
                                             const float* scratch) {
     const int64_t size = static_cast<int64_t>(p.d_b) * p.d_c;
     const float* base = x >= 0 ? own : x == -1 ? nullptr : scratch;
-    const bool turned = x >= 0 && p.state_t;
+    const bool turned = x >= 0 ? p.state_t : p.scratch_t;
     return {base != nullptr
                 ? base + (static_cast<int64_t>(x >= 0 ? x : -2 - x) * p.heads + h) * size
                 : nullptr,
@@ -57,9 +57,8 @@ struct LaSplit {
     int32_t base, parts, seq, unused;  // segment r's state: slot base + r, r >= 1
 };
 struct LaPlan {
-    LaWork main, states;
+    LaWork main[2], states;  // (main: for either of two launches that share the lists)
     int32_t splits, seg_tokens;
-    int32_t pad[2];
 };
 
 // How a kernel's segments cost: in chunks of its main pass, a chunk of the pass
@@ -79,12 +78,18 @@ struct LaLists {
     LaSplit* splits = nullptr;
     float* slots = nullptr;
     bool split = false;  // some sequences may be in segments: run the states' pass
+    int uses = 0;        // launches that have used them
 };
-// grid: CTAs of the persistent kernels; blocks: jobs of each (entry, head).
-cudaError_t la_prepare(const LaCore& p, int grid, int blocks, LaSplitCost o, LaLists& lists,
-                       cudaStream_t stream);
+// grid: CTAs of the persistent kernels; blocks: jobs of each (entry, head); shared: two
+// launches will use the lists.
+cudaError_t la_prepare(const LaCore& p, int grid, int blocks, LaSplitCost o, bool shared,
+                       LaLists& lists, cudaStream_t stream);
 void la_scan_states(const LaCore& p, const LaLists& lists, cudaStream_t stream);
 cudaError_t la_release(const LaLists& lists, cudaStream_t stream);
 int la_sm_count();
+// Two cores whose lists would be the same (jobs of 128 columns).
+inline bool la_same_lists(const LaCore& x, const LaCore& y) {
+    return (x.d_c + 127) / 128 == (y.d_c + 127) / 128;
+}
 
 }  // namespace gdr

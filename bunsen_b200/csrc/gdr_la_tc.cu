@@ -983,7 +983,8 @@ bool la_tc_supports(const LaCore& p) {
            static_cast<int64_t>(p.n_seqs) * p.heads < (int64_t{1} << 30);
 }
 
-cudaError_t launch_la_tc(const LaCore& p, bool split, bool must, int forced, cudaStream_t stream) {
+cudaError_t launch_la_tc(const LaCore& p, bool split, bool must, int forced, cudaStream_t stream,
+                         LaLists* shared) {
     CUtensorMap ma, mb, mc, mo;
     const int64_t tokens = la_tokens(p);
     if (!tile_map(&ma, p.a, tokens, p.heads_a, p.d_b, kC) ||
@@ -998,23 +999,27 @@ cudaError_t launch_la_tc(const LaCore& p, bool split, bool must, int forced, cud
         if ((e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                       static_cast<int>(kSmemBytes))) != cudaSuccess)
             return e;
-    // A chunk takes 3.8 us at one CTA an SM; the states' pass 0.85 of that (it waits for
-    // the same operand), and its launches and the scan some 6 chunks.
+    // A chunk takes 2.9 us at one CTA an SM, one of the states' pass 0.45 of that; that
+    // pass's start, the list's kernel and the scan 11 chunks.
     const int sms = la_sm_count();
-    LaLists lists;
-    e = la_prepare(p, sms, 1, {split, must, forced, 0.5f, 9.f}, lists, stream);
-    if (e != cudaSuccess) return e;
-    if (lists.split) {
-        states<<<sms, kThreads, kSmemBytes, stream>>>(p, ma, mb, mc, mo, &lists.plan->states,
-                                                      lists.states, lists.slots);
-        la_scan_states(p, lists, stream);
+    LaLists own;
+    LaLists& lists = shared != nullptr ? *shared : own;
+    if (lists.uses == 0) {
+        e = la_prepare(p, sms, 1, {split, must, forced, 0.45f, 11.f}, shared != nullptr, lists, stream);
+        if (e != cudaSuccess) return e;
+        if (lists.split) {
+            states<<<sms, kThreads, kSmemBytes, stream>>>(p, ma, mb, mc, mo, &lists.plan->states,
+                                                          lists.states, lists.slots);
+            la_scan_states(p, lists, stream);
+        }
     }
     const int64_t jobs = static_cast<int64_t>(p.n_seqs) * p.heads;
     full<<<lists.plan != nullptr ? sms : static_cast<int>(jobs), kThreads, kSmemBytes, stream>>>(
-        p, ma, mb, mc, mo, lists.plan != nullptr ? &lists.plan->main : nullptr, lists.main,
-        lists.slots);
+        p, ma, mb, mc, mo, lists.plan != nullptr ? &lists.plan->main[lists.uses] : nullptr,
+        lists.main, lists.slots);
+    ++lists.uses;
     e = cudaGetLastError();
-    const cudaError_t f = la_release(lists, stream);
+    const cudaError_t f = la_release(own, stream);
     return e != cudaSuccess ? e : f;
 }
 
