@@ -50,7 +50,7 @@ using namespace sm100;
 constexpr int kC = 64, kCols = 128;
 constexpr int kWarps = 16, kThreads = 32 * (kWarps + 4);
 constexpr uint32_t kRows64 = 64 * 128, kRows128 = 128 * 128;  // bytes of a tile 64 wide
-constexpr uint32_t kColSc = 0, kColO1 = 64, kColO2 = 128, kColU = 192, kColC = 320, kColW = 416;
+constexpr uint32_t kColSc = 0, kColO2 = 0, kColO1 = 64, kColU = 128, kColC = 256, kColS = 352;
 
 template <typename T, int kDb, bool kStateOnly>
 struct Layout {
@@ -59,20 +59,22 @@ struct Layout {
     static constexpr int kPs = sizeof(T) == 4 ? 3 : 2;
     static constexpr int kHalves = kDb / 64;
     static constexpr uint32_t kTileAb = kHalves * kRows64, kTileS = kHalves * kRows128;
+    // a, b, the weighted b, the third part of the state's copy, P; or two weighted b.
     static constexpr uint32_t kA = 0, kB = kA + kIn * kTileAb;
-    static constexpr uint32_t kS = kB + kIn * kTileAb;
-    static constexpr uint32_t kP = kS + (kStateOnly ? 0 : kPs * kTileS);
+    static constexpr uint32_t kBw = kStateOnly ? 0 : kB + kIn * kTileAb;
+    static constexpr uint32_t kS = kBw + (kStateOnly ? 6 : 3) * kTileAb;
+    static constexpr uint32_t kP = kS + (kStateOnly || kPs < 3 ? 0 : kTileS);
     static constexpr uint32_t kMisc = kP + (kStateOnly ? 0 : kPs * kRows64);
     static constexpr uint32_t kBytes = kMisc + 2048;
 };
 
 struct Misc {
     // Powers for a job's whole chunks, and for its short one:
-    alignas(16) float wt[2][kC];     // sigma w^{len-1-j}, the weights of c (backward w^{j+1})
+    alignas(16) float wt[2][kC];     // sigma w^{len-1-j}, the weights of b (backward w^{j+1})
     alignas(16) float ahead[2][kC];  // tau w^{i+1}, of a_i . S (backward w^{len-1-i})
     float2 f[2];                     // w^len, in two parts
     float decay[kC];                 // sigma w^0 .. w^{kC-1}
-    uint64_t ab_ready, s_ready, p_ready, sc_full, o_full, u_full[2], drain;
+    uint64_t ab_ready, s_ready, p_ready, w_ready, sc_full, o_full, u_full[2], drain;
     uint32_t tmem;
     int next;
 };
@@ -207,7 +209,8 @@ la_parts(const LaCore p, LaWork* work, const LaEntry* entries, float* scratch, b
     if (tid == 0) {
         mbar_init(&M.ab_ready, kWarps);
         mbar_init(&M.s_ready, kWarps);
-        mbar_init(&M.p_ready, kWarps / 2);
+        mbar_init(&M.p_ready, kWarps);
+        mbar_init(&M.w_ready, kWarps);
         mbar_init(&M.sc_full, 1);
         mbar_init(&M.o_full, 1);
         mbar_init(&M.u_full[0], 1);
@@ -256,13 +259,14 @@ la_parts(const LaCore p, LaWork* work, const LaEntry* entries, float* scratch, b
     // 4 x 112 + 32.
     if (warp >= kWarps) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 32;");
-        each_job([&](const LaEntry& it, int, int, int nch) {
+        each_job([&](const LaEntry& it, int h, int n0, int nch) {
             // ---- the products ------------------------------------------------------
+            constexpr uint32_t kScores = idesc_bf16(64, kC, 0, 0, 0);
             constexpr uint32_t kKK = idesc_bf16(128, kC, 0, 0, 0);
             constexpr uint32_t kKMn = idesc_bf16(128, kDb, 0, 1, 0);
-            auto update = [&](uint32_t b_at, uint32_t w_at, uint32_t u_at) {
-                each_part<3, kIn, 2>([&](int i, int j, uint32_t acc) {
-                    product_ts<2048>(u_at, w_at + 32 * i,
+            auto update = [&](uint32_t b_at, uint32_t c_at, uint32_t u_at) {
+                each_part<kIn, 3, 2>([&](int i, int j, uint32_t acc) {
+                    product_ts<2048>(u_at, c_at + 32 * i,
                                      sdesc_sw128(b_at + j * L::kTileAb, kRows64, 1024), kKMn, acc);
                 });
             };
@@ -270,19 +274,21 @@ la_parts(const LaCore p, LaWork* work, const LaEntry* entries, float* scratch, b
 #pragma unroll 1
             for (int c = 0; warp == kWarps && ok && c < nch; ++c) {
                 const uint32_t ph = (n + c) & 1, base = here(smem_u32(sm));
-                if (!(ok = warp_wait(&M.ab_ready, ph))) break;
-                tc_fence_after();
                 if constexpr (kStateOnly) {
+                    if (!(ok = warp_wait(&M.w_ready, ph))) break;
+                    tc_fence_after();
                     if (elect_one()) {
-                        update(base + ph * L::kB, kColC + 96 * ph, 128 * ph);
+                        update(base + ph * 3 * L::kTileAb, kColC + 96 * ph, 128 * ph);
                         umma_commit(&M.u_full[ph]);
                     }
                 } else {
+                    if (!(ok = warp_wait(&M.ab_ready, ph))) break;
+                    tc_fence_after();
                     if (elect_one()) {
                         each_part<kIn, kIn, kOrder>([&](int i, int j, uint32_t acc) {
                             product_ss<kHalves, kRows64, kRows64>(
                                 kColSc, sdesc_sw128(base + L::kA + i * L::kTileAb, 16, 1024),
-                                sdesc_sw128(base + L::kB + j * L::kTileAb, 16, 1024), kKK, acc);
+                                sdesc_sw128(base + L::kB + j * L::kTileAb, 16, 1024), kScores, acc);
                         });
                         umma_commit(&M.sc_full);
                     }
@@ -290,9 +296,18 @@ la_parts(const LaCore p, LaWork* work, const LaEntry* entries, float* scratch, b
                     tc_fence_after();
                     if (elect_one())
                         each_part<kPs, kIn, kOrder>([&](int i, int j, uint32_t acc) {
-                            product_ss<kHalves, kRows128, kRows64>(
-                                kColO1, sdesc_sw128(base + L::kS + i * L::kTileS, 16, 1024),
-                                sdesc_sw128(base + L::kA + j * L::kTileAb, 16, 1024), kKK, acc);
+                            const uint32_t a_at = base + L::kA + j * L::kTileAb;
+                            if (i == 2) {
+                                product_ss<kHalves, kRows128, kRows64>(
+                                    kColO1, sdesc_sw128(base + L::kS, 16, 1024),
+                                    sdesc_sw128(a_at, 16, 1024), kKK, acc);
+                                return;
+                            }
+#pragma unroll
+                            for (int x = 0; x < kHalves; ++x)
+                                product_ts<32>(kColO1, kColS + kDb / 2 * i + 32 * x,
+                                               sdesc_sw128(a_at + x * kRows64, 16, 1024), kKK,
+                                               x == 0 ? acc : 1);
                         });
                     if (!(ok = warp_wait(&M.p_ready, ph))) break;
                     tc_fence_after();
@@ -303,10 +318,35 @@ la_parts(const LaCore p, LaWork* work, const LaEntry* entries, float* scratch, b
                                            acc);
                         });
                         umma_commit(&M.o_full);
-                        update(base + L::kB, kColW, kColU);
+                    }
+                    if (!(ok = warp_wait(&M.w_ready, ph))) break;
+                    tc_fence_after();
+                    if (elect_one()) {
+                        update(base + L::kBw, kColC, kColU);
                         umma_commit(&M.u_full[0]);
                     }
                 }
+            }
+            // The next chunk's lines to L2, by the group's other warps: its loads come when
+            // registers are free for them.
+            for (int c = 0; !kStateOnly && warp > kWarps && ok && c + 1 < nch; ++c) {
+                if (!(ok = warp_wait(&M.sc_full, (n + c) & 1))) break;
+                constexpr int kLine = 128 / static_cast<int>(sizeof(T));
+                const int x0 = kRev ? nch - 2 - c : c + 1;
+                const int64_t row = static_cast<int64_t>(it.start) + x0 * kC;
+                const int len = min(kC, it.len - x0 * kC);
+                auto lines = [&](const void* of, int heads, int d, int from, int width) {
+                    const T* src = static_cast<const T*>(of) +
+                                   (row * heads + h / (p.heads / heads)) * d + from;
+                    const int each = (min(width, d - from) + kLine - 1) / kLine;
+#pragma unroll 1
+                    for (int x = tid - 32 * (kWarps + 1); x < len * each; x += 96)
+                        asm volatile("prefetch.global.L2 [%0];" ::"l"(
+                            src + x / each * (heads * d) + x % each * kLine));
+                };
+                lines(p.a, p.heads_a, p.d_b, 0, kDb);
+                lines(p.c, p.heads_c, p.d_c, n0, kCols);
+                lines(p.b, p.heads_b, p.d_b, 0, kDb);
             }
         });
         if (warp == kWarps) {  // nothing of this CTA's may be in flight when it ends
@@ -359,64 +399,35 @@ la_parts(const LaCore p, LaWork* work, const LaEntry* entries, float* scratch, b
                     o.v[j >> 3].v[j & 7] = j < live ? src[j * step] : T(0.f);
                 return o;
             };
-            // The lines of a chunk to L2: its loads come when registers are free for them.
-            auto prefetch = [&](int c) {
-                int64_t row;
-                int len;
-                chunk_at(c, row, len);
-                const int tid = here(threadIdx.x), r = tid >> 3, x = (tid & 3) * 128 / static_cast<int>(sizeof(T));
-                if (r >= len) return;
-                auto line = [&](const void* base, int heads, int head, int d, int at) {
-                    if (at < d)
-                        asm volatile("prefetch.global.L2 [%0];" ::"l"(
-                            static_cast<const T*>(base) + ((row + r) * heads + head) * d + at));
-                };
-                if (tid & 4) {
-                    line(p.b, p.heads_b, hb, p.d_b, x);
-                } else {
-                    if (!kStateOnly) line(p.a, p.heads_a, ha, p.d_b, x);
-                    line(p.c, p.heads_c, hc, p.d_c, n0 + x);
-                }
-            };
-            // Parts of a or b: rows of 128 bytes, 16 of them exchanged by the row's number.
-            auto put = [&](uint32_t at, const Ab& from) {
+            // Parts of a or b, or of b with weights: rows of 128 bytes, 16 of them
+            // exchanged by the row's number.
+            auto put = [&](uint32_t at, const Ab& from, auto parts, const float* weights) {
                 const int tid = here(threadIdx.x);
 #pragma unroll
                 for (int i = 0; i < kEights; ++i) {
                     const int x = tid + 32 * kWarps * i, r = x / (kDb / 8), d = x % (kDb / 8);
+                    const float w = weights != nullptr ? weights[r] : 1.f;
                     float v[8];
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) v[j] = to_f32(from.v[i].v[j]);
+                    for (int j = 0; j < 8; ++j) {
+                        v[j] = to_f32(from.v[i].v[j]);
+                        if (weights != nullptr) v[j] *= w;
+                    }
                     const uint32_t dst = base + at + (d >> 3) * kRows64 + r * 128 + (((d ^ r) & 7) << 4);
-                    split<kIn>(v, [&](int k, const uint32_t(&r)[4]) {
+                    split<decltype(parts)::value>(v, [&](int k, const uint32_t(&r)[4]) {
                         st_shared(dst + k * L::kTileAb, r[0], r[1], r[2], r[3]);
                     });
                 }
             };
-            // Eight pairs of this thread's column of c.
-            auto put_column = [&](uint32_t at, float(&v)[16], auto parts) {
-                split<decltype(parts)::value>(v, [&](int k, const uint32_t(&r)[8]) {
-                    tmem_st8(quad + at + 32 * k + 8 * part, r);
-                });
-            };
-            auto put_c = [&](const Column& vc) {
+            constexpr std::integral_constant<int, kIn> as_read{};
+            constexpr std::integral_constant<int, 3> weighted{};
+            auto put_c = [&](uint32_t at, const Column& vc) {
                 float v[16];
 #pragma unroll
                 for (int j = 0; j < 16; ++j) v[j] = to_f32(vc.v[j >> 3].v[j & 7]);
-                put_column(kColC, v, std::integral_constant<int, kIn>{});
-            };
-            auto put_w = [&](uint32_t at, int len, const Column& vc) {
-                float v[16];
-                const float4* w = reinterpret_cast<const float4*>(&M.wt[len < kC][16 * part]);
-#pragma unroll
-                for (int j = 0; j < 16; j += 4) {
-                    const float4 f = w[j >> 2];
-                    v[j] = to_f32(vc.v[j >> 3].v[j & 7]) * f.x;
-                    v[j + 1] = to_f32(vc.v[j >> 3].v[(j & 7) + 1]) * f.y;
-                    v[j + 2] = to_f32(vc.v[j >> 3].v[(j & 7) + 2]) * f.z;
-                    v[j + 3] = to_f32(vc.v[j >> 3].v[(j & 7) + 3]) * f.w;
-                }
-                put_column(at, v, std::integral_constant<int, 3>{});
+                split<kIn>(v, [&](int k, const uint32_t(&r)[8]) {
+                    tmem_st8(quad + at + 32 * k + 8 * part, r);
+                });
             };
             auto arrive = [&](uint64_t* bar) {  // all of this warp's writes before
                 tmem_wait_st();
@@ -474,9 +485,9 @@ la_parts(const LaCore p, LaWork* work, const LaEntry* entries, float* scratch, b
 #pragma unroll 1
                 for (int c = 0; c < nch; ++c) {
                     const uint32_t ph = (n + c) & 1;
-                    put(ph * L::kB, vb);
-                    put_w(kColC + 96 * ph, len_of(c), vc);
-                    arrive(&M.ab_ready);
+                    put(ph * 3 * L::kTileAb, vb, weighted, M.wt[len_of(c) < kC]);
+                    put_c(kColC + 96 * ph, vc);
+                    arrive(&M.w_ready);
                     vb = fetch(p.b, p.heads_b, hb, c + 1);
                     vc = fetch_c(c + 1);
                     if (c > 0) {
@@ -493,59 +504,63 @@ la_parts(const LaCore p, LaWork* work, const LaEntry* entries, float* scratch, b
                     }
                 }
             } else {
-                put(L::kA, va);
-                put_c(vc);
+                put(L::kA, va, as_read, nullptr);
 #pragma unroll 1
                 for (int c = 0; c < nch; ++c) {
                     const uint32_t ph = (n + c) & 1;
                     const int x = kRev ? nch - 1 - c : c, len = len_of(c);
-                    put(L::kB, vb);
+                    put(L::kB, vb, as_read, nullptr);
                     arrive(&M.ab_ready);
-                    const Column vw = fetch_c(c);  // (again: the registers are not there to keep it)
-                    {
+                    // The state's copy: two parts on TMEM's lanes, the third in shared memory,
+                    // which the scores' product keeps busy.
+#pragma unroll
+                    for (int m = 0; m < kMine / 16; ++m) {
                         const int col = 32 * quarter + here(lane);
-                        const uint32_t row = L::kS + (kMine * part >> 6) * kRows128 + col * 128;
-                        const int first = kMine * part / 8;
+                        const int at = kMine * part + 16 * m;  // rows
+                        float v[16];
 #pragma unroll
-                        for (int m = 0; m < kMine / 8; ++m) {
-                            float v[8];
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) unpair(s[4 * m + j], v[2 * j], v[2 * j + 1]);
-                            const uint32_t dst = base + row + (((first + m) ^ col) & 7) * 16;
-                            split<kPs>(v, [&](int k, const uint32_t(&r)[4]) {
-                                st_shared(dst + k * L::kTileS, r[0], r[1], r[2], r[3]);
-                            });
-                        }
+                        for (int j = 0; j < 8; ++j) unpair(s[8 * m + j], v[2 * j], v[2 * j + 1]);
+                        split<kPs>(v, [&](int k, const uint32_t(&r)[8]) {
+                            if (k < 2) {
+                                tmem_st8(quad + kColS + kDb / 2 * k + at / 2, r);
+                                return;
+                            }
+                            const uint32_t dst = base + L::kS + (at >> 6) * kRows128 + col * 128;
+                            const int x = at >> 3 & 7;
+                            st_shared(dst + ((x ^ col) & 7) * 16, r[0], r[1], r[2], r[3]);
+                            st_shared(dst + (((x + 1) ^ col) & 7) * 16, r[4], r[5], r[6], r[7]);
+                        });
                     }
-                    put_w(kColW, len, vw);
                     arrive(&M.s_ready);
-                    prefetch(c + 1);
-                    if (quarter < 2) {
-                        // P: row i, 16 columns; what the mask leaves, decayed.
-                        const int i = 32 * quarter + here(lane);
+                    put_c(kColC, vc);
+                    {
+                        // P: the scores' 64 rows are the first 16 lanes of every quarter; the others
+                        // take half of their 16 columns. What the mask leaves, decayed.
+                        const int i = 16 * quarter + here(lane & 15);
+                        const int j0 = 16 * part + (lane & 16) / 2;
                         if (!(ok = warp_wait(&M.sc_full, ph))) break;
                         tc_fence_after();
+                        uint64_t near[4], far[4];
+                        tmem_ld8(quad + kColSc + 16 * part, near);
+                        tmem_ld8(quad + kColSc + 16 * part + 8, far);
+                        float v[8];
 #pragma unroll
-                        for (int m = 0; m < 2; ++m) {
-                            const int j0 = 16 * part + 8 * m;
-                            uint64_t u[4];
-                            tmem_ld8(quad + kColSc + j0, u);
-                            float v[8];
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) {
-                                const int e0 = kRev ? j0 + 2 * j - i : i - j0 - 2 * j;
-                                const int e1 = kRev ? e0 + 1 : e0 - 1;
-                                unpair(u[j], v[2 * j], v[2 * j + 1]);
-                                v[2 * j] = e0 >= 0 ? v[2 * j] * M.decay[e0] : 0.f;
-                                v[2 * j + 1] = e1 >= 0 ? v[2 * j + 1] * M.decay[e1] : 0.f;
-                            }
-                            const uint32_t dst = base + L::kP + i * 128 + (((j0 >> 3) ^ i) & 7) * 16;
-                            split<kPs>(v, [&](int k, const uint32_t(&r)[4]) {
-                                st_shared(dst + k * kRows64, r[0], r[1], r[2], r[3]);
-                            });
+                        for (int j = 0; j < 4; ++j) {
+                            const uint64_t other = __shfl_sync(0xffffffffu, far[j], lane & 15);
+                            unpair(lane < 16 ? near[j] : other, v[2 * j], v[2 * j + 1]);
+                            const int e0 = kRev ? j0 + 2 * j - i : i - j0 - 2 * j;
+                            const int e1 = kRev ? e0 + 1 : e0 - 1;
+                            v[2 * j] = e0 >= 0 ? v[2 * j] * M.decay[e0] : 0.f;
+                            v[2 * j + 1] = e1 >= 0 ? v[2 * j + 1] * M.decay[e1] : 0.f;
                         }
+                        const uint32_t dst = base + L::kP + i * 128 + (((j0 >> 3) ^ i) & 7) * 16;
+                        split<kPs>(v, [&](int k, const uint32_t(&r)[4]) {
+                            st_shared(dst + k * kRows64, r[0], r[1], r[2], r[3]);
+                        });
                         arrive(&M.p_ready);
                     }
+                    put(L::kBw, vb, weighted, M.wt[len < kC]);
+                    arrive(&M.w_ready);
                     const Ab na = fetch(p.a, p.heads_a, ha, c + 1);
                     if (!(ok = warp_wait(&M.o_full, ph))) break;
                     tc_fence_after();
@@ -581,12 +596,9 @@ la_parts(const LaCore p, LaWork* work, const LaEntry* entries, float* scratch, b
                         if (here(p.out_f32)) outputs(static_cast<float*>(p.out) + at);
                         else outputs(static_cast<T*>(p.out) + at);
                     }
-                    {
-                        const Column nc = fetch_c(c + 1);
-                        put(L::kA, na);
-                        put_c(nc);
-                        vb = fetch(p.b, p.heads_b, hb, c + 1);
-                    }
+                    put(L::kA, na, as_read, nullptr);
+                    vb = fetch(p.b, p.heads_b, hb, c + 1);
+                    vc = fetch_c(c + 1);
                     if (!(ok = warp_wait(&M.u_full[0], ph))) break;
                     tc_fence_after();
                     add_update(kColU, len);
