@@ -327,12 +327,13 @@ la_parts(const LaCore p, LaWork* work, const LaEntry* entries, float* scratch, b
                     }
                 }
             }
-            // The next chunk's lines to L2, by the group's other warps: its loads come when
-            // registers are free for them.
-            for (int c = 0; !kStateOnly && warp > kWarps && ok && c + 1 < nch; ++c) {
-                if (!(ok = warp_wait(&M.sc_full, (n + c) & 1))) break;
+            // Lines to L2, by the group's other warps, two chunks ahead: the loads come in bursts,
+            // of every SM at about the same time, and HBM would not keep up with them.
+#pragma unroll 1
+            for (int c = 1; !kStateOnly && warp > kWarps && ok && c < nch; ++c) {
+                if (c > 1 && !(ok = warp_wait(&M.sc_full, (n + c - 2) & 1))) break;
                 constexpr int kLine = 128 / static_cast<int>(sizeof(T));
-                const int x0 = kRev ? nch - 2 - c : c + 1;
+                const int x0 = kRev ? nch - 1 - c : c;
                 const int64_t row = static_cast<int64_t>(it.start) + x0 * kC;
                 const int len = min(kC, it.len - x0 * kC);
                 auto lines = [&](const void* of, int heads, int d, int from, int width) {
@@ -533,6 +534,9 @@ la_parts(const LaCore p, LaWork* work, const LaEntry* entries, float* scratch, b
                     }
                     arrive(&M.s_ready);
                     put_c(kColC, vc);
+                    // (The next chunk's loads go out in the waits: all at once they took 4000
+                    // cycles of the L2's time.)
+                    const Ab na = fetch(p.a, p.heads_a, ha, c + 1);
                     {
                         // P: the scores' 64 rows are the first 16 lanes of every quarter; the others
                         // take half of their 16 columns. What the mask leaves, decayed.
@@ -561,7 +565,8 @@ la_parts(const LaCore p, LaWork* work, const LaEntry* entries, float* scratch, b
                     }
                     put(L::kBw, vb, weighted, M.wt[len < kC]);
                     arrive(&M.w_ready);
-                    const Ab na = fetch(p.a, p.heads_a, ha, c + 1);
+                    vb = fetch(p.b, p.heads_b, hb, c + 1);
+                    vc = fetch_c(c + 1);
                     if (!(ok = warp_wait(&M.o_full, ph))) break;
                     tc_fence_after();
                     {
@@ -597,8 +602,6 @@ la_parts(const LaCore p, LaWork* work, const LaEntry* entries, float* scratch, b
                         else outputs(static_cast<T*>(p.out) + at);
                     }
                     put(L::kA, na, as_read, nullptr);
-                    vb = fetch(p.b, p.heads_b, hb, c + 1);
-                    vc = fetch_c(c + 1);
                     if (!(ok = warp_wait(&M.u_full[0], ph))) break;
                     tc_fence_after();
                     add_update(kColU, len);
