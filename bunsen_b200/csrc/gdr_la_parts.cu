@@ -634,9 +634,9 @@ cudaError_t start(const LaCore& p, LaLists* shared, cudaStream_t stream) {
     auto* states = la_parts<T, kDb, kRev, true>;
     constexpr int kFull = static_cast<int>(Layout<T, kDb, false>::kBytes),
                   kStates = static_cast<int>(Layout<T, kDb, true>::kBytes);
-    cudaError_t e = cudaFuncSetAttribute(full, cudaFuncAttributeMaxDynamicSharedMemorySize, kFull);
-    if (e == cudaSuccess)
-        e = cudaFuncSetAttribute(states, cudaFuncAttributeMaxDynamicSharedMemorySize, kStates);
+    static std::atomic<uint64_t> full_done{0}, states_done{0};
+    cudaError_t e = la_allow_smem(full, kFull, full_done);
+    if (e == cudaSuccess) e = la_allow_smem(states, kStates, states_done);
     if (e != cudaSuccess) return e;
     const bool vec = p.d_b % 8 == 0 && ((reinterpret_cast<uintptr_t>(p.a) |
                                          reinterpret_cast<uintptr_t>(p.b)) & 15) == 0;

@@ -23,6 +23,32 @@ constexpr int64_t kStateBudget = int64_t{2} << 30;  // scratch states of a call,
 constexpr int kPlanThreads = 1024, kBuckets = 1024;
 constexpr float kLinkCost = 0.05f;  // of the scan, a link, in chunks of the main pass
 
+// The longest time of a CTA, in chunks, with sequences in segments of L chunks: `sum`
+// chunks altogether, the longest sequence `most` of them, `each` jobs a CTA for an
+// entry; of the sequences above L, `again` chunks go through the states' pass, `whole`
+// segments are whole (or nearly), one sequence has `parts` segments at most.
+__host__ __device__ inline float split_time(const LaSplitCost& how, float each, int L, int sum,
+                                            int most, int again, int whole, int parts) {
+    // A pass takes the work's share of a CTA, and at least the most whole segments
+    // that fall to one.
+    const float longest = static_cast<float>(L < most ? L : most);
+    float t = fmaxf(fmaxf(longest * ceilf(whole * each), sum * each * 1.03f + 1.f), longest);
+    if (again > 0)
+        t += how.state_cost * fmaxf(longest * ceilf(again * each / L), again * each * 1.03f) +
+             how.fixed_cost + kLinkCost * parts;
+    return t;
+}
+__host__ __device__ inline float whole_time(float each, int sum, int most) {
+    return fmaxf(static_cast<float>(most), sum * each * 1.03f + 1.f);
+}
+// The lengths that are tried: 32, from l_min to the longest sequence.
+__host__ __device__ inline int candidate_length(int i, int l_min, int most) {
+    const float range = fmaxf(1.f, static_cast<float>(most) / l_min);
+    const int L = static_cast<int>(l_min * powf(range, i / 31.f));
+    return L > l_min ? L : l_min;
+}
+constexpr float kWorthIt = 0.97f;  // of the time without segments
+
 // The block's sum (op 0) or maximum (op 1) of x.
 __device__ int block_reduce(int x, bool maximum, int* ws) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -69,11 +95,7 @@ la_plan(const LaCore p, LaPlan* plan, LaEntry* main, LaEntry* states, LaSplit* s
     most = block_reduce(most, true, ws);
     // Candidate lengths from l_min to the longest sequence, one a warp.
     const float each = static_cast<float>(p.heads) * blocks / grid;
-    auto candidate = [&](int i) {
-        return forced > 0 ? forced
-                          : max(l_min, static_cast<int>(l_min * powf(fmaxf(1.f, static_cast<float>(most) / l_min),
-                                                                     i / 31.f)));
-    };
+    auto candidate = [&](int i) { return forced > 0 ? forced : candidate_length(i, l_min, most); };
     {
         const int L = candidate(warp);
         int again = 0, parts_most = 0, segs = 0, whole = 0;  // whole: segments of L chunks
@@ -93,14 +115,7 @@ la_plan(const LaCore p, LaPlan* plan, LaEntry* main, LaEntry* states, LaSplit* s
             whole += __shfl_xor_sync(0xffffffffu, whole, o);
             parts_most = max(parts_most, __shfl_xor_sync(0xffffffffu, parts_most, o));
         }
-        // A pass takes the work's share of a CTA, and at least the most whole segments
-        // that fall to one.
-        const float longest = static_cast<float>(min(L, most));
-        float t = fmaxf(longest * ceilf(whole * each), sum * each * 1.03f + 1.f);
-        t = fmaxf(t, longest);
-        if (again > 0)
-            t += how.state_cost * fmaxf(longest * ceilf(again * each / L), again * each * 1.03f) +
-                 how.fixed_cost + kLinkCost * parts_most;
+        float t = split_time(how, each, L, sum, most, again, whole, parts_most);
         if (segs > seg_cap) t = INFINITY;
         if (lane == 0) cost[warp] = t;
     }
@@ -108,7 +123,7 @@ la_plan(const LaCore p, LaPlan* plan, LaEntry* main, LaEntry* states, LaSplit* s
     int L = most > 0 ? most : 1;  // not split
     if (seg_cap > 0) {
         float best = must || forced > 0 ? INFINITY
-                                        : 0.97f * fmaxf(static_cast<float>(most), sum * each * 1.03f + 1.f);
+                                        : kWorthIt * whole_time(each, sum, most);
         for (int i = 0; i < 32; ++i)
             if (cost[i] < best) {
                 best = cost[i];
@@ -240,8 +255,21 @@ cudaError_t la_prepare(const LaCore& p, int grid, int blocks, LaSplitCost o, boo
     const int64_t most = p.cu_seqlens ? tokens / kLaChunk + p.n_seqs : longest * p.n_seqs;
     const double each = static_cast<double>(most) * p.heads * blocks / grid;
     const int l_min = o.forced > 0 ? o.forced : std::max(2, static_cast<int>(each / 4));
-    const bool split = o.may && longest > l_min &&
-                       (o.must || longest > 2 * l_min + static_cast<int>(o.fixed_cost));
+    bool split = o.may && longest > l_min &&
+                 (o.must || longest > 2 * l_min + static_cast<int>(o.fixed_cost));
+    if (split && !o.must && o.forced == 0 && p.cu_seqlens == nullptr) {
+        // Dense lengths are known here.
+        const int c = static_cast<int>(longest), n = p.n_seqs;
+        const float per = static_cast<float>(p.heads) * blocks / grid;
+        float best = kWorthIt * whole_time(per, n * c, c);
+        split = false;
+        for (int i = 0; i < 32 && !split; ++i) {
+            const int L = candidate_length(i, l_min, c);
+            if (L >= c) continue;
+            const int parts = (c + L - 1) / L;
+            split = split_time(o, per, L, n * c, c, n * (parts - 1) * L, n * ((c + L / 3) / L), parts) < best;
+        }
+    }
     if (!split && static_cast<int64_t>(p.n_seqs) * p.heads * blocks <= grid) return cudaSuccess;
     const size_t size = sizeof(float) * p.heads * p.d_b * p.d_c;
     // A split sequence of c > L chunks has ceil(c / L) < 2 c / L segments.

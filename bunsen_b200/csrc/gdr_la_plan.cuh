@@ -2,6 +2,8 @@
 // segments of them, and the states between segments.
 #pragma once
 
+#include <atomic>
+
 #include "gdr_la.cuh"
 
 namespace gdr {
@@ -87,6 +89,18 @@ cudaError_t la_prepare(const LaCore& p, int grid, int blocks, LaSplitCost o, boo
 void la_scan_states(const LaCore& p, const LaLists& lists, cudaStream_t stream);
 cudaError_t la_release(const LaLists& lists, cudaStream_t stream);
 int la_sm_count();
+// A kernel's dynamic shared memory, allowed once a device (the call costs a launch's time).
+template <typename K>
+cudaError_t la_allow_smem(K* kernel, int bytes, std::atomic<uint64_t>& done) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    const uint64_t bit = dev < 64 ? uint64_t{1} << dev : 0;
+    if (done.load(std::memory_order_relaxed) & bit) return cudaSuccess;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+    return e;
+}
 // Two cores whose lists would be the same (jobs of 128 columns).
 inline bool la_same_lists(const LaCore& x, const LaCore& y) {
     return (x.d_c + 127) / 128 == (y.d_c + 127) / 128;

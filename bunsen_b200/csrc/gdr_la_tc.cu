@@ -994,11 +994,11 @@ cudaError_t launch_la_tc(const LaCore& p, bool split, bool must, int forced, cud
         return cudaErrorInvalidValue;
     auto* full = p.reverse ? la_tc<true, false> : la_tc<false, false>;
     auto* states = p.reverse ? la_tc<true, true> : la_tc<false, true>;
-    cudaError_t e;
-    for (auto* k : {full, states})
-        if ((e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                      static_cast<int>(kSmemBytes))) != cudaSuccess)
-            return e;
+    static std::atomic<uint64_t> done[2][2];
+    cudaError_t e = la_allow_smem(full, static_cast<int>(kSmemBytes), done[p.reverse != 0][0]);
+    if (e == cudaSuccess)
+        e = la_allow_smem(states, static_cast<int>(kSmemBytes), done[p.reverse != 0][1]);
+    if (e != cudaSuccess) return e;
     // A chunk takes 2.9 us at one CTA an SM, one of the states' pass 0.45 of that; that
     // pass's start, the list's kernel and the scan 11 chunks.
     const int sms = la_sm_count();
