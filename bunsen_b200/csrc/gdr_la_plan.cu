@@ -77,6 +77,7 @@ la_plan(const LaCore p, LaPlan* plan, LaEntry* main, LaEntry* states, LaSplit* s
     const bool must = how.must;
     __shared__ int ws[32], hist[kBuckets], slots, n_splits, n_states;
     __shared__ float cost[32];
+    __shared__ int counts[kPlanThreads];  // the first sequences' chunks
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     auto chunks = [&](int s, int64_t& start, int64_t& len) {
         int64_t end;
@@ -85,9 +86,15 @@ la_plan(const LaCore p, LaPlan* plan, LaEntry* main, LaEntry* states, LaSplit* s
         return static_cast<int>((len + kLaChunk - 1) / kLaChunk);
     };
     int64_t start, len;
+    auto count = [&](int s) {
+        if (s < kPlanThreads) return counts[s];
+        int64_t x, y;
+        return chunks(s, x, y);
+    };
     int sum = 0, most = 0;
     for (int s = tid; s < p.n_seqs; s += kPlanThreads) {
         const int c = chunks(s, start, len);
+        if (s < kPlanThreads) counts[s] = c;
         sum += c;
         most = max(most, c);
     }
@@ -100,7 +107,7 @@ la_plan(const LaCore p, LaPlan* plan, LaEntry* main, LaEntry* states, LaSplit* s
         const int L = candidate(warp);
         int again = 0, parts_most = 0, segs = 0, whole = 0;  // whole: segments of L chunks
         for (int s = lane; s < p.n_seqs; s += 32) {
-            const int c = chunks(s, start, len);
+            const int c = count(s);
             if (c > L) {
                 const int parts = (c + L - 1) / L;
                 again += (parts - 1) * L;
@@ -122,13 +129,18 @@ la_plan(const LaCore p, LaPlan* plan, LaEntry* main, LaEntry* states, LaSplit* s
     __syncthreads();
     int L = most > 0 ? most : 1;  // not split
     if (seg_cap > 0) {
-        float best = must || forced > 0 ? INFINITY
-                                        : kWorthIt * whole_time(each, sum, most);
-        for (int i = 0; i < 32; ++i)
-            if (cost[i] < best) {
-                best = cost[i];
-                L = candidate(i);
+        float t = cost[lane];
+        int best = lane;
+        for (int o = 16; o > 0; o >>= 1) {
+            const float u = __shfl_xor_sync(0xffffffffu, t, o);
+            const int other = __shfl_xor_sync(0xffffffffu, best, o);
+            if (u < t || (u == t && other < best)) {
+                t = u;
+                best = other;
             }
+        }
+        if (t < (must || forced > 0 ? INFINITY : kWorthIt * whole_time(each, sum, most)))
+            L = candidate(best);
     }
     const int shift = max(0, 32 - __clz(min(L, most)) - 10);  // bucket: chunks >> shift
     for (int i = tid; i < kBuckets; i += kPlanThreads) hist[i] = 0;
@@ -136,7 +148,7 @@ la_plan(const LaCore p, LaPlan* plan, LaEntry* main, LaEntry* states, LaSplit* s
     __syncthreads();
     auto bucket = [&](int c) { return kBuckets - 1 - (c >> shift); };  // longest first
     for (int s = tid; s < p.n_seqs; s += kPlanThreads) {
-        const int c = chunks(s, start, len);
+        const int c = count(s);
         int parts = c > L ? (c + L - 1) / L : 1, at = 0;
         if (parts > 1) at = atomicAdd(&slots, parts);
         base[s] = at;
@@ -164,23 +176,28 @@ la_plan(const LaCore p, LaPlan* plan, LaEntry* main, LaEntry* states, LaSplit* s
     hist[tid] = before + x - mine;
     __syncthreads();
     for (int s = tid; s < p.n_seqs; s += kPlanThreads) {
-        const int c = chunks(s, start, len);
-        const int parts = c > L ? (c + L - 1) / L : 1;
-        if (parts == 1) {
-            main[atomicAdd(&hist[bucket(c)], 1)] = {static_cast<int32_t>(start),
-                                                    static_cast<int32_t>(len), s, s};
-            continue;
-        }
-        splits[atomicAdd(&n_splits, 1)] = {base[s], parts, s, 0};
-        for (int r = 0; r < parts; ++r) {  // in the order of time
+        const int c = count(s);
+        if (c > L) continue;
+        chunks(s, start, len);
+        main[atomicAdd(&hist[bucket(c)], 1)] = {static_cast<int32_t>(start),
+                                                static_cast<int32_t>(len), s, s};
+    }
+    // Sequences in segments, a warp each.
+    for (int s = warp; s < p.n_seqs; s += kPlanThreads / 32) {
+        const int c = count(s);
+        if (c <= L) continue;
+        chunks(s, start, len);
+        const int parts = (c + L - 1) / L, at = base[s];
+        if (lane == 0) splits[atomicAdd(&n_splits, 1)] = {at, parts, s, 0};
+        for (int r = lane; r < parts; r += 32) {  // in the order of time
             const int part = p.reverse ? parts - 1 - r : r;
             const int from = part * L, n = min(L, c - from);
             const int32_t t0 = static_cast<int32_t>(start) + from * kLaChunk;
             const int32_t tokens = min(n * kLaChunk, static_cast<int32_t>(len) - from * kLaChunk);
-            main[atomicAdd(&hist[bucket(n)], 1)] = {t0, tokens, r == 0 ? s : -2 - (base[s] + r),
+            main[atomicAdd(&hist[bucket(n)], 1)] = {t0, tokens, r == 0 ? s : -2 - (at + r),
                                                     r == parts - 1 ? s : -1};
             if (r < parts - 1)
-                states[atomicAdd(&n_states, 1)] = {t0, tokens, -1, -2 - (base[s] + r + 1)};
+                states[atomicAdd(&n_states, 1)] = {t0, tokens, -1, -2 - (at + r + 1)};
         }
     }
     __syncthreads();
