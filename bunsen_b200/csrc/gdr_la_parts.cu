@@ -74,8 +74,9 @@ struct Misc {
     alignas(16) float ahead[2][kC];  // tau w^{i+1}, of a_i . S (backward w^{len-1-i})
     float2 f[2];                     // w^len, in two parts
     float decay[kC];                 // sigma w^0 .. w^{kC-1}
-    uint64_t ab_ready, s_ready, p_ready, w_ready, sc_full, o_full, u_full[2], drain;
+    uint64_t ab_ready, s_ready, p_ready, w_ready[2], sc_full, o_full, u_full[2], drain;
     uint32_t tmem;
+    uint32_t scored;  // chunks whose scores' product is issued
     int next;
 };
 static_assert(sizeof(Misc) <= 2048, "its room");
@@ -207,10 +208,12 @@ la_parts(const LaCore p, LaWork* work, const LaEntry* entries, float* scratch, b
     Misc& M = *reinterpret_cast<Misc*>(sm + L::kMisc);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) {
+        M.scored = 0;
         mbar_init(&M.ab_ready, kWarps);
         mbar_init(&M.s_ready, kWarps);
         mbar_init(&M.p_ready, kWarps);
-        mbar_init(&M.w_ready, kWarps);
+        mbar_init(&M.w_ready[0], kWarps);
+        mbar_init(&M.w_ready[1], kWarps);
         mbar_init(&M.sc_full, 1);
         mbar_init(&M.o_full, 1);
         mbar_init(&M.u_full[0], 1);
@@ -275,7 +278,7 @@ la_parts(const LaCore p, LaWork* work, const LaEntry* entries, float* scratch, b
             for (int c = 0; warp == kWarps && ok && c < nch; ++c) {
                 const uint32_t ph = (n + c) & 1, base = here(smem_u32(sm));
                 if constexpr (kStateOnly) {
-                    if (!(ok = warp_wait(&M.w_ready, ph))) break;
+                    if (!(ok = warp_wait(&M.w_ready[ph], ((n + c) >> 1) & 1))) break;
                     tc_fence_after();
                     if (elect_one()) {
                         update(base + ph * 3 * L::kTileAb, kColC + 96 * ph, 128 * ph);
@@ -291,6 +294,7 @@ la_parts(const LaCore p, LaWork* work, const LaEntry* entries, float* scratch, b
                                 sdesc_sw128(base + L::kB + j * L::kTileAb, 16, 1024), kScores, acc);
                         });
                         umma_commit(&M.sc_full);
+                        *const_cast<volatile uint32_t*>(&M.scored) = n + c + 1;
                     }
                     if (!(ok = warp_wait(&M.s_ready, ph))) break;
                     tc_fence_after();
@@ -319,7 +323,7 @@ la_parts(const LaCore p, LaWork* work, const LaEntry* entries, float* scratch, b
                         });
                         umma_commit(&M.o_full);
                     }
-                    if (!(ok = warp_wait(&M.w_ready, ph))) break;
+                    if (!(ok = warp_wait(&M.w_ready[0], ph))) break;
                     tc_fence_after();
                     if (elect_one()) {
                         update(base + L::kBw, kColC, kColU);
@@ -330,8 +334,14 @@ la_parts(const LaCore p, LaWork* work, const LaEntry* entries, float* scratch, b
             // Lines to L2, by the group's other warps, two chunks ahead: the loads come in bursts,
             // of every SM at about the same time, and HBM would not keep up with them.
 #pragma unroll 1
-            for (int c = 1; !kStateOnly && warp > kWarps && ok && c < nch; ++c) {
-                if (c > 1 && !(ok = warp_wait(&M.sc_full, (n + c - 2) & 1))) break;
+            for (int c = 1; !kStateOnly && warp > kWarps && c < nch; ++c) {
+                // (By a count, not by a phase: these warps may fall behind by more than
+                // one. Nothing hangs on them: they go on when the tries run out.)
+                for (int tries = 0; tries < 4096; ++tries) {
+                    if (static_cast<int32_t>(*const_cast<volatile uint32_t*>(&M.scored) - (n + c)) >= -1)
+                        break;
+                    __nanosleep(200);
+                }
                 constexpr int kLine = 128 / static_cast<int>(sizeof(T));
                 const int x0 = kRev ? nch - 1 - c : c;
                 const int64_t row = static_cast<int64_t>(it.start) + x0 * kC;
@@ -488,7 +498,9 @@ la_parts(const LaCore p, LaWork* work, const LaEntry* entries, float* scratch, b
                     const uint32_t ph = (n + c) & 1;
                     put(ph * 3 * L::kTileAb, vb, weighted, M.wt[len_of(c) < kC]);
                     put_c(kColC + 96 * ph, vc);
-                    arrive(&M.w_ready);
+                    // (By buffer: a warp may be a chunk ahead of another, and must not arrive
+                    // in its place.)
+                    arrive(&M.w_ready[ph]);
                     vb = fetch(p.b, p.heads_b, hb, c + 1);
                     vc = fetch_c(c + 1);
                     if (c > 0) {
@@ -564,7 +576,7 @@ la_parts(const LaCore p, LaWork* work, const LaEntry* entries, float* scratch, b
                         arrive(&M.p_ready);
                     }
                     put(L::kBw, vb, weighted, M.wt[len < kC]);
-                    arrive(&M.w_ready);
+                    arrive(&M.w_ready[0]);
                     vb = fetch(p.b, p.heads_b, hb, c + 1);
                     vc = fetch_c(c + 1);
                     if (!(ok = warp_wait(&M.o_full, ph))) break;

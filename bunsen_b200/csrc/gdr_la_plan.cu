@@ -67,6 +67,12 @@ __device__ int block_reduce(int x, bool maximum, int* ws) {
     return x;
 }
 
+// A state updated in place: the last segment writes what the first one reads, and may do
+// so first. The scan copies it, to the slot of segment 0.
+__device__ __forceinline__ bool in_place(const LaCore& p) {
+    return p.state_in != nullptr && p.state_in == p.state_out;
+}
+
 // The work lists: every sequence, or its segments, the longest first (by buckets of
 // chunk counts), and the first pass's segments. seg_cap: state slots; 0: no
 // splitting. forced: a given segment length.
@@ -194,7 +200,8 @@ la_plan(const LaCore p, LaPlan* plan, LaEntry* main, LaEntry* states, LaSplit* s
             const int from = part * L, n = min(L, c - from);
             const int32_t t0 = static_cast<int32_t>(start) + from * kLaChunk;
             const int32_t tokens = min(n * kLaChunk, static_cast<int32_t>(len) - from * kLaChunk);
-            main[atomicAdd(&hist[bucket(n)], 1)] = {t0, tokens, r == 0 ? s : -2 - (at + r),
+            main[atomicAdd(&hist[bucket(n)], 1)] = {t0, tokens,
+                                                    r == 0 && !in_place(p) ? s : -2 - (at + r),
                                                     r == parts - 1 ? s : -1};
             if (r < parts - 1)
                 states[atomicAdd(&n_states, 1)] = {t0, tokens, -1, -2 - (at + r + 1)};
@@ -232,8 +239,13 @@ la_scan(const LaCore p, const LaPlan* plan, const LaSplit* splits, float* scratc
         const float g = p.log_decay[h];
         const int last = static_cast<int>(end - start) - (sp.parts - 1) * plan->seg_tokens;
         const float w = la_power(g, plan->seg_tokens);
-        float* slot = scratch + (static_cast<int64_t>(sp.base + 1) * p.heads + h) * size + e;
         const int64_t step = static_cast<int64_t>(p.heads) * size;
+        float* slot = scratch + (static_cast<int64_t>(sp.base) * p.heads + h) * size + e;
+        if (in_place(p)) {
+#pragma unroll
+            for (int v = 0; v < kVec; ++v) slot[v] = x[v];
+        }
+        slot += step;
 #pragma unroll 4
         for (int r = 0; r < sp.parts - 1; ++r, slot += step) {
             const float f = p.reverse && r == 0 ? la_power(g, last) : w;

@@ -56,7 +56,7 @@ __device__ __forceinline__ LaState la_state(const LaCore& p, int x, int h, const
 }
 
 struct LaSplit {
-    int32_t base, parts, seq, unused;  // segment r's state: slot base + r, r >= 1
+    int32_t base, parts, seq, unused;  // segment r's state: slot base + r (r = 0: in place only)
 };
 struct LaPlan {
     LaWork main[2], states;  // (main: for either of two launches that share the lists)

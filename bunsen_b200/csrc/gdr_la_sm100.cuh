@@ -8,7 +8,7 @@
 namespace gdr {
 namespace sm100 {
 
-constexpr int kWaitRounds = 1 << 24;  // of two tries: seconds
+constexpr int kWaitRounds = 1 << 20;  // of two tries of a microsecond or less: two seconds
 
 // Waits for a phase; false once the tries ran out. A try suspends the warp for
 // some 90 cycles (one with a time of its own becomes a loop of sleeps).

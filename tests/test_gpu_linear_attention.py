@@ -491,3 +491,68 @@ def test_many_sequences_on_few_heads():
     x = make(lens, 1, 2, 128, 128, torch.bfloat16, seed=16)
     check_forward(x)
     check_backward(x)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", [(33, 65), (64, 64), (128, 128), (128, 200)])
+@pytest.mark.parametrize("packed", [True, False])
+def test_long_sequences_of_every_width(packed, shape, dtype):
+    """Long enough for segments in every kernel, with shared key heads."""
+    x = make([1700, 0, 700] if packed else [1300, 1300], 1, 2, *shape, dtype, seed=shape[1],
+             packed=packed)
+    check_forward(x)
+    check_backward(x)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("lens,hv", [([6000], 2), ([20000, 130], 16)])
+def test_segments_update_a_state_in_place(lens, hv, dtype):
+    """The first segment reads the state that the last one writes, which may run
+    first where the jobs are more than the CTAs."""
+    x = make(lens, 2, hv, 64, 64, dtype, seed=len(lens))
+    rule = LinearAttention(algo="auto")
+    args = (x["q"], x["k"], x["v"], x["g"])
+    want, s_want = rule.chunked(*args, x["state"], cu_seqlens=x["cu"])
+    for _ in range(3):
+        state = x["state"].clone()
+        out, _ = rule.chunked(*args, state, cu_seqlens=x["cu"], state_out=state)
+        assert torch.equal(out, want) and torch.equal(state, s_want)
+    assert _lib.load().gdr_device_error() == _lib.GDR_OK
+
+
+def test_calls_from_threads():
+    """Four host threads, each with its own stream, at once."""
+    import threading
+
+    xs = [make([900, 3, 400], 2, 4, 64, 64, dt, seed=i)
+          for i, dt in enumerate((torch.bfloat16, torch.float32, torch.float16, torch.bfloat16))]
+
+    def call(x):
+        rule = LinearAttention()
+        return [*rule.chunked(x["q"], x["k"], x["v"], x["g"], x["state"], cu_seqlens=x["cu"]),
+                *rule.backward(x["q"], x["k"], x["v"], x["g"], x["do"], x["state"], x["ds"],
+                               cu_seqlens=x["cu"])]
+
+    ref = [call(x) for x in xs]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(i):
+        try:
+            stream = torch.cuda.Stream()
+            with torch.cuda.stream(stream):
+                for _ in range(10):
+                    got = call(xs[i])
+                    stream.synchronize()
+                    if not all(torch.equal(u, v) for u, v in zip(got, ref[i])):
+                        bad.append(i)
+        except Exception as e:  # noqa: BLE001
+            bad.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
+    assert _lib.load().gdr_device_error() == _lib.GDR_OK
