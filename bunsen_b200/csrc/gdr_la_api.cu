@@ -108,10 +108,12 @@ Kernel kernel_of(const gdr_la_params& a, const LaCore& p, bool chunked) {
     if (!chunked || tokens == 0) return Kernel::recurrent;
     const bool tc = la_tc_supports(p);
     if (!tc && a.algo >= GDR_ALGO_TENSOR) return Kernel::none;
+    // A few positions step as fast as a chunk does, and exactly (a chunk's few scores,
+    // rounded to bf16, would be all of some outputs); the others go in chunks.
+    const bool few = tokens <= 16 || tokens <= 4 * static_cast<int64_t>(p.n_seqs);
+    if (few && a.algo < GDR_ALGO_TENSOR) return Kernel::recurrent;
     if (tc && a.algo != GDR_ALGO_CUDA_CORE) return Kernel::tensor;
-    // Short sequences step as fast as a chunk does; the others go in chunks.
-    return la_parts_supports(p) && tokens > 4 * static_cast<int64_t>(p.n_seqs) ? Kernel::parts
-                                                                               : Kernel::recurrent;
+    return la_parts_supports(p) ? Kernel::parts : Kernel::recurrent;
 }
 
 cudaError_t run_core(const gdr_la_params& a, const LaCore& p, bool chunked, cudaStream_t s,
