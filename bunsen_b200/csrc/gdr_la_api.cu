@@ -108,11 +108,14 @@ Kernel kernel_of(const gdr_la_params& a, const LaCore& p, bool chunked) {
     if (!chunked || tokens == 0) return Kernel::recurrent;
     const bool tc = la_tc_supports(p);
     if (!tc && a.algo >= GDR_ALGO_TENSOR) return Kernel::none;
-    // A few positions step as fast as a chunk does, and exactly (a chunk's few scores,
-    // rounded to bf16, would be all of some outputs); the others go in chunks.
+    // A few positions step as fast as a chunk does, and in f32 (rounded to bf16, a chunk's few
+    // scores would be most of some outputs); the others go in chunks.
     const bool few = tokens <= 16 || tokens <= 4 * static_cast<int64_t>(p.n_seqs);
     if (few && a.algo < GDR_ALGO_TENSOR) return Kernel::recurrent;
-    if (tc && a.algo != GDR_ALGO_CUDA_CORE) return Kernel::tensor;
+    // Nor does a prompt of a chunk or less gain from bf16 scores and states: 12 us in parts,
+    // 10 us with them, and half their error in the sums.
+    const bool exact = tokens <= 64 && a.algo == GDR_ALGO_AUTO && la_parts_supports(p);
+    if (tc && a.algo != GDR_ALGO_CUDA_CORE && !exact) return Kernel::tensor;
     return la_parts_supports(p) ? Kernel::parts : Kernel::recurrent;
 }
 

@@ -12,23 +12,32 @@
 // f32 ones; three tf32 products by mma.sync make 163, FFMA 117.
 //
 // One CTA an SM takes a (sequence or segment, head) and 128 columns of the state:
-//   16 warps convert: a and b to parts in shared memory, c and the weighted c to TMEM with
-//            the columns of c on the lanes, the state's copy to shared memory; they turn
-//            scores into P, write the outputs, and hold the state, 32 values a thread
+//   16 warps convert: a, b and the weighted b to parts in shared memory, c to TMEM with the
+//            columns of c on the lanes, the state's copy to TMEM (its third part to shared
+//            memory); they turn scores into P, write the outputs, and hold the
+//            state, 32 values a thread
 //   1 warp   issues the products
+//   3 warps  bring the lines of the chunk after the next to L2
 // The products of a chunk, N positions or rows of b on the columns of TMEM:
-//   scores = A B^T          128 x 64 (the lower 64 lanes are not read)
+//   scores = A B^T          64 x 64
 //   O1^T   = S^T A^T        128 x 64, the state's copy as the first operand
-//   O2^T   = C^T P^T        128 x 64
-//   U^T    = (w C)^T B      128 x d_b
+//   O2^T   = C^T P^T        128 x 64, over the scores
+//   U^T    = C^T (w B)      128 x d_b
 // c never is in shared memory: a thread reads one column of it, 16 positions,
 // neighbouring lanes neighbouring columns, and that is how TMEM wants it; outputs go out
-// the same way. What the next chunk needs is read from HBM into registers while
-// the products run; a and c are converted beside the update's product, b, w c and
-// the state's copy beside the scores'.
+// the same way. A product with both operands in shared memory reads 6 KiB of it in the 32
+// cycles of 128 x 64 x 16, half again what it delivers, so what can be comes from
+// TMEM (the state's copy wholly in shared memory: 221 us for 8192 packed positions and
+// 16 heads, against 194 us). A chunk's loads go out in the waits for the products, a early,
+// b and c late: all at once they wait for one another.
 //
-// TMEM (512 columns): scores 64, O1 64, O2 64, U 128, c three parts of 32, w c the same.
-// Bound by the tensor cores: 5400 cycles a chunk at f32 and 128 x 128, 3.1 us.
+// TMEM (512 columns): scores and O2 64, O1 64, U 128, c three parts of 32, the state's copy two
+// of 64.
+//
+// Bound: 5000 tensor cycles a chunk at f32 and 128 x 128, 2.9 us, where a chunk takes 5.8 us
+// (8192 packed positions, 16 heads, d = 128: 186 us; with mma.sync in three tf32 products and
+// shared memory alone 988 us): issue slots, 0.6 of them taken by conversions and the address
+// work around them, in a chain with the products.
 #include <cuda_fp16.h>
 
 #include <algorithm>

@@ -31,19 +31,27 @@
 // Two issuing warps, because a wait and a commit cost their thread 100 to 200
 // cycles each beside products that keep shared memory busy, 17 of them a
 // chunk; the state in registers rather than scaled in TMEM, because there the
-// next update waited for the scaling (4.0 us a chunk with one issuer and the
-// state in TMEM, TIMEUS so).
+// next update waited for the scaling (5.4 us a chunk with one issuer and the
+// state in TMEM, 3.7 us so).
 //
 // What is rounded: P and Sb to bf16 (2^-8 relative each, on disjoint parts of
 // an output, which is itself rounded to bf16: inputs are bf16, so another
-// half-step of theirs; f32 operands would halve the tensor rate for a third
-// less error). The state accumulates in f32 over every chunk, so its operand
-// is not rounded: w c goes in as three bf16 parts, 24 bits. Measured against
-// 64 bits: outputs 2.3e-3 (a bf16 rounding alone: 1.7e-3), states below 1e-6.
+// half-step of theirs; a second part of either would be a product more, 32 KiB of
+// shared memory that is not there, and a third less error). The state accumulates
+// in f32 over every chunk, so its operand is not rounded: w c goes in as three bf16
+// parts, 24 bits. Measured against 64 bits: outputs 2.3e-3 (a bf16 rounding alone:
+// 1.7e-3), states 3.2e-7.
 //
-// Bound: by HBM at 128 x (768 to 1024) bytes a chunk and head (q and k shared
-// or not), 2.2 to 3.0 us per SM at the measured copy rate, against 6 products of
-// 512 tensor cycles, 1.6 us.
+// Jobs come from a list, the longest first, handed out by a counter; long sequences
+// go in segments whose states a pass of their own finds (kStateOnly: loads, (w c)^T and
+// the update alone; gdr_la_plan.cu).
+//
+// Bound: HBM, at 128 x (768 to 1024) bytes a chunk and head (q and k shared or not),
+// 2.2 to 3.0 us per SM at the measured copy rate; six products are 3100 tensor cycles, 1.8 us;
+// shared memory moves 480 KiB a chunk, 3800 cycles. A chunk takes 3.7 us (131072
+// packed positions, 32 heads: 830 us, 4.2 TB/s, 0.64 of the copy rate): the chains between
+// the roles, 250 cycles from a commit to the waiting warp's next instruction, are what is
+// left. The states' pass takes 2 us a chunk.
 #include <cudaTypedefs.h>
 
 #include <algorithm>
@@ -310,150 +318,187 @@ la_tc(const LaCore p, const __grid_constant__ CUtensorMap ma,
 
     if (warp >= 24) {
         give_registers<40>();
-    if (warp == 24) {
-        // ---- loads -------------------------------------------------------------
-        {
-            uint32_t n = 0;
-            const int heads = p.heads;
-            const int jobs = work != nullptr ? work->count * heads : p.n_seqs * heads;
+        if (warp == 24) {
+            // ---- loads -------------------------------------------------------------
+            {
+                uint32_t n = 0;
+                const int heads = p.heads;
+                const int jobs = work != nullptr ? work->count * heads : p.n_seqs * heads;
 #pragma unroll 1
-            for (uint32_t k = 0; ok; ++k) {
-                const uint32_t slot = k % kJobs;
-                if (k >= kJobs && !(ok = warp_wait(&B.job_free[slot], (k / kJobs & 1) ^ 1))) break;
-                int id = k == 0 ? static_cast<int>(blockIdx.x) : jobs;
-                if (work != nullptr && k > 0) {
-                    if (lane == 0) id = atomicAdd(&work->next, 1);
-                    id = __shfl_sync(0xffffffffu, id, 0);
-                }
-                Job it{0, -1, 0, -1, -1};
-                if (id < jobs) {
-                    const int e = id / heads;
-                    it.h = id - e * heads;
-                    if (work != nullptr) {
-                        const LaEntry x = entries[e];
-                        it.start = x.start, it.len = x.len, it.in = x.in, it.out = x.out;
-                    } else {
-                        int64_t start, end;
-                        la_span(p, e, start, end);
-                        it.start = static_cast<int>(start);
-                        it.len = static_cast<int>(end - start);
-                        it.in = it.out = e;
+                for (uint32_t k = 0; ok; ++k) {
+                    const uint32_t slot = k % kJobs;
+                    if (k >= kJobs && !(ok = warp_wait(&B.job_free[slot], (k / kJobs & 1) ^ 1))) break;
+                    int id = k == 0 ? static_cast<int>(blockIdx.x) : jobs;
+                    if (work != nullptr && k > 0) {
+                        if (lane == 0) id = atomicAdd(&work->next, 1);
+                        id = __shfl_sync(0xffffffffu, id, 0);
                     }
-                }
-                if (lane == 0) {
-                    B.jobs[slot] = it;
-                    mbar_arrive(&B.job_full[slot]);
-                }
-                __syncwarp();
-                if (it.len < 0) break;
-                const int nch = (it.len + kC - 1) / kC;
-                const int ha = it.h / (p.heads / p.heads_a), hb = it.h / (p.heads / p.heads_b),
-                          hc = it.h / (p.heads / p.heads_c);
-#pragma unroll 1
-                for (int c = 0; ok && c < nch; ++c, ++n) {
-                    const int st = n & 1;
-                    const uint32_t ph = ((n >> 1) & 1) ^ 1;
-                    int64_t row;
-                    int len;
-                    chunk_of<kRev>(it, nch, c, row, len);
-                    const int r = static_cast<int>(row);
-                    uint8_t* base = sm + st * kStage;
-                    auto load = [&](uint64_t* full, uint8_t* dst, const CUtensorMap* map, int head) {
-                        if (elect_one()) {
-                            mbar_expect_tx(full, kTile);
-                            tma_load_3d(dst, map, full, 0, head, r);
-                            tma_load_3d(dst + kHalf, map, full, 64, head, r);
+                    Job it{0, -1, 0, -1, -1};
+                    if (id < jobs) {
+                        const int e = id / heads;
+                        it.h = id - e * heads;
+                        if (work != nullptr) {
+                            const LaEntry x = entries[e];
+                            it.start = x.start, it.len = x.len, it.in = x.in, it.out = x.out;
+                        } else {
+                            int64_t start, end;
+                            la_span(p, e, start, end);
+                            it.start = static_cast<int>(start);
+                            it.len = static_cast<int>(end - start);
+                            it.in = it.out = e;
                         }
-                    };
-                    // Chunk n - 2: its products with b and with c are done, its operand's
-                    // warps have read c, and its output has left the tiles.
-                    if (!kStateOnly && n >= 2 && !(ok = warp_wait(&B.in_full[st], ph))) break;
-                    if (n >= 2 && !(ok = warp_wait(&B.u_full[st], ph))) break;
-                    load(&B.b_full[st], base + kTile, &mb, hb);
-                    if (!kStateOnly && n >= 2) {
-                        if (p.out_f32 && !(ok = warp_wait(&B.a_free[st], ph))) break;
-                        if (!(ok = warp_wait(&B.o_full[st], ph))) break;
                     }
-                    if (n >= 2 && !(ok = warp_wait(&B.c_read[st], ph))) break;
-                    load(&B.c_full[st], base + 2 * kTile, &mc, hc);
-                    if (kStateOnly) continue;
-                    if (n >= 2 && !(ok = warp_wait(&B.a_free[st], ph))) break;
-                    load(&B.a_full[st], base, &ma, ha);
-                }
-            }
-            // Nothing of this CTA's may be in flight when it ends.
+                    if (lane == 0) {
+                        B.jobs[slot] = it;
+                        mbar_arrive(&B.job_full[slot]);
+                    }
+                    __syncwarp();
+                    if (it.len < 0) break;
+                    const int nch = (it.len + kC - 1) / kC;
+                    const int ha = it.h / (p.heads / p.heads_a), hb = it.h / (p.heads / p.heads_b),
+                              hc = it.h / (p.heads / p.heads_c);
 #pragma unroll 1
-            for (uint32_t i = n >= 2 ? n - 2 : 0; i < n + (ok ? 0 : 1); ++i)
-                for (uint64_t* full : {B.b_full, B.c_full, kStateOnly ? B.b_full : B.a_full})
-                    warp_wait(&full[i & 1], (i >> 1) & 1);
-        }
-        __syncwarp();
-    } else if (!kStateOnly && warp == 25) {
-        // ---- the outputs' products -------------------------------------------------
-        {
-            constexpr uint32_t kKK = idesc_bf16(128, 128, 0, 0, 0);
-            constexpr uint32_t kKMn = idesc_bf16(128, 128, 0, 1, 0);
-            const uint32_t base = smem_u32(sm);
-            auto from_a = [&](uint32_t st, uint32_t d, uint32_t b_tile) {
-                product_ss(tm + d, sdesc_sw128(base + st * kStage, 16, 1024),
-                           sdesc_sw128(b_tile, 16, 1024), kKK);
-            };
-            auto from_p = [&](uint32_t st) {
-                product_ts(tm + kColO, tm + kColP,
-                           sdesc_sw128(base + st * kStage + 2 * kTile, kHalf, 1024), kKMn);
-            };
-            uint32_t n = 0, tails = 0;
-#pragma unroll 1
-            for (uint32_t k = 0; ok; ++k) {
-                if (!(ok = warp_wait(&B.job_full[k % kJobs], k / kJobs & 1))) break;
-                const Job it = take(k % kJobs);
-                if (it.len < 0) break;
-                const int nch = (it.len + kC - 1) / kC;
-#pragma unroll 1
-                for (int c = 0; c < nch; ++c, ++n) {
-                    const uint32_t st = n & 1, ph = n & 1;
-                    if (!(ok = warp_wait(&B.b_full[st], (n >> 1) & 1))) break;
-                    if (!(ok = warp_wait(&B.a_full[st], (n >> 1) & 1))) break;
-                    if (chunk_len<kRev>(it, nch, c) < kC) {  // (by stage: bits of `tails`)
-                        if (!(ok = warp_wait(&B.fix[st], (tails >> st) & 1))) break;
-                        tails ^= 1u << st;
-                    }
-                    tc_fence_after();
-                    if (elect_one()) {
-                        from_a(st, kColP, base + st * kStage + kTile);
-                        umma_commit(&B.sc_full);
-                    }
-                    if (!(ok = warp_wait(&B.sb_ready, ph))) break;
-                    if (n > 0 && !(ok = warp_wait(&B.o_free, ph ^ 1))) break;
-                    tc_fence_after();
-                    if (elect_one()) {
-                        from_a(st, kColO, base + kOffSb);
-                        umma_commit(&B.in_full[st]);
-                    }
-                    // (P is written, and the c tile is there: its warps waited for it.)
-                    if (!(ok = warp_wait(&B.pa_ready, ph))) break;
-                    tc_fence_after();
-                    if (elect_one()) {
-                        from_p(st);
-                        umma_commit(&B.o_full[st]);
+                    for (int c = 0; ok && c < nch; ++c, ++n) {
+                        const int st = n & 1;
+                        const uint32_t ph = ((n >> 1) & 1) ^ 1;
+                        int64_t row;
+                        int len;
+                        chunk_of<kRev>(it, nch, c, row, len);
+                        const int r = static_cast<int>(row);
+                        uint8_t* base = sm + st * kStage;
+                        auto load = [&](uint64_t* full, uint8_t* dst, const CUtensorMap* map,
+                                        int head) {
+                            if (elect_one()) {
+                                mbar_expect_tx(full, kTile);
+                                tma_load_3d(dst, map, full, 0, head, r);
+                                tma_load_3d(dst + kHalf, map, full, 64, head, r);
+                            }
+                        };
+                        // Chunk n - 2: its products with b and with c are done, its operand's
+                        // warps have read c, and its output has left the tiles.
+                        if (!kStateOnly && n >= 2 && !(ok = warp_wait(&B.in_full[st], ph))) break;
+                        if (n >= 2 && !(ok = warp_wait(&B.u_full[st], ph))) break;
+                        load(&B.b_full[st], base + kTile, &mb, hb);
+                        if (!kStateOnly && n >= 2) {
+                            if (p.out_f32 && !(ok = warp_wait(&B.a_free[st], ph))) break;
+                            if (!(ok = warp_wait(&B.o_full[st], ph))) break;
+                        }
+                        if (n >= 2 && !(ok = warp_wait(&B.c_read[st], ph))) break;
+                        load(&B.c_full[st], base + 2 * kTile, &mc, hc);
+                        if (kStateOnly) continue;
+                        if (n >= 2 && !(ok = warp_wait(&B.a_free[st], ph))) break;
+                        load(&B.a_full[st], base, &ma, ha);
                     }
                 }
+                // Nothing of this CTA's may be in flight when it ends.
+#pragma unroll 1
+                for (uint32_t i = n >= 2 ? n - 2 : 0; i < n + (ok ? 0 : 1); ++i)
+                    for (uint64_t* full : {B.b_full, B.c_full, kStateOnly ? B.b_full : B.a_full})
+                        warp_wait(&full[i & 1], (i >> 1) & 1);
             }
-            if (elect_one()) umma_commit(&B.drain[0]);
-            warp_wait(&B.drain[0], 0);
-        }
-        __syncwarp();
-    } else if (warp == 26) {
-        // ---- the update's products -------------------------------------------------
-        {
-            constexpr uint32_t kKMn = idesc_bf16(128, 128, 0, 1, 0);
-            const uint32_t base = smem_u32(sm);
-            auto update = [&](uint32_t st, uint32_t q, uint32_t buf) {  // 32 positions
-                product_ts3(tm + kColU, tm + kColW + buf * kColWBuf,
-                            sdesc_sw128(base + st * kStage + kTile + q * 4096, kHalf, 1024), kKMn,
-                            q);
-            };
-            uint32_t n = 0, w = 0, tails = 0;
+            __syncwarp();
+        } else if (!kStateOnly && warp == 25) {
+            // ---- the outputs' products -------------------------------------------------
+            {
+                constexpr uint32_t kKK = idesc_bf16(128, 128, 0, 0, 0);
+                constexpr uint32_t kKMn = idesc_bf16(128, 128, 0, 1, 0);
+                const uint32_t base = smem_u32(sm);
+                auto from_a = [&](uint32_t st, uint32_t d, uint32_t b_tile) {
+                    product_ss(tm + d, sdesc_sw128(base + st * kStage, 16, 1024),
+                               sdesc_sw128(b_tile, 16, 1024), kKK);
+                };
+                auto from_p = [&](uint32_t st) {
+                    product_ts(tm + kColO, tm + kColP,
+                               sdesc_sw128(base + st * kStage + 2 * kTile, kHalf, 1024), kKMn);
+                };
+                uint32_t n = 0, tails = 0;
+#pragma unroll 1
+                for (uint32_t k = 0; ok; ++k) {
+                    if (!(ok = warp_wait(&B.job_full[k % kJobs], k / kJobs & 1))) break;
+                    const Job it = take(k % kJobs);
+                    if (it.len < 0) break;
+                    const int nch = (it.len + kC - 1) / kC;
+#pragma unroll 1
+                    for (int c = 0; c < nch; ++c, ++n) {
+                        const uint32_t st = n & 1, ph = n & 1;
+                        if (!(ok = warp_wait(&B.b_full[st], (n >> 1) & 1))) break;
+                        if (!(ok = warp_wait(&B.a_full[st], (n >> 1) & 1))) break;
+                        if (chunk_len<kRev>(it, nch, c) < kC) {  // (by stage: bits of `tails`)
+                            if (!(ok = warp_wait(&B.fix[st], (tails >> st) & 1))) break;
+                            tails ^= 1u << st;
+                        }
+                        tc_fence_after();
+                        if (elect_one()) {
+                            from_a(st, kColP, base + st * kStage + kTile);
+                            umma_commit(&B.sc_full);
+                        }
+                        if (!(ok = warp_wait(&B.sb_ready, ph))) break;
+                        if (n > 0 && !(ok = warp_wait(&B.o_free, ph ^ 1))) break;
+                        tc_fence_after();
+                        if (elect_one()) {
+                            from_a(st, kColO, base + kOffSb);
+                            umma_commit(&B.in_full[st]);
+                        }
+                        // (P is written, and the c tile is there: its warps waited for it.)
+                        if (!(ok = warp_wait(&B.pa_ready, ph))) break;
+                        tc_fence_after();
+                        if (elect_one()) {
+                            from_p(st);
+                            umma_commit(&B.o_full[st]);
+                        }
+                    }
+                }
+                if (elect_one()) umma_commit(&B.drain[0]);
+                warp_wait(&B.drain[0], 0);
+            }
+            __syncwarp();
+        } else if (warp == 26) {
+            // ---- the update's products -------------------------------------------------
+            {
+                constexpr uint32_t kKMn = idesc_bf16(128, 128, 0, 1, 0);
+                const uint32_t base = smem_u32(sm);
+                auto update = [&](uint32_t st, uint32_t q, uint32_t buf) {  // 32 positions
+                    product_ts3(tm + kColU, tm + kColW + buf * kColWBuf,
+                                sdesc_sw128(base + st * kStage + kTile + q * 4096, kHalf, 1024), kKMn,
+                                q);
+                };
+                uint32_t n = 0, w = 0, tails = 0;
+#pragma unroll 1
+                for (uint32_t k = 0; ok; ++k) {
+                    if (!(ok = warp_wait(&B.job_full[k % kJobs], k / kJobs & 1))) break;
+                    const Job it = take(k % kJobs);
+                    if (it.len < 0) break;
+                    const int nch = (it.len + kC - 1) / kC;
+#pragma unroll 1
+                    for (int c = 0; c < nch; ++c, ++n) {
+                        const uint32_t st = n & 1;
+                        if (!(ok = warp_wait(&B.b_full[st], (n >> 1) & 1))) break;
+                        if (chunk_len<kRev>(it, nch, c) < kC) {  // (by stage: bits of `tails`)
+                            if (!(ok = warp_wait(&B.fix[st], (tails >> st) & 1))) break;
+                            tails ^= 1u << st;
+                        }
+                        if (n > 0 && !(ok = warp_wait(&B.u_free, (n & 1) ^ 1))) break;
+#pragma unroll 1
+                        for (uint32_t q = 0; q < 4; ++q, ++w) {
+                            const uint32_t buf = w % kRing;
+                            if (!(ok = warp_wait(&B.wv_full[buf], w / kRing & 1))) break;
+                            tc_fence_after();
+                            if (elect_one()) {
+                                update(st, q, buf);
+                                umma_commit(&B.wv_free[buf]);
+                                if (q == 3) umma_commit(&B.u_full[st]);
+                            }
+                        }
+                        if (!ok) break;
+                    }
+                }
+                if (elect_one()) umma_commit(&B.drain[1]);
+                warp_wait(&B.drain[1], 0);
+            }
+            __syncwarp();
+        } else if (!kStateOnly && warp == 27) {
+            // ---- the outputs' stores -----------------------------------------------------
+            uint32_t n = 0;
 #pragma unroll 1
             for (uint32_t k = 0; ok; ++k) {
                 if (!(ok = warp_wait(&B.job_full[k % kJobs], k / kJobs & 1))) break;
@@ -463,80 +508,44 @@ la_tc(const LaCore p, const __grid_constant__ CUtensorMap ma,
 #pragma unroll 1
                 for (int c = 0; c < nch; ++c, ++n) {
                     const uint32_t st = n & 1;
-                    if (!(ok = warp_wait(&B.b_full[st], (n >> 1) & 1))) break;
-                    if (chunk_len<kRev>(it, nch, c) < kC) {  // (by stage: bits of `tails`)
-                        if (!(ok = warp_wait(&B.fix[st], (tails >> st) & 1))) break;
-                        tails ^= 1u << st;
-                    }
-                    if (n > 0 && !(ok = warp_wait(&B.u_free, (n & 1) ^ 1))) break;
+                    int64_t row;
+                    int len;
+                    chunk_of<kRev>(it, nch, c, row, len);
+                    if (!(ok = lane_wait(&B.o_staged[st], (n >> 1) & 1))) break;
+                    uint8_t* tile = sm + st * kStage;
+                    // Boxes of 32 positions, 128 bytes of features each; the last rows one
+                    // by one: behind them another sequence's stay as they are.
+                    const int whole = len & ~31, boxes = p.out_f32 ? 4 : 2, width = p.out_f32 ? 32 : 64;
+                    if (lane == 0) {
 #pragma unroll 1
-                    for (uint32_t q = 0; q < 4; ++q, ++w) {
-                        const uint32_t buf = w % kRing;
-                        if (!(ok = warp_wait(&B.wv_full[buf], w / kRing & 1))) break;
-                        tc_fence_after();
-                        if (elect_one()) {
-                            update(st, q, buf);
-                            umma_commit(&B.wv_free[buf]);
-                            if (q == 3) umma_commit(&B.u_full[st]);
-                        }
+                        for (int x = 0; x < boxes && x * width < p.d_c; ++x)
+#pragma unroll 1
+                            for (int r = 0; r < whole; r += 32)
+                                tma_store_3d(&mo, staged(tile, x) + r * 128, x * width, it.h,
+                                             static_cast<int>(row) + r);
+                        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
                     }
-                    if (!ok) break;
+                    const int piece = p.out_f32 ? 4 : 8;  // features in 16 bytes
+                    uint8_t* out = static_cast<uint8_t*>(p.out);
+#pragma unroll 1
+                    for (int r = whole; r < len; ++r) {
+                        const int64_t at = ((row + r) * p.heads + it.h) * p.d_c + lane * piece;
+                        if (lane * piece < p.d_c)
+                            *reinterpret_cast<uint4*>(out + at * (16 / piece)) =
+                                *reinterpret_cast<const uint4*>(staged(tile, lane >> 3) + r * 128 +
+                                                                (((lane & 7) ^ (r & 7)) << 4));
+                    }
+                    fence_proxy_async();  // the tile's next writer is the async proxy
+                    __syncwarp();
+                    if (lane == 0) {
+                        asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+                        mbar_arrive(&B.a_free[st]);
+                    }
                 }
             }
-            if (elect_one()) umma_commit(&B.drain[1]);
-            warp_wait(&B.drain[1], 0);
+            if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+            __syncwarp();
         }
-        __syncwarp();
-    } else if (!kStateOnly && warp == 27) {
-        // ---- the outputs' stores -----------------------------------------------------
-        uint32_t n = 0;
-#pragma unroll 1
-        for (uint32_t k = 0; ok; ++k) {
-            if (!(ok = warp_wait(&B.job_full[k % kJobs], k / kJobs & 1))) break;
-            const Job it = take(k % kJobs);
-            if (it.len < 0) break;
-            const int nch = (it.len + kC - 1) / kC;
-#pragma unroll 1
-            for (int c = 0; c < nch; ++c, ++n) {
-                const uint32_t st = n & 1;
-                int64_t row;
-                int len;
-                chunk_of<kRev>(it, nch, c, row, len);
-                if (!(ok = lane_wait(&B.o_staged[st], (n >> 1) & 1))) break;
-                uint8_t* tile = sm + st * kStage;
-                // Boxes of 32 positions, 128 bytes of features each; the last rows one
-                // by one: behind them another sequence's stay as they are.
-                const int whole = len & ~31, boxes = p.out_f32 ? 4 : 2, width = p.out_f32 ? 32 : 64;
-                if (lane == 0) {
-#pragma unroll 1
-                    for (int x = 0; x < boxes && x * width < p.d_c; ++x)
-#pragma unroll 1
-                        for (int r = 0; r < whole; r += 32)
-                            tma_store_3d(&mo, staged(tile, x) + r * 128, x * width, it.h,
-                                         static_cast<int>(row) + r);
-                    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-                }
-                const int piece = p.out_f32 ? 4 : 8;  // features in 16 bytes
-                uint8_t* out = static_cast<uint8_t*>(p.out);
-#pragma unroll 1
-                for (int r = whole; r < len; ++r) {
-                    const int64_t at = ((row + r) * p.heads + it.h) * p.d_c + lane * piece;
-                    if (lane * piece < p.d_c)
-                        *reinterpret_cast<uint4*>(out + at * (16 / piece)) =
-                            *reinterpret_cast<const uint4*>(staged(tile, lane >> 3) + r * 128 +
-                                                            (((lane & 7) ^ (r & 7)) << 4));
-                }
-                fence_proxy_async();  // the tile's next writer is the async proxy
-                __syncwarp();
-                if (lane == 0) {
-                    asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-                    mbar_arrive(&B.a_free[st]);
-                }
-            }
-        }
-        if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
-        __syncwarp();
-    }
     } else if (warp < 8) {
         if constexpr (kStateOnly) give_registers<24>();
         // ---- scores and outputs -------------------------------------------------------
@@ -597,49 +606,49 @@ la_tc(const LaCore p, const __grid_constant__ CUtensorMap ma,
 #pragma unroll 1
                 for (int cb = first; cb < last; ++cb) {
 #pragma unroll
-                for (int hb = 0; hb < 2; ++hb) {  // half blocks: 16 scores a thread
-                    const int x = cb & 1;
-                    const bool diag = cb == quarter;
-                    uint64_t s[8];
-                    tmem_ld16(pcol + 32 * x + 16 * hb, s);
-                    uint32_t packed[8];
-                    // The powers run from the larger exponents' side of either half.
-                    const bool far = kRev ? hb == 1 : hb == 0;
-                    const int me = lane - 16 * hb;  // this row's column in the half, if diag
-                    if (gentle || !diag) {
-                        float f = x == 0 ? fb[0] : fb[1];
-                        if (far) f *= w16;
-                        uint64_t f2 = kRev ? pair(f, f * w) : pair(f * w, f);
+                    for (int hb = 0; hb < 2; ++hb) {  // half blocks: 16 scores a thread
+                        const int x = cb & 1;
+                        const bool diag = cb == quarter;
+                        uint64_t s[8];
+                        tmem_ld16(pcol + 32 * x + 16 * hb, s);
+                        uint32_t packed[8];
+                        // The powers run from the larger exponents' side of either half.
+                        const bool far = kRev ? hb == 1 : hb == 0;
+                        const int me = lane - 16 * hb;  // this row's column in the half, if diag
+                        if (gentle || !diag) {
+                            float f = x == 0 ? fb[0] : fb[1];
+                            if (far) f *= w16;
+                            uint64_t f2 = kRev ? pair(f, f * w) : pair(f * w, f);
 #pragma unroll
-                        for (int t = 0; t < 8; ++t) {
-                            const int j = kRev ? t : 7 - t;
-                            packed[j] = pack_bf16(mul2(s[j], f2));
-                            f2 = mul2(f2, step);
-                        }
-                    } else {
-                        float f = far ? steep : p.sigma * p.tau;
+                            for (int t = 0; t < 8; ++t) {
+                                const int j = kRev ? t : 7 - t;
+                                packed[j] = pack_bf16(mul2(s[j], f2));
+                                f2 = mul2(f2, step);
+                            }
+                        } else {
+                            float f = far ? steep : p.sigma * p.tau;
 #pragma unroll
-                        for (int t = 0; t < 8; ++t) {
-                            const int j = kRev ? t : 7 - t;
-                            float u, v;
-                            unpair(s[j], u, v);
-                            (kRev ? u : v) *= f;
-                            if (kRev ? 2 * j >= me : 2 * j + 1 <= me) f *= w;
-                            (kRev ? v : u) *= f;
-                            if (kRev ? 2 * j + 1 >= me : 2 * j <= me) f *= w;
-                            packed[j] = pack_bf16(u, v);
+                            for (int t = 0; t < 8; ++t) {
+                                const int j = kRev ? t : 7 - t;
+                                float u, v;
+                                unpair(s[j], u, v);
+                                (kRev ? u : v) *= f;
+                                if (kRev ? 2 * j >= me : 2 * j + 1 <= me) f *= w;
+                                (kRev ? v : u) *= f;
+                                if (kRev ? 2 * j + 1 >= me : 2 * j <= me) f *= w;
+                                packed[j] = pack_bf16(u, v);
+                            }
                         }
+                        if (diag) {  // j <= i, or j >= i
+                            const int edge16 = 16 * (kRev ? me : me + 1);  // bits kept, or not
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) {
+                                const uint32_t low = low_bits(max(edge16 - 32 * j, 0));
+                                packed[j] &= kRev ? ~low : low;
+                            }
+                        }
+                        tmem_st8(pcol + 16 * x + 8 * hb, packed);
                     }
-                    if (diag) {  // j <= i, or j >= i
-                        const int edge16 = 16 * (kRev ? me : me + 1);  // bits of the pairs kept, or not
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) {
-                            const uint32_t low = low_bits(max(edge16 - 32 * j, 0));
-                            packed[j] &= kRev ? ~low : low;
-                        }
-                    }
-                    tmem_st8(pcol + 16 * x + 8 * hb, packed);
-                }
                 }
                 uint32_t zero[16];
 #pragma unroll

@@ -316,7 +316,13 @@ gdr_status gdr_mixed_noalloc(const gdr_params* params, const void* q, const void
  * infinity: a position sees only itself), a constant without a gradient.
  * dtypes f32, bf16 and f16; d_k and d_v up to 256 (else
  * GDR_ERR_UNSUPPORTED). A sequence of length 0 passes its state through;
- * positions behind the last sequence are neither read nor written. */
+ * positions behind the last sequence are neither read nor written. No output
+ * may overlap an input, but `state_out` may be `state_in`.
+ *
+ * GDR_ALGO_AUTO takes the kernel: positions one by one where there are few, chunks with
+ * bf16 scores and state operands for bf16 prompts (GDR_ALGO_TENSOR: not in segments,
+ * GDR_ALGO_TENSOR_SPLIT: in segments), chunks at f32 accuracy for the rest
+ * (GDR_ALGO_CUDA_CORE: these or one by one, whatever the type). */
 typedef struct gdr_la_params {
     int32_t batch;        /* B of a dense batch; ignored when cu_seqlens != NULL */
     int32_t seq_len;      /* T of a dense batch, or T_total of a packed one      */
