@@ -16,7 +16,7 @@
 // the row's sums by shuffles inside its lanes; products by f32 pairs. (With 8
 // consecutive features a lane, partners by shuffle and single products it was
 // bound by instructions: 165 us for 32768 x 32 heads of 128, against 102 us, 5.4 TB/s,
-// 0.83 of the copy rate; the gradient of 16384 x 32 heads 230 us against 109 us, 3.8 TB/s.)
+// 0.83 of the copy rate; the gradient of 16384 x 32 heads 230 us against 98 us, 4.2 TB/s.)
 // A warp takes kRows rows of one token per lane group, all of their loads issued before
 // any is computed; the token's angles are read once for them. Other shapes (odd
 // widths, unaligned rows) take one warp per row, scalar accesses.
@@ -168,7 +168,7 @@ __device__ __forceinline__ void block_weights(const NormRope& p, float (*acc)[kM
 // `q_warps` of all warps work on q. Rows past the last head are the last again,
 // not stored.
 template <typename T, int G, int kRows, bool kInter, bool kGrad>
-__global__ void __launch_bounds__(kThreads, kGrad ? 3 : 4)
+__global__ void __launch_bounds__(kThreads, kGrad ? 2 : 4)
 norm_rope_vec(const NormRope p, uint32_t q_warps, float* part) {
     constexpr int kSub = 32 / G, kPer = kSub * kRows;
     __shared__ float acc[kGrad ? 2 * kWarps : 1][kMaxD];
@@ -194,8 +194,12 @@ norm_rope_vec(const NormRope p, uint32_t q_warps, float* part) {
     for (int j = 0; j < 4; ++j) wt[j] = pair(1.f, 1.f), wsum[j] = 0;
     if (weight != nullptr) load_pairs(weight, o0, o1, wt);
     const float inv_d = 1.f / p.d;
+    const uint32_t first = is_k ? me - q_warps : me;
+    // The gradient's CTAs are few and stay (their weights' sums): a unit ahead they read
+    // its position, which the angles' loads wait for. (Its rows too: 113 us against 98.)
+    int next = kGrad && first < units ? p.positions[first / each] : 0;
 #pragma unroll 1
-    for (uint32_t u = is_k ? me - q_warps : me; u < units; u += step) {
+    for (uint32_t u = first; u < units; u += step) {
         const uint32_t token = u / each;
         const int head0 = static_cast<int>(u - token * each) * kPer + sub;
         const T* row = x + token * token_stride;
@@ -207,7 +211,8 @@ norm_rope_vec(const NormRope p, uint32_t q_warps, float* part) {
             rx[i] = load_raw(row + h * head_stride, o0, o1);
             if constexpr (kGrad) rd[i] = load_raw(dy + (flat + h) * p.d, o0, o1);
         }
-        const int pos = p.positions[token];
+        const int pos = kGrad ? next : p.positions[token];
+        if (kGrad && u + step < units) next = p.positions[(u + step) / each];
         if (!in_tables(p, pos)) {
             report_position();
             continue;
@@ -376,7 +381,7 @@ sum_weights(const float* part, int blocks, int d, float* dq_weight, float* dk_we
 
 // Accesses of four features need these; else the scalar kernel.
 bool vectors(const NormRope& p) {
-        if (p.d % 8 || p.rot % 8) return false;
+    if (p.d % 8 || p.rot % 8) return false;
     if (p.q_token % 4 || p.q_head % 4 || p.k_token % 4 || p.k_head % 4) return false;
     uintptr_t a = 0;
     for (const void* x : {p.q, p.k, static_cast<const void*>(p.q_out),
@@ -401,11 +406,12 @@ int sm_count() {
     return n > 0 ? n : 148;
 }
 
-// Rows a lane group takes at once: four, or in the gradient (two tensors' rows, and
-// the next unit's) two; one where that leaves SMs without work.
 int lanes_of(const NormRope& p) { return p.d <= 64 ? 8 : p.d <= 128 ? 16 : 32; }
+// Rows a lane group takes at once: four (the gradient's at 128 registers a thread, two CTAs
+// an SM: 98 us where three CTAs, two rows and 80 registers, which spilled, took 118); one
+// where that leaves SMs without work.
 int rows_of(const NormRope& p) {
-    const int rows = p.dq_out != nullptr ? 2 : 4;
+    constexpr int rows = 4;
     const int64_t units = p.tokens * (p.heads_q + p.heads_k) / (32 / lanes_of(p) * rows);
     return units < 2 * kWarps * sm_count() ? 1 : rows;
 }
@@ -414,7 +420,7 @@ Launch launch_of(const NormRope& p) {
     const int64_t rows = p.tokens * (p.heads_q + p.heads_k);
     const int per = vectors(p) ? 32 / lanes_of(p) * rows_of(p) : 1;
     const int64_t want = (rows / per + kWarps) / kWarps;
-    const int64_t most = static_cast<int64_t>(sm_count()) * (p.dq_out != nullptr ? 3 : kWaves * 4);
+    const int64_t most = static_cast<int64_t>(sm_count()) * (p.dq_out != nullptr ? 2 : kWaves * 4);
     Launch l;
     l.blocks = static_cast<int>(want < 1 ? 1 : want < most ? want : most);
     const int64_t warps = static_cast<int64_t>(l.blocks) * kWarps;
@@ -427,7 +433,7 @@ template <typename T, int G, bool kInter>
 void start_rows(const NormRope& p, float* part, Launch l, cudaStream_t s) {
     const bool one = rows_of(p) == 1;
     if (p.dq_out != nullptr)
-        (one ? norm_rope_vec<T, G, 1, kInter, true> : norm_rope_vec<T, G, 2, kInter, true>)
+        (one ? norm_rope_vec<T, G, 1, kInter, true> : norm_rope_vec<T, G, 4, kInter, true>)
             <<<l.blocks, kThreads, 0, s>>>(p, l.q_warps, part);
     else
         (one ? norm_rope_vec<T, G, 1, kInter, false> : norm_rope_vec<T, G, 4, kInter, false>)
