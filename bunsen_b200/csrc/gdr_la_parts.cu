@@ -235,6 +235,7 @@ la_parts(const LaCore p, LaWork* work, const LaEntry* entries, float* scratch, b
         tmem_relinquish();
     }
     tc_fence_before();
+    after_last_kernel();
     __syncthreads();
     tc_fence_after();
     bool ok = M.tmem == 0 && (smem_u32(sm) & 1023) == 0;  // (all columns: they begin at 0)
@@ -670,17 +671,19 @@ cudaError_t start(const LaCore& p, LaLists* shared, cudaStream_t stream) {
         e = la_prepare(p, grid, blocks, {true, false, 0, 0.3f, 2.f}, shared != nullptr, lists, stream);
         if (e != cudaSuccess) return e;
         if (lists.split) {
-            states<<<grid, kThreads, kStates, stream>>>(p, &lists.plan->states, lists.states,
-                                                        lists.slots, vec);
-            la_scan_states(p, lists, stream);
+            e = la_launch_next(states, grid, kThreads, kStates, stream, p, &lists.plan->states,
+                               lists.states, lists.slots, vec);
+            if (e == cudaSuccess) e = la_scan_states(p, lists, stream);
         }
     }
     const int64_t jobs = static_cast<int64_t>(p.n_seqs) * p.heads * blocks;
-    full<<<lists.plan != nullptr ? grid : static_cast<int>(jobs), kThreads, kFull, stream>>>(
-        p, lists.plan != nullptr ? &lists.plan->main[lists.uses] : nullptr, lists.main, lists.slots,
-        vec);
+    if (e == cudaSuccess && lists.plan != nullptr)
+        e = la_launch_next(full, grid, kThreads, kFull, stream, p, &lists.plan->main[lists.uses],
+                           lists.main, lists.slots, vec);
+    else if (e == cudaSuccess)
+        full<<<static_cast<int>(jobs), kThreads, kFull, stream>>>(p, nullptr, nullptr, nullptr, vec);
     ++lists.uses;
-    e = cudaGetLastError();
+    if (e == cudaSuccess) e = cudaGetLastError();
     const cudaError_t f = la_release(own, stream);
     return e != cudaSuccess ? e : f;
 }

@@ -85,6 +85,7 @@ la_plan(const LaCore p, LaPlan* plan, LaEntry* main, LaEntry* states, LaSplit* s
     __shared__ float cost[32];
     __shared__ int counts[kPlanThreads];  // the first sequences' chunks
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    after_last_kernel();
     auto chunks = [&](int s, int64_t& start, int64_t& len) {
         int64_t end;
         la_span(p, s, start, end);
@@ -221,6 +222,7 @@ la_plan(const LaCore p, LaPlan* plan, LaEntry* main, LaEntry* states, LaSplit* s
 template <int kVec>
 __global__ void __launch_bounds__(256)
 la_scan(const LaCore p, const LaPlan* plan, const LaSplit* splits, float* scratch) {
+    after_last_kernel();
     const int size = p.d_b * p.d_c, tiles = (size + 256 * kVec - 1) / (256 * kVec);
     const int64_t jobs = static_cast<int64_t>(plan->splits) * p.heads * tiles;
     for (int64_t job = blockIdx.x; job < jobs; job += gridDim.x) {
@@ -326,9 +328,9 @@ cudaError_t la_prepare(const LaCore& p, int grid, int blocks, LaSplitCost o, boo
     return cudaGetLastError();
 }
 
-void la_scan_states(const LaCore& p, const LaLists& lists, cudaStream_t stream) {
-    auto* kernel = p.d_c % 4 == 0 ? la_scan<4> : la_scan<1>;
-    kernel<<<4 * la_sm_count(), 256, 0, stream>>>(p, lists.plan, lists.splits, lists.slots);
+cudaError_t la_scan_states(const LaCore& p, const LaLists& lists, cudaStream_t stream) {
+    return la_launch_next(p.d_c % 4 == 0 ? la_scan<4> : la_scan<1>, 4 * la_sm_count(), 256, 0, stream,
+                          p, lists.plan, lists.splits, lists.slots);
 }
 
 cudaError_t la_release(const LaLists& lists, cudaStream_t stream) {

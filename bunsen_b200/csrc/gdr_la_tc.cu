@@ -298,6 +298,7 @@ la_tc(const LaCore p, const __grid_constant__ CUtensorMap ma,
         tmem_relinquish();
     }
     tc_fence_before();
+    after_last_kernel();
     __syncthreads();
     tc_fence_after();
     bool ok = true;  // false: a wait ran out, and its role with it
@@ -1017,17 +1018,20 @@ cudaError_t launch_la_tc(const LaCore& p, bool split, bool must, int forced, cud
         e = la_prepare(p, sms, 1, {split, must, forced, 0.45f, 11.f}, shared != nullptr, lists, stream);
         if (e != cudaSuccess) return e;
         if (lists.split) {
-            states<<<sms, kThreads, kSmemBytes, stream>>>(p, ma, mb, mc, mo, &lists.plan->states,
-                                                          lists.states, lists.slots);
-            la_scan_states(p, lists, stream);
+            e = la_launch_next(states, sms, kThreads, static_cast<int>(kSmemBytes), stream, p, ma, mb,
+                               mc, mo, &lists.plan->states, lists.states, lists.slots);
+            if (e == cudaSuccess) e = la_scan_states(p, lists, stream);
         }
     }
     const int64_t jobs = static_cast<int64_t>(p.n_seqs) * p.heads;
-    full<<<lists.plan != nullptr ? sms : static_cast<int>(jobs), kThreads, kSmemBytes, stream>>>(
-        p, ma, mb, mc, mo, lists.plan != nullptr ? &lists.plan->main[lists.uses] : nullptr,
-        lists.main, lists.slots);
+    if (e == cudaSuccess && lists.plan != nullptr)
+        e = la_launch_next(full, sms, kThreads, static_cast<int>(kSmemBytes), stream, p, ma, mb, mc,
+                           mo, &lists.plan->main[lists.uses], lists.main, lists.slots);
+    else if (e == cudaSuccess)
+        full<<<static_cast<int>(jobs), kThreads, kSmemBytes, stream>>>(p, ma, mb, mc, mo, nullptr,
+                                                                       nullptr, nullptr);
     ++lists.uses;
-    e = cudaGetLastError();
+    if (e == cudaSuccess) e = cudaGetLastError();
     const cudaError_t f = la_release(own, stream);
     return e != cudaSuccess ? e : f;
 }
