@@ -64,12 +64,13 @@ struct LaLists;
 // Kernels of the core (each its own file) and what they take.
 cudaError_t launch_la_recurrent(const LaCore& p, cudaStream_t stream);
 bool la_parts_supports(const LaCore& p);
-cudaError_t launch_la_parts(const LaCore& p, cudaStream_t stream, LaLists* shared = nullptr);
+cudaError_t launch_la_parts(const LaCore& p, cudaStream_t stream, LaLists* shared, bool chained);
 bool la_tc_supports(const LaCore& p);
 // split: long sequences may go in segments (scratch from the library's pool);
 // must: they do even where it looks slower; forced: segment length in chunks, or 0.
+// chained: the stream's last kernel is one of this call's that lets the next one in.
 cudaError_t launch_la_tc(const LaCore& p, bool split, bool must, int forced, cudaStream_t stream,
-                         LaLists* shared = nullptr);
+                         LaLists* shared, bool chained);
 cudaError_t take_la_error(int* flag);
 constexpr int kLaMaxD = 256;  // d_k, d_v of any kernel here
 

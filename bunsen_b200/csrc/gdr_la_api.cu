@@ -1,6 +1,7 @@
 // The entry points of include/gdr.h for the decayed linear attention and for
 // the head norms with rotation: argument checks, then the kernels.
 #include <cmath>
+#include <type_traits>
 
 #include "gdr_la.cuh"
 #include "gdr_la_plan.cuh"
@@ -23,6 +24,7 @@ template <typename T>
 __global__ void __launch_bounds__(256)
 sum_group(const float* __restrict__ part, T* __restrict__ out, int heads_qk, int group, int d,
           int64_t tokens, const int32_t* cu, int n_seqs) {
+    after_last_kernel();
     int64_t first = 0, last = tokens;
     if (cu != nullptr) {
         first = cu[0] < 0 ? 0 : cu[0];
@@ -44,20 +46,16 @@ cudaError_t launch_sum_group(int dtype, const float* part, void* out, int heads_
                              cudaStream_t s) {
     const int64_t want = (tokens * heads_qk * d + 255) / 256;
     const int blocks = static_cast<int>(want < 148 * 16 ? want : 148 * 16);
+    auto go = [&](auto* to) {
+        using T = std::remove_pointer_t<decltype(to)>;
+        return la_launch_next(sum_group<T>, blocks, 256, 0, s, part, to, heads_qk, group, d, tokens, cu,
+                              n_seqs);
+    };
     switch (dtype) {
-        case GDR_DTYPE_BF16:
-            sum_group<<<blocks, 256, 0, s>>>(part, static_cast<__nv_bfloat16*>(out), heads_qk,
-                                             group, d, tokens, cu, n_seqs);
-            break;
-        case GDR_DTYPE_F16:
-            sum_group<<<blocks, 256, 0, s>>>(part, static_cast<__half*>(out), heads_qk, group, d,
-                                             tokens, cu, n_seqs);
-            break;
-        default:
-            sum_group<<<blocks, 256, 0, s>>>(part, static_cast<float*>(out), heads_qk, group, d,
-                                             tokens, cu, n_seqs);
+        case GDR_DTYPE_BF16: return go(static_cast<__nv_bfloat16*>(out));
+        case GDR_DTYPE_F16: return go(static_cast<__half*>(out));
+        default: return go(static_cast<float*>(out));
     }
-    return cudaGetLastError();
 }
 
 gdr_status check_la(const gdr_la_params* params, const int32_t* cu_seqlens) {
@@ -120,13 +118,13 @@ Kernel kernel_of(const gdr_la_params& a, const LaCore& p, bool chunked) {
 }
 
 cudaError_t run_core(const gdr_la_params& a, const LaCore& p, bool chunked, cudaStream_t s,
-                     LaLists* shared = nullptr) {
+                     LaLists* shared = nullptr, bool chained = false) {
     switch (kernel_of(a, p, chunked)) {
         case Kernel::none: return cudaErrorNotSupported;
         case Kernel::tensor:
             return launch_la_tc(p, a.algo != GDR_ALGO_TENSOR, a.algo == GDR_ALGO_TENSOR_SPLIT,
-                                a.split_chunks, s, shared);
-        case Kernel::parts: return launch_la_parts(p, s, shared);
+                                a.split_chunks, s, shared, chained);
+        case Kernel::parts: return launch_la_parts(p, s, shared, chained);
         default: return launch_la_recurrent(p, s);
     }
 }
@@ -246,7 +244,7 @@ gdr_status gdr_la_backward(const gdr_la_params* params, const void* q, const voi
     const cudaError_t r = la_release(lists, s);
     if (e == cudaSuccess) e = r;
     if (e == cudaSuccess && tokens > 0) {
-        e = run_core(a, q_core, true, s);
+        e = run_core(a, q_core, true, s, nullptr, true);
         if (e == cudaSuccess) e = sum(dq);
     }
     if (part != nullptr) {

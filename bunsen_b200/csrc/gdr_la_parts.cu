@@ -651,7 +651,7 @@ la_parts(const LaCore p, LaWork* work, const LaEntry* entries, float* scratch, b
 }
 
 template <typename T, int kDb, bool kRev>
-cudaError_t start(const LaCore& p, LaLists* shared, cudaStream_t stream) {
+cudaError_t start(const LaCore& p, LaLists* shared, bool chained, cudaStream_t stream) {
     auto* full = la_parts<T, kDb, kRev, false>;
     auto* states = la_parts<T, kDb, kRev, true>;
     constexpr int kFull = static_cast<int>(Layout<T, kDb, false>::kBytes),
@@ -668,7 +668,8 @@ cudaError_t start(const LaCore& p, LaLists* shared, cudaStream_t stream) {
     LaLists own;
     LaLists& lists = shared != nullptr ? *shared : own;
     if (lists.uses == 0) {
-        e = la_prepare(p, grid, blocks, {true, false, 0, 0.3f, 2.f}, shared != nullptr, lists, stream);
+        e = la_prepare(p, grid, blocks, {true, false, 0, 0.3f, 2.f}, shared != nullptr, chained, lists,
+                       stream);
         if (e != cudaSuccess) return e;
         if (lists.split) {
             e = la_launch_next(states, grid, kThreads, kStates, stream, p, &lists.plan->states,
@@ -689,10 +690,10 @@ cudaError_t start(const LaCore& p, LaLists* shared, cudaStream_t stream) {
 }
 
 template <typename T>
-cudaError_t pick(const LaCore& p, LaLists* shared, cudaStream_t stream) {
+cudaError_t pick(const LaCore& p, LaLists* shared, bool chained, cudaStream_t stream) {
     if (p.d_b <= 64)
-        return p.reverse ? start<T, 64, true>(p, shared, stream) : start<T, 64, false>(p, shared, stream);
-    return p.reverse ? start<T, 128, true>(p, shared, stream) : start<T, 128, false>(p, shared, stream);
+        return (p.reverse ? start<T, 64, true> : start<T, 64, false>)(p, shared, chained, stream);
+    return (p.reverse ? start<T, 128, true> : start<T, 128, false>)(p, shared, chained, stream);
 }
 
 }  // namespace
@@ -702,11 +703,11 @@ bool la_parts_supports(const LaCore& p) {
            static_cast<int64_t>(p.n_seqs) * p.heads < (int64_t{1} << 28);
 }
 
-cudaError_t launch_la_parts(const LaCore& p, cudaStream_t stream, LaLists* shared) {
+cudaError_t launch_la_parts(const LaCore& p, cudaStream_t stream, LaLists* shared, bool chained) {
     switch (p.dtype) {
-        case GDR_DTYPE_BF16: return pick<__nv_bfloat16>(p, shared, stream);
-        case GDR_DTYPE_F16: return pick<__half>(p, shared, stream);
-        default: return pick<float>(p, shared, stream);
+        case GDR_DTYPE_BF16: return pick<__nv_bfloat16>(p, shared, chained, stream);
+        case GDR_DTYPE_F16: return pick<__half>(p, shared, chained, stream);
+        default: return pick<float>(p, shared, chained, stream);
     }
 }
 

@@ -274,7 +274,7 @@ int la_sm_count() {
 }
 
 cudaError_t la_prepare(const LaCore& p, int grid, int blocks, LaSplitCost o, bool shared,
-                       LaLists& out, cudaStream_t stream) {
+                       bool chained, LaLists& out, cudaStream_t stream) {
     if (shared) {  // two passes over the segments for one that finds their states
         o.state_cost *= 0.5f;
         o.fixed_cost *= 0.5f;
@@ -322,9 +322,12 @@ cudaError_t la_prepare(const LaCore& p, int grid, int blocks, LaSplitCost o, boo
     out.splits = reinterpret_cast<LaSplit*>(at + o_splits);
     out.slots = reinterpret_cast<float*>(at + o_slots);
     out.split = split;
-    la_plan<<<1, kPlanThreads, 0, stream>>>(p, out.plan, out.main, out.states, out.splits,
-                                            reinterpret_cast<int32_t*>(at + o_base), grid, blocks,
-                                            l_min, static_cast<int>(cap), o);
+    int32_t* base = reinterpret_cast<int32_t*>(at + o_base);
+    if (chained)
+        return la_launch_next(la_plan, 1, kPlanThreads, 0, stream, p, out.plan, out.main, out.states,
+                              out.splits, base, grid, blocks, l_min, static_cast<int>(cap), o);
+    la_plan<<<1, kPlanThreads, 0, stream>>>(p, out.plan, out.main, out.states, out.splits, base, grid,
+                                            blocks, l_min, static_cast<int>(cap), o);
     return cudaGetLastError();
 }
 

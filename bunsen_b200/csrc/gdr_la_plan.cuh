@@ -85,7 +85,7 @@ struct LaLists {
 // grid: CTAs of the persistent kernels; blocks: jobs of each (entry, head); shared: two
 // launches will use the lists.
 cudaError_t la_prepare(const LaCore& p, int grid, int blocks, LaSplitCost o, bool shared,
-                       LaLists& lists, cudaStream_t stream);
+                       bool chained, LaLists& lists, cudaStream_t stream);
 cudaError_t la_scan_states(const LaCore& p, const LaLists& lists, cudaStream_t stream);
 cudaError_t la_release(const LaLists& lists, cudaStream_t stream);
 int la_sm_count();

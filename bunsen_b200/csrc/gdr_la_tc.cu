@@ -994,7 +994,7 @@ bool la_tc_supports(const LaCore& p) {
 }
 
 cudaError_t launch_la_tc(const LaCore& p, bool split, bool must, int forced, cudaStream_t stream,
-                         LaLists* shared) {
+                         LaLists* shared, bool chained) {
     CUtensorMap ma, mb, mc, mo;
     const int64_t tokens = la_tokens(p);
     if (!tile_map(&ma, p.a, tokens, p.heads_a, p.d_b, kC) ||
@@ -1015,7 +1015,8 @@ cudaError_t launch_la_tc(const LaCore& p, bool split, bool must, int forced, cud
     LaLists own;
     LaLists& lists = shared != nullptr ? *shared : own;
     if (lists.uses == 0) {
-        e = la_prepare(p, sms, 1, {split, must, forced, 0.45f, 11.f}, shared != nullptr, lists, stream);
+        e = la_prepare(p, sms, 1, {split, must, forced, 0.45f, 11.f}, shared != nullptr, chained,
+                       lists, stream);
         if (e != cudaSuccess) return e;
         if (lists.split) {
             e = la_launch_next(states, sms, kThreads, static_cast<int>(kSmemBytes), stream, p, ma, mb,
