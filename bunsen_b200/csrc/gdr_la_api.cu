@@ -110,9 +110,11 @@ Kernel kernel_of(const gdr_la_params& a, const LaCore& p, bool chunked) {
     // scores would be most of some outputs); the others go in chunks.
     const bool few = tokens <= 16 || tokens <= 4 * static_cast<int64_t>(p.n_seqs);
     if (few && a.algo < GDR_ALGO_TENSOR) return Kernel::recurrent;
-    // Nor does a prompt of a chunk or less gain from bf16 scores and states: 12 us in parts,
-    // 10 us with them, and half their error in the sums.
-    const bool exact = tokens <= 64 && a.algo == GDR_ALGO_AUTO && la_parts_supports(p);
+    // Nor do prompts of a chunk or less, where every sequence and head has an SM, gain from
+    // bf16 scores and states: 12 us in parts, 10 us with them, and half their error in the
+    // sums. (Several an SM do: 12 sequences of 64 heads 61 us against 40.)
+    const bool exact = tokens <= 64 && a.algo == GDR_ALGO_AUTO && la_parts_supports(p) &&
+                       static_cast<int64_t>(p.n_seqs) * p.heads <= la_sm_count();
     if (tc && a.algo != GDR_ALGO_CUDA_CORE && !exact) return Kernel::tensor;
     return la_parts_supports(p) ? Kernel::parts : Kernel::recurrent;
 }

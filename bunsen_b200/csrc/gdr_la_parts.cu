@@ -35,7 +35,7 @@
 // of 64.
 //
 // Bound: 5000 tensor cycles a chunk at f32 and 128 x 128, 2.9 us, where a chunk takes 5.8 us
-// (8192 packed positions, 16 heads, d = 128: 186 us; with mma.sync in three tf32 products and
+// (8192 packed positions, 16 heads, d = 128: 182 us; with mma.sync in three tf32 products and
 // shared memory alone 988 us): issue slots, 0.67 of them taken by conversions and the address
 // work around them, in a chain with the products.
 #include <cuda_fp16.h>

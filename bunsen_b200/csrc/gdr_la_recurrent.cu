@@ -14,7 +14,7 @@
 // (a warp reads whole 512-byte state rows) when that fills the GPU, else 32
 // columns, four times the CTAs with a quarter of the loads each, for the
 // latency of small batches. 256 rows of 32 heads, d = 128: 164 us, 6.6 TB/s, the copy
-// rate; one row 5 us on the device.
+// rate; one row 3 us on the device.
 #include "gdr_la.cuh"
 
 namespace gdr {

@@ -49,7 +49,7 @@
 // Bound: HBM, at 128 x (768 to 1024) bytes a chunk and head (q and k shared or not),
 // 2.2 to 3.0 us per SM at the measured copy rate; six products are 3100 tensor cycles, 1.8 us;
 // shared memory moves 480 KiB a chunk, 3800 cycles. A chunk takes 3.7 us (131072
-// packed positions, 32 heads: 830 us, 4.2 TB/s, 0.64 of the copy rate): the chains between
+// packed positions, 32 heads: 837 us, 4.2 TB/s, 0.64 of the copy rate): the chains between
 // the roles, 250 cycles from a commit to the waiting warp's next instruction, are what is
 // left. The states' pass takes 2 us a chunk.
 #include <cudaTypedefs.h>

@@ -556,3 +556,29 @@ def test_calls_from_threads():
         t.join()
     assert not bad
     assert _lib.load().gdr_device_error() == _lib.GDR_OK
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_offsets_past_32_bits(dtype):
+    """A tensor of more than 2^31 elements: the sequence at its end equals the
+    same one alone, and agrees with its steps: in bf16 to the two outputs' own
+    roundings and the chunk's operands' (3 x 2^-8 of the largest), else to f32
+    sums of (200 + 128 + 64) terms (2^-23 each: 5e-5)."""
+    t, tail, hv, d = 270000, 200, 64, 128
+    assert (t - tail) * hv * d > 2**31
+    gen = torch.Generator(device=DEV).manual_seed(2)
+    v = torch.empty(t, hv, d, device=DEV, dtype=dtype).normal_(generator=gen)
+    q, k = (torch.empty(t, 1, d, device=DEV, dtype=dtype).normal_(generator=gen) for _ in range(2))
+    g = -0.2 * torch.rand(hv, device=DEV, generator=gen)
+    cu = torch.tensor([0, t - tail, t], dtype=torch.int32, device=DEV)
+    rule = LinearAttention()
+    out, state = rule.chunked(q, k, v, g, cu_seqlens=cu)
+    one = torch.tensor([0, tail], dtype=torch.int32, device=DEV)
+    want, s_want = rule.chunked(q[-tail:], k[-tail:], v[-tail:], g, cu_seqlens=one)
+    assert torch.equal(out[-tail:], want) and torch.equal(state[1:], s_want)
+    step, s_step = rule.recurrent(q, k, v, g, cu_seqlens=cu[1:])
+    tol = 2.0**-6 if dtype == torch.bfloat16 else 1e-4
+    assert float((step[-tail:].float() - want.float()).abs().max()) <= \
+        tol * float(want.float().abs().max())
+    assert float((s_step - s_want).abs().max()) <= 1e-4 * float(s_want.abs().max())
+    assert _lib.load().gdr_device_error() == _lib.GDR_OK
