@@ -239,9 +239,6 @@ __device__ __forceinline__ void take_registers() {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegs));
 }
 
-// Heads whose decay's powers to w^-128 are far from overflow (e^51).
-__device__ __forceinline__ bool is_gentle(float g) { return g >= -0.4f && g <= 0.4f; }
-
 // Chunk c of an item, in the order they run: its length, and its first row.
 template <bool kRev>
 __device__ __forceinline__ int chunk_len(const Job& it, int nch, int c) {
@@ -550,12 +547,11 @@ la_tc(const LaCore p, const __grid_constant__ CUtensorMap ma,
     } else if (warp < 8) {
         if constexpr (kStateOnly) give_registers<24>();
         // ---- scores and outputs -------------------------------------------------------
-        // Where w^-128 is far from overflow, the powers come out of the sums:
-        //   out_i = tau w^{i+1} [ a_i . S + sum_{j<=i} sigma w^{-(j+1)} (a_i.b_j) c_j ]
-        // (backward w^{len-1-i} and w^{-(len-1-j)}): one column factor on the
-        // scores, one row factor on the output, the inter product untouched. Each row's
-        // terms keep their ratios, so no bits are lost. Steeper heads scale scores by
-        // w^{i-j} and the inter product by rows, a pass over O more.
+        // Scores are scaled by w^{i-j} and the inter product, before P C is added to it, by
+        // rows: a pass over O, but every factor is at most 1, so nothing overflows that
+        // the result does not. (With the powers out of the sums, w^{-(j+1)} on the scores'
+        // columns and w^{i+1} on O's rows at its end, scores above 2e16 did at a log decay of
+        // -0.4; the 131072 packed positions took 814 us so, 852 us now.)
         // A block's 32 column factors run from the largest exponent down by
         // products with w^2 in registers: a table in shared memory waits there
         // behind the tensor cores' operands.
@@ -574,32 +570,28 @@ la_tc(const LaCore p, const __grid_constant__ CUtensorMap ma,
             if (it.len < 0) break;
             const int nch = (it.len + kC - 1) / kC;
             const float g = p.log_decay[it.h], w = la_power(g, 1);
-            const bool gentle = is_gentle(g);
             const uint64_t step = pair(w * w, w * w);
             const float w16 = la_power(g, 16);
-            // Steep, the diagonal block's second half.
+            // Of the diagonal block, its half that is farther from the diagonal.
             const float steep = p.sigma * p.tau * la_power(g, kRev ? max(16 - lane, 0)
                                                                 : max(lane - 15, 0));
-            float ahead = 0.f, fb[2];  // O's row factor; the blocks' first column factors
-            int known = 0;             // the chunk length they are for
+            // Off the diagonal block: w^{i-j} splits in two exponents that are not
+            // negative, rows' and columns'; the blocks' first column factors.
+            const float edge = p.sigma * p.tau * la_power(g, kRev ? 32 - lane : lane + 1);
+            float fb[2];
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                const int cb = 2 * half + x, apart = kRev ? cb - quarter : quarter - cb;
+                fb[x] = edge * la_power(g, 32 * (apart - 1));
+            }
+            float ahead = 0.f;  // O's row factor
+            int known = 0;      // the chunk length it is for
 #pragma unroll 1
             for (int c = 0; c < nch; ++c, ++n) {
                 const uint32_t st = n & 1, ph = n & 1, ph2 = (n >> 1) & 1;
                 const int len = chunk_len<kRev>(it, nch, c);
                 if (len != known) {
                     ahead = p.tau * la_power(g, kRev ? max(len - 1 - i, 0) : i + 1);
-                    // Steep, off the diagonal block: w^{i-j} splits in two
-                    // exponents that are not negative, rows' and columns'.
-                    const float edge = p.sigma * p.tau * la_power(g, kRev ? 32 - lane : lane + 1);
-#pragma unroll
-                    for (int x = 0; x < 2; ++x) {
-                        const int cb = 2 * half + x;
-                        const int e = kRev ? len - 1 - 32 * cb : 32 * cb + 32;
-                        const int apart = kRev ? cb - quarter : quarter - cb;
-                        fb[x] = (gentle ? p.sigma : edge) *
-                                la_power(gentle && e >= 0 ? -g : g,
-                                      gentle ? abs(e) : 32 * (apart - 1));
-                    }
                     known = len;
                 }
                 if (!(ok = warp_wait(&B.sc_full, ph))) break;
@@ -616,7 +608,7 @@ la_tc(const LaCore p, const __grid_constant__ CUtensorMap ma,
                         // The powers run from the larger exponents' side of either half.
                         const bool far = kRev ? hb == 1 : hb == 0;
                         const int me = lane - 16 * hb;  // this row's column in the half, if diag
-                        if (gentle || !diag) {
+                        if (!diag) {
                             float f = x == 0 ? fb[0] : fb[1];
                             if (far) f *= w16;
                             uint64_t f2 = kRev ? pair(f, f * w) : pair(f * w, f);
@@ -657,18 +649,16 @@ la_tc(const LaCore p, const __grid_constant__ CUtensorMap ma,
 #pragma unroll 1
                 for (int cb = 2 * half; cb < 2 * half + 2; ++cb)
                     if (cb < first || cb >= last) tmem_st16(pcol + 16 * (cb & 1), zero);
-                if (!gentle) {
-                    if (!(ok = warp_wait(&B.in_full[st], ph2))) break;
-                    tc_fence_after();
+                if (!(ok = warp_wait(&B.in_full[st], ph2))) break;
+                tc_fence_after();
 #pragma unroll 1
-                    for (int blk = 0; blk < 4; ++blk) {
-                        const uint32_t at = quad + kColO + 64 * half + 16 * blk;
-                        uint64_t o[8];
-                        tmem_ld16(at, o);
+                for (int blk = 0; blk < 4; ++blk) {
+                    const uint32_t at = quad + kColO + 64 * half + 16 * blk;
+                    uint64_t o[8];
+                    tmem_ld16(at, o);
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) o[j] = mul2(o[j], pair(ahead, ahead));
-                        tmem_st16(at, o);
-                    }
+                    for (int j = 0; j < 8; ++j) o[j] = mul2(o[j], pair(ahead, ahead));
+                    tmem_st16(at, o);
                 }
                 if (!(ok = warp_wait(&B.c_full[st], ph2))) break;
                 tmem_wait_st();
@@ -676,12 +666,10 @@ la_tc(const LaCore p, const __grid_constant__ CUtensorMap ma,
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&B.pa_ready);
 
-                // The output: scaled, converted, staged where a was (f32: and c).
+                // The output: converted, staged where a was (f32: and c).
                 if (!(ok = warp_wait(&B.o_full[st], ph2))) break;
                 if (p.out_f32 && !(ok = warp_wait(&B.c_read[st], ph2))) break;
                 tc_fence_after();
-                const float last_factor = gentle ? ahead : 1.f;
-                const uint64_t scale = pair(last_factor, last_factor);
                 uint8_t* tile = sm + st * kStage;
 #pragma unroll 1
                 for (int blk = 0; blk < 4; ++blk) {
@@ -692,8 +680,6 @@ la_tc(const LaCore p, const __grid_constant__ CUtensorMap ma,
                         __syncwarp();
                         if (lane == 0) mbar_arrive(&B.o_free);
                     }
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) u[j] = mul2(u[j], scale);
                     if (p.out_f32) {
                         uint8_t* dst = staged(tile, 2 * half + (blk >> 1)) + i * 128;
 #pragma unroll
