@@ -250,8 +250,9 @@ norm_rope_vec(const NormRope p, uint32_t q_warps, float* part) {
                 }
                 const float r =
                     rsqrtf(fmaf(group_sum<G>(live ? sum_pair(ss) : 0.f), inv_d, p.eps));
+                // (Step by step: r^3 leaves f32 where r and the gradient do not.)
                 const float back =
-                    -group_sum<G>(live ? sum_pair(dot) : 0.f) * inv_d * (r * r * r);
+                    -group_sum<G>(live ? sum_pair(dot) : 0.f) * inv_d * r * r * r;
                 const float r_own = mine ? r : 0.f;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
@@ -333,7 +334,7 @@ norm_rope_any(const NormRope p, int64_t rows, float* part) {
             }
             if (kGrad) dot = fmaf(v[j] * wt(e), g[j], dot);
         }
-        const float back = kGrad ? warp_sum(dot) / p.d * (r * r) : 0.f;
+        const float back = kGrad ? warp_sum(dot) / p.d * r * r : 0.f;
 #pragma unroll
         for (int j = 0; j < kE; ++j) {
             const int e = lane + 32 * j;
