@@ -65,7 +65,7 @@ gdr_status check_la(const gdr_la_params* params, const int32_t* cu_seqlens) {
     if (a.d_k <= 0 || a.d_v <= 0 || a.seq_len < 0) return GDR_ERR_INVALID;
     if (a.dtype != GDR_DTYPE_F32 && a.dtype != GDR_DTYPE_BF16 && a.dtype != GDR_DTYPE_F16)
         return GDR_ERR_INVALID;
-    if (!std::isfinite(a.scale)) return GDR_ERR_INVALID;
+    if (!std::isfinite(static_cast<float>(a.scale))) return GDR_ERR_INVALID;  // as the kernels have it
     if ((cu_seqlens == nullptr ? a.batch : a.n_seqs) < 0) return GDR_ERR_INVALID;
     if (a.algo < GDR_ALGO_AUTO || a.algo > GDR_ALGO_TENSOR_SPLIT || a.split_chunks < 0)
         return GDR_ERR_INVALID;
@@ -271,7 +271,7 @@ gdr_status make_rope(const gdr_qk_norm_rope_params* params, const void* q, const
         return GDR_ERR_INVALID;
     if (a.dtype != GDR_DTYPE_F32 && a.dtype != GDR_DTYPE_BF16 && a.dtype != GDR_DTYPE_F16)
         return GDR_ERR_INVALID;
-    if (!(a.eps >= 0.0) || !std::isfinite(a.eps)) return GDR_ERR_INVALID;
+    if (!(a.eps >= 0.0) || !std::isfinite(static_cast<float>(a.eps))) return GDR_ERR_INVALID;
     if (a.head_dim > gdr::norm_rope_max_d()) return GDR_ERR_UNSUPPORTED;
     if (a.tokens >= (int64_t{1} << 31) ||
         a.tokens * (static_cast<int64_t>(a.heads_q) + a.heads_k) >= (int64_t{1} << 31))

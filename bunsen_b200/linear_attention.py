@@ -23,12 +23,13 @@ from __future__ import annotations
 
 import ctypes
 import dataclasses
-import math
 
 import torch
 
 from . import _lib
 from .rule import _ALGOS, _DTYPES, _ptr, on_device
+
+_F32_MAX = torch.finfo(torch.float32).max
 
 
 @dataclasses.dataclass(frozen=True)
@@ -117,8 +118,8 @@ class LinearAttention:
             if state.shape != (n, h_v, qs[-1], vs[-1]):
                 raise ValueError(f"the state is [N, H_v, d_k, d_v] = {(n, h_v, qs[-1], vs[-1])}; "
                                  f"got {tuple(state.shape)}")
-        if self.scale is not None and not math.isfinite(self.scale):
-            raise ValueError("scale is finite")
+        if self.scale is not None and not abs(self.scale) <= _F32_MAX:
+            raise ValueError("scale is finite in f32")
         if dev.type != "cuda":
             raise RuntimeError("libgdr runs on CUDA tensors only")
         _same_device(dev, k, v, log_decay, state)

@@ -147,3 +147,20 @@ def test_rope_entry_points_reject_bad_parameters(bad, status):
     lib, d, p = _lib.load(), ctypes.c_void_p(16), _lib.GdrQkNormRopeParams(**{**base, **bad})
     assert lib.gdr_qk_norm_rope(ctypes.byref(p), *[d] * 9, None) == status
     assert lib.gdr_qk_norm_rope_backward(ctypes.byref(p), *[d] * 13, None) == status
+
+
+@pytest.mark.parametrize("value", [1e39, -1e39])
+def test_scales_and_epsilons_beyond_f32_are_rejected(value):
+    """The kernels compute in f32: what is infinite there is not a finite scale."""
+    lib, d, p = _lib.load(), ctypes.c_void_p(16), _la(scale=value)
+    for fn in (lib.gdr_la_recurrent, lib.gdr_la_chunked):
+        assert fn(ctypes.byref(p), d, d, d, d, None, d, d, None, None) == _lib.GDR_ERR_INVALID
+    assert lib.gdr_la_backward(ctypes.byref(p), d, d, d, d, d, None, None, d, d, d, None, None,
+                               None) == _lib.GDR_ERR_INVALID
+    p = _lib.GdrQkNormRopeParams(tokens=3, q_token_stride=16, q_head_stride=8, k_token_stride=8,
+                                 k_head_stride=8, heads_q=2, heads_k=1, head_dim=8, rotary_dim=8,
+                                 table_rows=9, interleaved=0, dtype=_lib.GDR_DTYPE_BF16, eps=value)
+    assert lib.gdr_qk_norm_rope(ctypes.byref(p), *[d] * 9, None) == _lib.GDR_ERR_INVALID
+    assert lib.gdr_qk_norm_rope_backward(ctypes.byref(p), *[d] * 13, None) == _lib.GDR_ERR_INVALID
+    with pytest.raises(ValueError, match="finite"):
+        LinearAttention(scale=value).chunked(**OK)
