@@ -163,7 +163,7 @@ __device__ __forceinline__ void block_weights(const NormRope& p, float (*acc)[kM
 }
 
 // The outputs, or (kGrad) the gradients. A warp works on q or on k throughout (in
-// proportion to their heads; its weights stay in registers), a unit of kRows x
+// proportion to their units; its weights stay in registers), a unit of kRows x
 // (32 / G) heads of one token at a time, every load before the first use.
 // `q_warps` of all warps work on q. Rows past the last head are the last again,
 // not stored.
@@ -413,20 +413,19 @@ int lanes_of(const NormRope& p) { return p.d <= 64 ? 8 : p.d <= 128 ? 16 : 32; }
 // where that leaves SMs without work.
 int rows_of(const NormRope& p) {
     constexpr int rows = 4;
-    const int64_t units = p.tokens * (p.heads_q + p.heads_k) / (32 / lanes_of(p) * rows);
+    const int64_t units =
+        p.tokens * norm_rope_units(p.heads_q, p.heads_k, 32 / lanes_of(p) * rows);
     return units < 2 * kWarps * sm_count() ? 1 : rows;
 }
 
 Launch launch_of(const NormRope& p) {
-    const int64_t rows = p.tokens * (p.heads_q + p.heads_k);
     const int per = vectors(p) ? 32 / lanes_of(p) * rows_of(p) : 1;
-    const int64_t want = (rows / per + kWarps) / kWarps;
+    const int64_t units = p.tokens * norm_rope_units(p.heads_q, p.heads_k, per);
+    const int64_t want = (units + kWarps) / kWarps;
     const int64_t most = static_cast<int64_t>(sm_count()) * (p.dq_out != nullptr ? 2 : kWaves * 4);
     Launch l;
     l.blocks = static_cast<int>(want < 1 ? 1 : want < most ? want : most);
-    const int64_t warps = static_cast<int64_t>(l.blocks) * kWarps;
-    int64_t q = warps * p.heads_q / (p.heads_q + p.heads_k);
-    l.q_warps = static_cast<uint32_t>(q < 1 ? 1 : q > warps - 1 ? warps - 1 : q);
+    l.q_warps = norm_rope_q_warps(static_cast<int64_t>(l.blocks) * kWarps, p.heads_q, p.heads_k, per);
     return l;
 }
 
