@@ -36,6 +36,9 @@ struct LaCore {
     int32_t out_f32;
     int32_t dtype;              // of a, b, c
     int32_t scratch_t;          // states between segments are there as [d_c, d_b]
+    int32_t steps_most;         // a pack in two launches: sequences of at most so many
+                                // positions are the recurrent one's, longer ones the
+                                // chunked one's; -1: one launch takes them all
 };
 
 inline int64_t la_tokens(const LaCore& p) {

@@ -84,6 +84,7 @@ LaCore core_of(const gdr_la_params& a, const int32_t* cu_seqlens, const float* l
     p.heads = a.heads_v;
     p.log_decay = log_decay;
     p.dtype = a.dtype;
+    p.steps_most = -1;
     return p;
 }
 
@@ -99,7 +100,8 @@ void operands(LaCore& p, const void* x, int hx, const void* y, int hy, const voi
     p.d_c = d_c;
 }
 
-enum class Kernel { none, recurrent, tensor, parts };
+enum class Kernel { none, recurrent, tensor, parts, both };
+constexpr int kFewEach = 4;  // positions of a sequence that step as fast as their chunk runs
 
 Kernel kernel_of(const gdr_la_params& a, const LaCore& p, bool chunked) {
     const int64_t tokens = la_tokens(p);
@@ -107,9 +109,19 @@ Kernel kernel_of(const gdr_la_params& a, const LaCore& p, bool chunked) {
     const bool tc = la_tc_supports(p);
     if (!tc && a.algo >= GDR_ALGO_TENSOR) return Kernel::none;
     // A few positions step as fast as a chunk does, and in f32 (rounded to bf16, a chunk's few
-    // scores would be most of some outputs); the others go in chunks.
-    const bool few = tokens <= 16 || tokens <= 4 * static_cast<int64_t>(p.n_seqs);
-    if (few && a.algo < GDR_ALGO_TENSOR) return Kernel::recurrent;
+    // scores would be most of some outputs); the others go in chunks. The lengths of a pack
+    // are on the device: one with few positions a sequence on average may still hold a long
+    // one, whose steps, 0.7 to 1.3 us each, would bound the call. So such a pack goes to both
+    // kernels, each with the sequences that are its own, both at f32 accuracy: a prompt of
+    // 3000 between 1000 single positions, 32 heads of 128, 4420 us in steps, 887 so. The second
+    // kernel and its plan are 12 to 20 us where no sequence is theirs (256 single positions 181 and
+    // 194 us): up to 64 positions, where no walk takes 80 us, steps alone.
+    const bool few =
+        tokens <= 16 || tokens <= kFewEach * static_cast<int64_t>(p.n_seqs);  // on average
+    if (few && a.algo < GDR_ALGO_TENSOR) {
+        const bool mixed = p.cu_seqlens != nullptr && tokens > 64 && la_parts_supports(p);
+        return mixed ? Kernel::both : Kernel::recurrent;
+    }
     // Nor do prompts of a chunk or less, where every sequence and head has an SM, gain from
     // bf16 scores and states: 12 us in parts, 10 us with them, and half their error in the
     // sums. (Several an SM do: 12 sequences of 64 heads 61 us against 40.)
@@ -127,6 +139,12 @@ cudaError_t run_core(const gdr_la_params& a, const LaCore& p, bool chunked, cuda
             return launch_la_tc(p, a.algo != GDR_ALGO_TENSOR, a.algo == GDR_ALGO_TENSOR_SPLIT,
                                 a.split_chunks, s, shared, chained);
         case Kernel::parts: return launch_la_parts(p, s, shared, chained);
+        case Kernel::both: {
+            LaCore two = p;
+            two.steps_most = kFewEach;
+            const cudaError_t e = launch_la_recurrent(two, s);
+            return e != cudaSuccess ? e : launch_la_parts(two, s, shared, false);
+        }
         default: return launch_la_recurrent(p, s);
     }
 }
@@ -234,7 +252,7 @@ gdr_status gdr_la_backward(const gdr_la_params* params, const void* q, const voi
     };
     // dv and dk run over the same D: one of them finds its states between segments.
     const Kernel kernel = kernel_of(a, v_core, true);
-    const bool same = (kernel == Kernel::tensor || kernel == Kernel::parts) &&
+    const bool same = kernel != Kernel::none && kernel != Kernel::recurrent &&
                       kernel_of(a, k_core, true) == kernel && la_same_lists(v_core, k_core);
     LaLists lists;
     k_core.scratch_t = same;

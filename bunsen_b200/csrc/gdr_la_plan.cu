@@ -73,9 +73,9 @@ __device__ __forceinline__ bool in_place(const LaCore& p) {
     return p.state_in != nullptr && p.state_in == p.state_out;
 }
 
-// The work lists: every sequence, or its segments, the longest first (by buckets of
-// chunk counts), and the first pass's segments. seg_cap: state slots; 0: no
-// splitting. forced: a given segment length.
+// The work lists: every sequence of more than p.steps_most positions, or its segments, the
+// longest first (by buckets of chunk counts), and the first pass's segments. seg_cap: state
+// slots; 0: no splitting. forced: a given segment length.
 __global__ void __launch_bounds__(kPlanThreads)
 la_plan(const LaCore p, LaPlan* plan, LaEntry* main, LaEntry* states, LaSplit* splits, int32_t* base,
         int grid, int blocks, int l_min, int seg_cap, LaSplitCost how) {
@@ -90,6 +90,7 @@ la_plan(const LaCore p, LaPlan* plan, LaEntry* main, LaEntry* states, LaSplit* s
         int64_t end;
         la_span(p, s, start, end);
         len = end - start;
+        if (len <= p.steps_most) return -1;  // another launch's
         return static_cast<int>((len + kLaChunk - 1) / kLaChunk);
     };
     int64_t start, len;
@@ -98,13 +99,16 @@ la_plan(const LaCore p, LaPlan* plan, LaEntry* main, LaEntry* states, LaSplit* s
         int64_t x, y;
         return chunks(s, x, y);
     };
-    int sum = 0, most = 0;
+    int sum = 0, most = 0, listed = 0;
     for (int s = tid; s < p.n_seqs; s += kPlanThreads) {
         const int c = chunks(s, start, len);
         if (s < kPlanThreads) counts[s] = c;
+        if (c < 0) continue;
+        ++listed;
         sum += c;
         most = max(most, c);
     }
+    listed = block_reduce(listed, false, ws);
     sum = block_reduce(sum, false, ws);
     most = block_reduce(most, true, ws);
     // Candidate lengths from l_min to the longest sequence, one a warp.
@@ -156,6 +160,7 @@ la_plan(const LaCore p, LaPlan* plan, LaEntry* main, LaEntry* states, LaSplit* s
     auto bucket = [&](int c) { return kBuckets - 1 - (c >> shift); };  // longest first
     for (int s = tid; s < p.n_seqs; s += kPlanThreads) {
         const int c = count(s);
+        if (c < 0) continue;
         int parts = c > L ? (c + L - 1) / L : 1, at = 0;
         if (parts > 1) at = atomicAdd(&slots, parts);
         base[s] = at;
@@ -184,7 +189,7 @@ la_plan(const LaCore p, LaPlan* plan, LaEntry* main, LaEntry* states, LaSplit* s
     __syncthreads();
     for (int s = tid; s < p.n_seqs; s += kPlanThreads) {
         const int c = count(s);
-        if (c > L) continue;
+        if (c < 0 || c > L) continue;
         chunks(s, start, len);
         main[atomicAdd(&hist[bucket(c)], 1)] = {static_cast<int32_t>(start),
                                                 static_cast<int32_t>(len), s, s};
@@ -210,7 +215,7 @@ la_plan(const LaCore p, LaPlan* plan, LaEntry* main, LaEntry* states, LaSplit* s
     }
     __syncthreads();
     if (tid == 0) {
-        plan->main[0] = plan->main[1] = {p.n_seqs + slots - n_splits, grid};
+        plan->main[0] = plan->main[1] = {listed + slots - n_splits, grid};
         plan->states = {n_states, grid};
         plan->splits = n_splits;
         plan->seg_tokens = L * kLaChunk;
@@ -301,7 +306,8 @@ cudaError_t la_prepare(const LaCore& p, int grid, int blocks, LaSplitCost o, boo
             split = split_time(o, per, L, n * c, c, n * (parts - 1) * L, n * ((c + L / 3) / L), parts) < best;
         }
     }
-    if (!split && static_cast<int64_t>(p.n_seqs) * p.heads * blocks <= grid) return cudaSuccess;
+    if (!split && p.steps_most < 0 && static_cast<int64_t>(p.n_seqs) * p.heads * blocks <= grid)
+        return cudaSuccess;
     const size_t size = sizeof(float) * p.heads * p.d_b * p.d_c;
     // A split sequence of c > L chunks has ceil(c / L) < 2 c / L segments.
     const int64_t cap = split ? std::min<int64_t>(2 * most / l_min + 2, kStateBudget / size) : 0;

@@ -40,6 +40,7 @@ la_recurrent(const LaCore p) {
     const int col0 = static_cast<int>(blockIdx.z) * kSlab, col = col0 + li * kVec;
     int64_t t0, t1;
     la_span(p, s, t0, t1);
+    if (p.steps_most >= 0 && t1 - t0 > p.steps_most) return;
     const int64_t hs = (static_cast<int64_t>(s) * p.heads + h) * p.d_b * p.d_c;
     const int64_t rs = p.state_t ? 1 : p.d_c, cs = p.state_t ? p.d_b : 1;  // state strides
     // The decay in two parts: applied position after position, the rounding of
