@@ -124,3 +124,30 @@ def test_a_long_sequence_among_rows_is_not_walked():
         t.append(microseconds(lambda: LinearAttention().chunked(  # noqa: B023
             x["q"], x["k"], x["v"], x["g"], x["state"], cu_seqlens=x["cu"], out=out, state_out=s1)))
     assert t[0] <= 2 * (t[1] + t[2]), t
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("lens,packed", [
+    ([1], True), ([16], True), ([16], False), ([4, 4, 4, 4, 4], False), ([3, 1, 4, 4, 4, 4, 0], True),
+    ([64], True), ([64], False), ([20, 0, 44], True), ([32, 32], False), ([17], True)])
+def test_small_calls_at_f32_accuracy(lens, packed, dtype, strict):
+    """Few positions, and 64 or fewer where every sequence and head has an SM."""
+    x = make(lens, 2, 4, 128, 128, dtype, seed=sum(lens), packed=packed)
+    check_forward(x)
+    check_backward(x)
+
+
+@pytest.mark.parametrize("shape", [(33, 65), (1, 1), (5, 128), (128, 5), (60, 64), (160, 96),
+                                   (256, 256)])
+def test_other_widths_at_f32_accuracy(shape, strict):
+    """bf16 widths that the chunks with bf16 scores do not take."""
+    x = make([200, 1, 170], 1, 2, *shape, torch.bfloat16, seed=sum(shape))
+    check_forward(x)
+    check_backward(x)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_cuda_core_at_f32_accuracy(dtype, strict):
+    x = make([300, 0, 513, 64], 2, 4, 128, 128, dtype, seed=14)
+    check_forward(x, "cuda_core")
+    check_backward(x, "cuda_core")
