@@ -8,10 +8,11 @@
 namespace gdr {
 namespace sm100 {
 
-constexpr int kWaitRounds = 1 << 20;  // of two tries of a microsecond or less: two seconds
+constexpr int kWaitRounds = 1 << 20;  // of two tries of 90 cycles or more: a tenth of a second
 
 // Waits for a phase; false once the tries ran out. A try suspends the warp for
-// some 90 cycles (one with a time of its own becomes a loop of sleeps).
+// some 90 cycles (one with a time of its own becomes a loop of sleeps). One lane's answer:
+// a role leaves its loop as a warp, so it asks warp_wait.
 __device__ __forceinline__ bool lane_wait(uint64_t* bar, uint32_t parity) {
     uint32_t ok;
     asm volatile(

@@ -509,7 +509,7 @@ la_tc(const LaCore p, const __grid_constant__ CUtensorMap ma,
                     int64_t row;
                     int len;
                     chunk_of<kRev>(it, nch, c, row, len);
-                    if (!(ok = lane_wait(&B.o_staged[st], (n >> 1) & 1))) break;
+                    if (!(ok = warp_wait(&B.o_staged[st], (n >> 1) & 1))) break;
                     uint8_t* tile = sm + st * kStage;
                     // Boxes of 32 positions, 128 bytes of features each; the last rows one
                     // by one: behind them another sequence's stay as they are.
