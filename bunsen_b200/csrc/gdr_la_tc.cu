@@ -48,10 +48,11 @@
 //
 // Bound: HBM, at 128 x (768 to 1024) bytes a chunk and head (q and k shared or not),
 // 2.2 to 3.0 us per SM at the measured copy rate; six products are 3100 tensor cycles, 1.8 us;
-// shared memory moves 480 KiB a chunk, 3800 cycles. A chunk takes 3.7 us (131072
-// packed positions, 32 heads: 837 us, 4.2 TB/s, 0.64 of the copy rate): the chains between
-// the roles, 250 cycles from a commit to the waiting warp's next instruction, are what is
-// left. The states' pass takes 2 us a chunk.
+// shared memory moves 480 KiB a chunk, 3800 cycles. A chunk takes 3.8 us (131072
+// packed positions, 32 heads: 852 us, 4.1 TB/s, 0.63 of the copy rate, one call at a
+// time; 1049 us, 0.51, among other calls, at lower clocks): the chains between the roles,
+// 250 cycles from a commit to the waiting warp's next instruction, are what is left. The
+// states' pass takes 1.7 to 2 us a chunk.
 #include <cudaTypedefs.h>
 
 #include <algorithm>
@@ -995,8 +996,8 @@ cudaError_t launch_la_tc(const LaCore& p, bool split, bool must, int forced, cud
     if (e == cudaSuccess)
         e = la_allow_smem(states, static_cast<int>(kSmemBytes), done[p.reverse != 0][1]);
     if (e != cudaSuccess) return e;
-    // A chunk takes 2.9 us at one CTA an SM, one of the states' pass 0.45 of that; that
-    // pass's start, the list's kernel and the scan 11 chunks.
+    // In chunks of the main pass, 3.8 us: one of the states' pass 0.45; that pass's start, the
+    // list's kernel and the scan 11 (9 and 12 us the last two, cold).
     const int sms = la_sm_count();
     LaLists own;
     LaLists& lists = shared != nullptr ? *shared : own;

@@ -319,10 +319,21 @@ gdr_status gdr_mixed_noalloc(const gdr_params* params, const void* q, const void
  * positions behind the last sequence are neither read nor written. No output
  * may overlap an input, but `state_out` may be `state_in`.
  *
- * GDR_ALGO_AUTO takes the kernel: positions one by one where there are few, chunks with
- * bf16 scores and state operands for bf16 prompts (GDR_ALGO_TENSOR: not in segments,
- * GDR_ALGO_TENSOR_SPLIT: in segments), chunks at f32 accuracy for the rest
- * (GDR_ALGO_CUDA_CORE: these or one by one, whatever the type). */
+ * GDR_ALGO_AUTO takes the kernel:
+ * - positions one by one where there are few: 16 in all, or four a sequence (in a pack on
+ *   average; above 64 positions its longer sequences go in chunks at f32 accuracy);
+ * - chunks with bf16 scores and state operands for bf16 prompts of widths up to 128,
+ *   multiples of 8 (GDR_ALGO_TENSOR: not in segments, GDR_ALGO_TENSOR_SPLIT: in segments),
+ *   unless the call has 64 positions or fewer and an SM for every sequence and head. Outputs
+ *   are off by 2.3e-3 in the relative 2-norm, where their own rounding alone is 1.7e-3;
+ * - chunks at f32 accuracy for the rest of widths up to 128 (GDR_ALGO_CUDA_CORE: these or one
+ *   by one, whatever the type). d_v may be 256 in the forward call;
+ * - wider ones one by one, whatever the length, 0.6 to 1.3 us a position: the forward call and
+ *   dv where d_k is above 128, dk and dq where d_v is.
+ * Which it takes hangs on counts of the whole call, so a sequence's outputs may be rounded
+ * differently in another batch; equal calls give equal bits. A NaN or an infinity stays in its
+ * sequence; from its position on (chunked: its 128 positions), in the direction of the call,
+ * outputs may be NaN. */
 typedef struct gdr_la_params {
     int32_t batch;        /* B of a dense batch; ignored when cu_seqlens != NULL */
     int32_t seq_len;      /* T of a dense batch, or T_total of a packed one      */
