@@ -320,8 +320,8 @@ gdr_status gdr_mixed_noalloc(const gdr_params* params, const void* q, const void
  * may overlap an input, but `state_out` may be `state_in`.
  *
  * GDR_ALGO_AUTO takes the kernel:
- * - positions one by one where there are few: 16 in all, or four a sequence (in a pack on
- *   average; above 64 positions its longer sequences go in chunks at f32 accuracy);
+ * - positions one by one where there are few: 16 in all, or four a sequence (in a pack seq_len
+ *   over n_seqs; above 64 positions its longer sequences go in chunks at f32 accuracy);
  * - chunks with bf16 scores and state operands for bf16 prompts of widths up to 128,
  *   multiples of 8 (GDR_ALGO_TENSOR: not in segments, GDR_ALGO_TENSOR_SPLIT: in segments),
  *   unless the call has 64 positions or fewer and an SM for every sequence and head. Outputs
