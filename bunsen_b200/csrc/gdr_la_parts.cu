@@ -64,7 +64,10 @@ constexpr uint32_t kColSc = 0, kColO2 = 0, kColO1 = 64, kColU = 128, kColC = 256
 template <typename T, int kDb, bool kStateOnly>
 struct Layout {
     static constexpr int kIn = sizeof(T) == 4 ? 3 : std::is_same_v<T, __half> ? 2 : 1;
-    // P and the state's copy, and the parts' products: outputs of 16 bits need 16.
+    // P and the state's copy, and the parts' products: outputs of 16 bits need 16. Each is off by
+    // 2^-16 of itself at most, and so is each product of two parts left out: 2^-16 of the
+    // sums of absolute terms for bf16, three times that for f16, where rounding the output takes
+    // 2^-8 and 2^-11 of what has not cancelled.
     static constexpr int kPs = sizeof(T) == 4 ? 3 : 2;
     static constexpr int kHalves = kDb / 64;
     static constexpr uint32_t kTileAb = kHalves * kRows64, kTileS = kHalves * kRows128;

@@ -39,7 +39,8 @@ class LinearAttention:
     which kernels run ``chunked`` and ``backward``. ``"auto"`` runs bf16 prompts (widths up
     to 128) with the chunks' scores and a copy of the state rounded to bf16: outputs are off
     by 2.3e-3 (relative 2-norm; their own rounding is 1.7e-3), states by 3e-7. ``"cuda_core"``
-    computes them at f32 accuracy, as every other type and calls of few positions are. The
+    computes them as every other type and calls of few positions are, at f32 accuracy (of
+    16-bit types in chunks, scores and the state's copy to 2^-16 of their terms). The
     kernel hangs on the call's counts of positions, sequences and heads, so a sequence may be
     rounded differently in another batch."""
 

@@ -327,7 +327,9 @@ gdr_status gdr_mixed_noalloc(const gdr_params* params, const void* q, const void
  *   unless the call has 64 positions or fewer and an SM for every sequence and head. Outputs
  *   are off by 2.3e-3 in the relative 2-norm, where their own rounding alone is 1.7e-3;
  * - chunks at f32 accuracy for the rest of widths up to 128 (GDR_ALGO_CUDA_CORE: these or one
- *   by one, whatever the type). d_v may be 256 in the forward call;
+ *   by one, whatever the type). d_v may be 256 in the forward call. Where outputs have 16 bits,
+ *   so have the scores and the state's copy: off by 2^-16 (f16: 3 x 2^-16) of the sums of
+ *   absolute terms at most, far below the outputs' own rounding but where they cancel;
  * - wider ones one by one, whatever the length, 0.6 to 1.3 us a position: the forward call and
  *   dv where d_k is above 128, dk and dq where d_v is.
  * Which it takes hangs on counts of the whole call, so a sequence's outputs may be rounded

@@ -151,3 +151,22 @@ def test_cuda_core_at_f32_accuracy(dtype, strict):
     x = make([300, 0, 513, 64], 2, 4, 128, 128, dtype, seed=14)
     check_forward(x, "cuda_core")
     check_backward(x, "cuda_core")
+
+
+# Chunks of 16-bit types take scores and the state's copy in two bf16 parts, each off by at most
+# 2^-8 x 2^-8 of itself, on disjoint parts of an output. Operands of f16 are two parts
+# themselves: products leave out the second part of one with the second of the other, 2^-16
+# again, once in the scores and once in the outputs.
+PARTS = {torch.float32: 0.0, torch.bfloat16: 2.0**-16, torch.float16: 3 * 2.0**-16}
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", [(1, 3), (3, 1), (8, 8)])
+@pytest.mark.parametrize("lens", [[5, 0, 1, 2, 4] * 50, [5] * 100, [17] * 10 + [64]])
+def test_narrow_heads(lens, shape, dtype, monkeypatch):
+    """Sums of few terms, where nothing averages what a part leaves out."""
+    monkeypatch.setattr(base, "op_rounding", lambda x, algo: PARTS[x["q"].dtype])
+    g = [-0.01, -0.39, 0.0, -0.41, -5.0, -0.0001, -1.0, -50.0, 0.0, -0.01, -0.0001, float("-inf")]
+    x = make(lens, 3, 12, *shape, dtype, seed=len(lens), g=g)
+    check_forward(x, "cuda_core")
+    check_backward(x, "cuda_core")
